@@ -39,6 +39,14 @@ class L2Prefetch(ctypes.Structure):
     _fields_ = [("ptr", c_vp * 4), ("bytes", c_i64 * 4), ("count", c_i32), ("flags", c_i32)]
 
 
+class Q8CacheStruct(ctypes.Structure):
+    """accel_b200_q8_cache (include/accel_b200.h)."""
+
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp), ("seq_stride", c_i64),
+                ("head_stride", c_i64), ("scale_seq_stride", c_i64), ("scale_head_stride", c_i64), ("slots", c_i32),
+                ("kv_heads", c_i32), ("head_dim", c_i32), ("context", c_i32), ("block", c_i32)]
+
+
 class LlamaConfig(ctypes.Structure):
     """AccelLlamaConfig (include/accel_b200_llama.h)."""
 
@@ -48,6 +56,7 @@ class LlamaConfig(ctypes.Structure):
 
 P_plane = ctypes.POINTER(Q8Plane)
 P_ep = ctypes.POINTER(Epilogue)
+P_q8c = ctypes.POINTER(Q8CacheStruct)
 
 # name -> (restype, argtypes). Device pointers and streams travel as c_void_p.
 SIGNATURES = {
@@ -100,6 +109,15 @@ SIGNATURES = {
     "accel_b200_decode_attention_prefetch": (c_int, [c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp,
                                                      c_i32, c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp,
                                                      ctypes.POINTER(L2Prefetch), c_vp]),
+    "accel_b200_rope_append_q8": (c_int, [c_vp, c_i64, c_i64, P_q8c, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_vp, c_vp,
+                                          c_vp, c_i64, c_vp, c_vp]),
+    "accel_b200_cache_rows_q8": (c_int, [P_q8c, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp]),
+    "accel_b200_attention_decode_q8_workspace": (c_sz, [P_q8c, c_i64, c_i32, c_i32, c_i32]),
+    "accel_b200_attention_decode_q8": (c_int, [c_vp, c_i64, P_q8c, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_i64,
+                                               c_vp, c_sz, c_vp, c_vp]),
+    "accel_b200_attention_prefill_q8_workspace": (c_sz, [P_q8c, c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "accel_b200_attention_prefill_q8": (c_int, [c_vp, c_i64, P_q8c, c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32,
+                                                c_i32, c_i32, c_vp, c_i64, c_vp, c_sz, c_vp, c_vp]),
     "accel_b200_silu_mul_rows": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp]),
     "accel_b200_sample_rows": (c_int, [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_f32, c_vp, c_i32, c_vp]),
     "accel_b200_greedy_step": (c_int, [c_vp, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32,

@@ -1,0 +1,83 @@
+// The int8 key/value cache (accel_b200_q8_cache): host checks of its layout and
+// of the ragged row lists that name its sequences, and the device side of both.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "accel_b200.h"
+#include "common.cuh"
+
+namespace accel_b200 {
+
+// Whether n0 runs at stride s0 and, inside them, n1 runs at stride s1 of
+// `inner` elements each do not overlap, in either order.
+inline bool Disjoint(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t inner) {
+  if (n1 <= 1) return n0 <= 1 || s0 >= inner;
+  if (n0 <= 1) return s1 >= inner;
+  return (s1 >= inner && s0 / n1 >= s1) || (s0 >= inner && s1 / n0 >= s0);
+}
+
+// ACCEL_B200_OK, or EINVAL with a message that begins with `what`.
+inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
+  const std::string w(what);
+  if (c == nullptr || c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) {
+    return SetError(ACCEL_B200_EINVAL, w + ": the cache has a null plane");
+  }
+  if (c->head_dim != 64 && c->head_dim != 128) {
+    return SetError(ACCEL_B200_EINVAL, w + ": head_dim must be 64 or 128");
+  }
+  if (c->block != 32 && c->block != 64 && c->block != 128) {
+    return SetError(ACCEL_B200_EINVAL, w + ": block must be 32, 64 or 128 tokens");
+  }
+  if (c->slots <= 0 || c->kv_heads <= 0 || c->context <= 0) {
+    return SetError(ACCEL_B200_EINVAL, w + ": the cache has no slots, heads or context");
+  }
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 != 0 || c->seq_stride % 16 != 0 ||
+      c->head_stride % 16 != 0) {
+    return SetError(ACCEL_B200_EINVAL, w + ": cache rows must be 16-byte aligned");
+  }
+  if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) % 4 != 0) {
+    return SetError(ACCEL_B200_EINVAL, w + ": cache scales must be 4-byte aligned");
+  }
+  const int64_t run = static_cast<int64_t>(c->context) * c->head_dim;
+  const int64_t blocks = CeilDiv(c->context, c->block);
+  if (!Disjoint(c->slots, c->seq_stride, c->kv_heads, c->head_stride, run) ||
+      !Disjoint(c->slots, c->scale_seq_stride, c->kv_heads, c->scale_head_stride, blocks)) {
+    return SetError(ACCEL_B200_EINVAL, w + ": cache strides do not hold the context");
+  }
+  return ACCEL_B200_OK;
+}
+
+// The rows of one sequence of a ragged list: sequence b owns `count` rows from
+// `first` at positions pos0 + i. count 0: nothing to do, or not in bounds.
+struct RaggedRows {
+  const int32_t* first;
+  const int32_t* count;
+  const int32_t* pos0;
+  int32_t max_rows;
+  int64_t rows;  // rows of the buffers that first / count index
+};
+
+struct Run {
+  int64_t first;
+  int32_t count;
+  int32_t pos0;
+};
+
+// Sequence b's rows, all inside the buffers and the cache. One that does not
+// fit is empty here and, if `report`, noted in *status.
+__device__ __forceinline__ Run RunOf(const RaggedRows& r, int b, int32_t context, bool report, int32_t* status) {
+  Run run{r.first[b], r.count[b], r.pos0[b]};
+  if (run.pos0 < 0 || run.count <= 0) return Run{0, 0, 0};
+  if (run.count > r.max_rows || run.first < 0 || run.first + run.count > r.rows ||
+      static_cast<int64_t>(run.pos0) + run.count > context) {
+    if (report && status != nullptr) atomicOr(status, ACCEL_B200_STATUS_BAD_POSITION);
+    return Run{0, 0, 0};
+  }
+  return run;
+}
+
+}  // namespace accel_b200

@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._lib import P_i64, Epilogue, Q8Plane, check, load
+from ._lib import P_i64, Epilogue, Q8CacheStruct, Q8Plane, check, load
 
 ACT = {"none": 0, "relu": 1, "gelu": 2}
 
@@ -338,3 +338,173 @@ def attention_decode_workspace(batch, heads, kv_heads, max_len, chunk=64, device
     """A zeroed workspace for attention_decode (its counters start at zero)."""
     need = load().accel_b200_attention_decode_workspace(batch, heads, kv_heads, max_len, chunk)
     return torch.zeros(need, dtype=torch.uint8, device=device)
+
+
+class Q8Cache:
+    """An int8 key/value cache (accel_b200_q8_cache) over torch tensors: k and
+    v int8 [slots, kv_heads, context, head_dim] and their fp32 scales [slots,
+    kv_heads, ceil(context / block)], all on one CUDA device. The planes may be
+    views of larger ones as long as a (slot, head) run is contiguous."""
+
+    def __init__(self, k, v, k_scale, v_scale, block=64):
+        slots, kv_heads, context, head_dim = k.shape
+        blocks = -(-context // block)
+        for name, t, dtype, shape in (("k", k, torch.int8, k.shape), ("v", v, torch.int8, k.shape),
+                                      ("k_scale", k_scale, torch.float32, (slots, kv_heads, blocks)),
+                                      ("v_scale", v_scale, torch.float32, (slots, kv_heads, blocks))):
+            if t.dtype != dtype or tuple(t.shape) != tuple(shape) or t.device != k.device or not t.is_cuda:
+                raise ValueError(f"{name} must be {dtype} {tuple(shape)} on one CUDA device")
+        if k.stride() != v.stride() or k_scale.stride() != v_scale.stride():
+            raise ValueError("k and v (and their scales) must have the same strides")
+        if k.stride(3) != 1 or (k.stride(2) != head_dim and context > 1) or (k_scale.stride(2) != 1 and blocks > 1):
+            raise ValueError("a (slot, head) run of the cache must be contiguous")
+        self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
+        self.slots, self.kv_heads, self.context, self.head_dim = slots, kv_heads, context, head_dim
+        self.device = k.device
+        self.native = Q8CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0),
+                                    k.stride(1), k_scale.stride(0), k_scale.stride(1), slots, kv_heads, head_dim,
+                                    context, block)
+        self._ref = ctypes.byref(self.native)
+
+    @classmethod
+    def zeros(cls, slots, kv_heads, context, head_dim, block=64, device="cuda"):
+        planes = [torch.zeros(slots, kv_heads, context, head_dim, dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros(slots, kv_heads, -(-context // block), device=device) for _ in range(2)]
+        return cls(*planes, *scales, block)
+
+
+def _rows(name, t, device, width=None):
+    """The row stride of a 2-D fp32 tensor on `device`."""
+    if t.dtype != torch.float32 or t.dim() != 2 or t.device != device or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name} must be 2-D fp32 with contiguous rows on {device}")
+    if width is not None and t.shape[1] != width:
+        raise ValueError(f"{name} must have {width} columns")
+    # One row has no stride that matters (torch may report any).
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def _i32(device, n, **tensors):
+    for name, t in tensors.items():
+        if t is not None and (t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n or
+                              not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 vector of {n} on {device}")
+
+
+def _table(name, t, cache):
+    if (t.dtype != torch.float32 or t.device != cache.device or t.dim() != 2 or t.shape[0] < cache.context or
+            t.shape[1] != cache.head_dim or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous fp32 [context, head_dim] on {cache.device}")
+
+
+def _call(device, fn, *args):
+    """fn(*args, stream) with `device` current, on its current stream."""
+    if torch.cuda.current_device() == device.index:
+        check(fn(*args, _s()))
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _s()))
+
+
+def rope_append_q8(qkv, cache, first, count, pos0, heads, max_rows, cos_t, sin_t, q_out=None, status=None):
+    """Rope and quantising append: sequence b's rows first[b] .. + count[b] - 1
+    of qkv [rows, (heads + 2 kv_heads) * head_dim] at positions pos0[b] + i of
+    slot b (int32 device vectors; count[b] <= max_rows). Returns the roped
+    queries [rows, heads * head_dim] (q_out; rows of no sequence are left)."""
+    dev, d = cache.device, cache.head_dim
+    ld = _rows("qkv", qkv, dev, (heads + 2 * cache.kv_heads) * d)
+    rows, batch = qkv.shape[0], first.shape[0]
+    _i32(dev, batch, first=first, count=count, pos0=pos0)
+    _i32(dev, 1, status=status)
+    _table("cos_t", cos_t, cache)
+    _table("sin_t", sin_t, cache)
+    if q_out is None:
+        q_out = torch.zeros(rows, heads * d, dtype=torch.float32, device=dev)
+    q_ld = _rows("q_out", q_out, dev, heads * d)
+    if q_out.shape[0] != rows:
+        raise ValueError("q_out must have a row for each row of qkv")
+    _call(dev, load().accel_b200_rope_append_q8, _p(qkv), ld, rows, cache._ref, _p(first), _p(count), _p(pos0), batch,
+          max_rows, heads, _p(cos_t), _p(sin_t), _p(q_out), q_ld, _p(status))
+    return q_out
+
+
+def cache_rows_q8(cache, first, count, pos0, max_rows, k_out=None, v_out=None, status=None):
+    """Cache positions pos0[b] + i of slot b as fp32 into rows first[b] + i of
+    k_out and v_out [rows, kv_heads * head_dim] (either may be None)."""
+    dev = cache.device
+    _i32(dev, first.shape[0], first=first, count=count, pos0=pos0)
+    _i32(dev, 1, status=status)
+    given = [t for t in (k_out, v_out) if t is not None]
+    lds = [_rows("k_out / v_out", t, dev, cache.kv_heads * cache.head_dim) for t in given]
+    if not given or len({t.shape[0] for t in given}) != 1 or len(set(lds)) != 1:
+        raise ValueError("k_out and v_out must have the same rows and strides, and one must be given")
+    _call(dev, load().accel_b200_cache_rows_q8, cache._ref, _p(first), _p(count), _p(pos0), first.shape[0], max_rows,
+          _p(k_out), _p(v_out), lds[0], given[0].shape[0], _p(status))
+    return k_out, v_out
+
+
+def _attention_io(q, cache, heads, out):
+    dev, width = cache.device, heads * cache.head_dim
+    q_ld = _rows("q", q, dev, width)
+    if out is None:
+        out = torch.zeros(q.shape[0], width, dtype=torch.float32, device=dev)
+    out_ld = _rows("out", out, dev, width)
+    if out.shape[0] != q.shape[0]:
+        raise ValueError("out must have a row for each row of q")
+    return q_ld, out, out_ld
+
+
+def _bytes(name, ws, device):
+    if ws is not None and (ws.device != device or ws.dtype != torch.uint8 or not ws.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous uint8 tensor on {device}")
+
+
+def attention_decode_q8_workspace(cache, rows, heads, window=0, sinks=0):
+    """A zeroed workspace for attention_decode_q8 calls of these sizes (None:
+    none needed)."""
+    need = load().accel_b200_attention_decode_q8_workspace(cache._ref, rows, heads, window, sinks)
+    return torch.zeros(need, dtype=torch.uint8, device=cache.device) if need else None
+
+
+def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=0, out=None, workspace=None,
+                        status=None):
+    """Attention of roped query rows q [rows, heads * head_dim], row r at
+    position row_pos[r] of slot row_seq[r] (None: slot r), over an int8 cache.
+    window: how many of the last tokens a row sees (0: all); sinks: first
+    tokens it sees besides. Rows with row_pos < 0 are left."""
+    dev = cache.device
+    q_ld, out, out_ld = _attention_io(q, cache, heads, out)
+    _i32(dev, q.shape[0], row_pos=row_pos, row_seq=row_seq)
+    _i32(dev, 1, status=status)
+    if workspace is None:
+        workspace = attention_decode_q8_workspace(cache, q.shape[0], heads, window, sinks)
+    _bytes("workspace", workspace, dev)
+    _call(dev, load().accel_b200_attention_decode_q8, _p(q), q_ld, cache._ref, _p(row_seq), _p(row_pos), q.shape[0],
+          heads, window, sinks, _p(out), out_ld, _p(workspace), 0 if workspace is None else workspace.numel(),
+          _p(status))
+    return out
+
+
+def attention_prefill_q8_workspace(cache, batch, max_rows, heads, window=0, sinks=0):
+    """A zeroed workspace for attention_prefill_q8 calls of these sizes (None:
+    none needed)."""
+    need = load().accel_b200_attention_prefill_q8_workspace(cache._ref, batch, max_rows, heads, window, sinks)
+    return torch.zeros(need, dtype=torch.uint8, device=cache.device) if need else None
+
+
+def attention_prefill_q8(q, cache, first, count, pos0, heads, max_rows, window=0, sinks=0, out=None, workspace=None,
+                         status=None):
+    """Causal attention of sequence b's rows first[b] .. + count[b] - 1 of q
+    (roped) at positions pos0[b] + i over slot b of an int8 cache that holds
+    their keys and values. window and sinks as in attention_decode_q8."""
+    dev = cache.device
+    q_ld, out, out_ld = _attention_io(q, cache, heads, out)
+    batch = first.shape[0]
+    _i32(dev, batch, first=first, count=count, pos0=pos0)
+    _i32(dev, 1, status=status)
+    if workspace is None:
+        workspace = attention_prefill_q8_workspace(cache, batch, max_rows, heads, window, sinks)
+    _bytes("workspace", workspace, dev)
+    _call(dev, load().accel_b200_attention_prefill_q8, _p(q), q_ld, cache._ref, _p(first), _p(count), _p(pos0), batch,
+          max_rows, q.shape[0], heads, window, sinks, _p(out), out_ld, _p(workspace),
+          0 if workspace is None else workspace.numel(), _p(status))
+    return out

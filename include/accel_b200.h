@@ -46,7 +46,12 @@ enum { ACCEL_B200_ACT_NONE = 0, ACCEL_B200_ACT_RELU = 1, ACCEL_B200_ACT_GELU = 2
 
 /* Bits of a device status word written by kernels that validate data or
    that gave up a bounded wait. */
-enum { ACCEL_B200_STATUS_BAD_TOKEN = 1, ACCEL_B200_STATUS_COPY_TIMEOUT = 2 };
+enum {
+  ACCEL_B200_STATUS_BAD_TOKEN = 1,
+  ACCEL_B200_STATUS_COPY_TIMEOUT = 2,
+  ACCEL_B200_STATUS_BAD_POSITION = 4, /* rows, a position or a slot outside the buffers or the cache */
+  ACCEL_B200_STATUS_NONFINITE = 8     /* an infinity or NaN was quantised */
+};
 
 ACCEL_B200_API const char* accel_b200_last_error(void);
 /* Number of kernel launches this library has issued in this process
@@ -434,6 +439,112 @@ ACCEL_B200_API int accel_b200_decode_attention_prefetch(
     int32_t kv_heads, int32_t head_dim, const float* cos_table, const float* sin_table, int32_t context,
     float* k_cache, float* v_cache, int64_t seq_stride, int64_t head_stride, float* out, int64_t out_ld,
     int32_t* status, const accel_b200_l2_prefetch* prefetch, void* stream);
+
+/* ------------------------------------------------------ int8 key/value cache
+   A cache with 8-bit keys and values and one fp32 scale per block of tokens
+   and kv head, its write, its read-back, and attention over it. No reference
+   counterpart (the reference's cache is fp32, src/llama_model.cc:259-270): an
+   addition of this backend, for four times the context or sequences per GPU.
+
+   Element (slot s, kv head g, position t, dim d) is k[s * seq_stride + g *
+   head_stride + t * head_dim + d] and stands for that integer times
+   k_scale[s * scale_seq_stride + g * scale_head_stride + t / block]; v the
+   same. The planes are 16-byte aligned with strides that are multiples of
+   16, the scales 4-byte aligned; no two (slot, head) runs overlap, in either
+   order of slots and heads. head_dim is 64 or 128, block 32, 64 or 128 tokens.
+   Device memory of the current device throughout. */
+typedef struct accel_b200_q8_cache {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t seq_stride;
+  int64_t head_stride;
+  int64_t scale_seq_stride;
+  int64_t scale_head_stride;
+  int32_t slots;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t context;
+  int32_t block;
+} accel_b200_q8_cache;
+
+/* RoPE and append with quantisation. Sequence b < batch owns fused projection
+   rows first[b] .. first[b] + count[b] - 1 of qkv (device arrays; rows as in
+   accel_b200_rope_append, `rows` of them in all, max_rows >= every count) at
+   positions pos0[b] + i of slot b. The roped queries go to q_out (row stride
+   q_ld; qkv itself with qkv_ld rotates in place, any other overlap is not
+   allowed), roped keys and values to the cache.
+
+   Block by block of a (slot, head) plane: amax is the largest finite |x| of
+   the new rows, `need` the least power of two >= 2^-126 with amax <= 127 *
+   need. The block keeps its scale if it holds rows before pos0 and 127 *
+   scale >= amax; otherwise its scale becomes `need`, and rows it holds before
+   pos0 are requantised to rint(q * old / need). New elements are rint(x /
+   scale), clamped to +-127. Rows of the block at or behind pos0 + count hold
+   nothing afterwards. Powers of two make x / scale and the stored value
+   exact, and bound the error of a block that grows step by step: each
+   requantising adds at most half a step of its scale, and every later scale
+   is at least twice that, so the sum stays under one step of the last.
+
+   The roped values are accel_b200_rope_append's. A NaN is stored as 0 and an
+   infinity as +-127, and ACCEL_B200_STATUS_NONFINITE is ORed into *status
+   (device int; may be NULL). A sequence with pos0 < 0 or count <= 0 is
+   skipped; one whose rows or positions do not fit (count > max_rows, rows
+   outside [0, rows), pos0 + count > context) is skipped with
+   ACCEL_B200_STATUS_BAD_POSITION. Rows are 16-byte aligned. */
+ACCEL_B200_API int accel_b200_rope_append_q8(const float* qkv, int64_t qkv_ld, int64_t rows,
+                                             const accel_b200_q8_cache* cache, const int32_t* first,
+                                             const int32_t* count, const int32_t* pos0, int32_t batch,
+                                             int32_t max_rows, int32_t heads, const float* cos_table,
+                                             const float* sin_table, float* q_out, int64_t q_ld, int32_t* status,
+                                             void* stream);
+
+/* Reads cache rows back as fp32: position pos0[b] + i of slot b to row
+   first[b] + i of k_out and v_out (either may be NULL; kv_heads * head_dim
+   floats per row, row stride out_ld, `rows` rows), i < count[b]. Exact.
+   Sequences are skipped as by accel_b200_rope_append_q8. */
+ACCEL_B200_API int accel_b200_cache_rows_q8(const accel_b200_q8_cache* cache, const int32_t* first,
+                                            const int32_t* count, const int32_t* pos0, int32_t batch,
+                                            int32_t max_rows, float* k_out, float* v_out, int64_t out_ld,
+                                            int64_t rows, int32_t* status, void* stream);
+
+/* Attention of single rows over an int8 cache: row r (roped queries q + r *
+   q_ld, heads * head_dim floats) at position row_pos[r] of slot row_seq[r]
+   (row_seq may be NULL: slot r) sees position t when t <= row_pos[r] and
+   either window is 0, t > row_pos[r] - window, or t < sinks. out row r =
+   softmax(q . k / sqrt(head_dim)) v. Several rows may name one slot. Rows with
+   row_pos[r] < 0 are skipped (their output is not written); a position or
+   slot outside the cache is skipped with ACCEL_B200_STATUS_BAD_POSITION.
+   heads is any multiple of kv_heads; rows are 16-byte aligned. The result
+   does not depend on how the work is split between calls of the same sizes.
+   The workspace holds accel_b200_attention_decode_q8_workspace(...) bytes (0:
+   none) whose first 64 KiB are zero before the first call, as for the
+   products; every call leaves them zero. Calls that share it must not overlap
+   on the GPU. */
+ACCEL_B200_API size_t accel_b200_attention_decode_q8_workspace(const accel_b200_q8_cache* cache, int64_t rows,
+                                                               int32_t heads, int32_t window, int32_t sinks);
+ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
+                                                  const int32_t* row_seq, const int32_t* row_pos, int64_t rows,
+                                                  int32_t heads, int32_t window, int32_t sinks, float* out,
+                                                  int64_t out_ld, void* workspace, size_t workspace_bytes,
+                                                  int32_t* status, void* stream);
+
+/* The same attention for many rows of each sequence: rows first[b] ..
+   first[b] + count[b] - 1 of q and out (`rows` of them in all, max_rows >=
+   every count) at positions pos0[b] + i of slot b; the cache already holds
+   their keys and values. Sequences are skipped as by
+   accel_b200_rope_append_q8 (a skipped sequence's output is not written).
+   Workspace as above. */
+ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200_q8_cache* cache, int32_t batch,
+                                                                int32_t max_rows, int32_t heads, int32_t window,
+                                                                int32_t sinks);
+ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
+                                                   const int32_t* first, const int32_t* count, const int32_t* pos0,
+                                                   int32_t batch, int32_t max_rows, int64_t rows, int32_t heads,
+                                                   int32_t window, int32_t sinks, float* out, int64_t out_ld,
+                                                   void* workspace, size_t workspace_bytes, int32_t* status,
+                                                   void* stream);
 
 /* SiluMul (src/sim_silu.cc:8-13) over fused rows [gate (inter) | up (inter)]
    of row stride ld into out[r, i] (row stride ldo). */

@@ -1,0 +1,131 @@
+"""The int8 key/value cache's entry points refuse what they cannot do, before
+they touch the device (none is needed here), and the Python mirror of the
+cache's struct agrees with the header."""
+
+import ctypes
+import subprocess
+
+import pytest
+import torch
+
+from accelep_b200 import kernels as K
+from accelep_b200._lib import Q8CacheStruct
+from tests.conftest import ROOT
+
+P = 1 << 20  # an aligned address that is never read
+
+
+def cache(**change):
+    d = {"k": P, "v": P, "k_scale": P, "v_scale": P, "seq_stride": 2 * 100 * 64, "head_stride": 100 * 64,
+         "scale_seq_stride": 4, "scale_head_stride": 2, "slots": 3, "kv_heads": 2, "head_dim": 64, "context": 100,
+         "block": 64}
+    d.update(change)
+    return ctypes.byref(Q8CacheStruct(*[d[name] for name, _ in Q8CacheStruct._fields_]))
+
+
+BAD_CACHES = [{"k": None}, {"v_scale": None}, {"head_dim": 96}, {"head_dim": 32}, {"block": 16}, {"block": 0},
+              {"block": 48}, {"slots": 0}, {"kv_heads": 0}, {"context": 0}, {"k": P + 8}, {"v_scale": P + 2},
+              {"head_stride": 99 * 64}, {"seq_stride": 100 * 64}, {"seq_stride": 2 * 100 * 64 + 8},
+              {"scale_head_stride": 1}, {"scale_seq_stride": 3}, {"head_stride": -100 * 64}]
+
+
+def append(lib, c, **change):
+    d = {"qkv": P, "ld": 8 * 64, "rows": 5, "first": P, "count": P, "pos0": P, "batch": 3, "max_rows": 4, "heads": 4,
+         "cos": P, "sin": P, "q": P, "q_ld": 4 * 64}
+    d.update(change)
+    return lib.accel_b200_rope_append_q8(d["qkv"], d["ld"], d["rows"], c, d["first"], d["count"], d["pos0"],
+                                         d["batch"], d["max_rows"], d["heads"], d["cos"], d["sin"], d["q"], d["q_ld"],
+                                         None, None)
+
+
+def read(lib, c, **change):
+    d = {"first": P, "count": P, "pos0": P, "batch": 3, "max_rows": 4, "k": P, "v": P, "ld": 128, "rows": 5}
+    d.update(change)
+    return lib.accel_b200_cache_rows_q8(c, d["first"], d["count"], d["pos0"], d["batch"], d["max_rows"], d["k"],
+                                        d["v"], d["ld"], d["rows"], None, None)
+
+
+def decode(lib, c, **change):
+    d = {"q": P, "ld": 256, "seq": None, "pos": P, "rows": 3, "heads": 4, "window": 0, "sinks": 0, "out": P,
+         "out_ld": 256}
+    d.update(change)
+    return lib.accel_b200_attention_decode_q8(d["q"], d["ld"], c, d["seq"], d["pos"], d["rows"], d["heads"],
+                                              d["window"], d["sinks"], d["out"], d["out_ld"], None, 0, None, None)
+
+
+def prefill(lib, c, **change):
+    d = {"q": P, "ld": 256, "first": P, "count": P, "pos0": P, "batch": 3, "max_rows": 4, "rows": 5, "heads": 4,
+         "window": 0, "sinks": 0, "out": P, "out_ld": 256}
+    d.update(change)
+    return lib.accel_b200_attention_prefill_q8(d["q"], d["ld"], c, d["first"], d["count"], d["pos0"], d["batch"],
+                                               d["max_rows"], d["rows"], d["heads"], d["window"], d["sinks"],
+                                               d["out"], d["out_ld"], None, 0, None, None)
+
+
+@pytest.mark.parametrize("change", BAD_CACHES, ids=str)
+@pytest.mark.parametrize("call", [append, read, decode, prefill])
+def test_bad_caches_are_refused(lib, call, change):
+    assert call(lib, cache(**change)) == 1
+    assert lib.accel_b200_last_error()
+    assert call(lib, None) == 1
+
+
+@pytest.mark.parametrize("call,change", [
+    (append, {"qkv": None}), (append, {"q": None}), (append, {"pos0": None}), (append, {"cos": None}),
+    (append, {"rows": -1}), (append, {"batch": -1}), (append, {"batch": 4}), (append, {"heads": 3}),
+    (append, {"heads": 0}), (append, {"ld": 7 * 64}), (append, {"q_ld": 4 * 64 - 4}), (append, {"ld": 8 * 64 + 2}),
+    (append, {"qkv": P + 4}), (append, {"q": P + 8}), (append, {"max_rows": -1}),
+    (read, {"first": None}), (read, {"batch": 4}), (read, {"ld": 124}), (read, {"ld": 130}), (read, {"k": P + 4}),
+    (read, {"rows": -2}),
+    (decode, {"q": None}), (decode, {"pos": None}), (decode, {"rows": 4}), (decode, {"rows": -1}),
+    (decode, {"rows": 65536, "seq": P}), (decode, {"heads": 5}), (decode, {"window": -1}), (decode, {"sinks": -1}),
+    (decode, {"ld": 252}), (decode, {"out_ld": 258}), (decode, {"out": P + 4}),
+    (prefill, {"count": None}), (prefill, {"batch": 4}), (prefill, {"heads": 6 + 1}), (prefill, {"window": -5}),
+    (prefill, {"out": None}), (prefill, {"rows": -1}), (prefill, {"out_ld": 128}),
+], ids=str)
+def test_bad_arguments_are_refused(lib, call, change):
+    assert call(lib, cache(), **change) == 1
+    assert lib.accel_b200_last_error()
+
+
+def test_empty_calls_queue_nothing(lib):
+    before = lib.accel_b200_launch_count()
+    for empty in ({"batch": 0}, {"max_rows": 0}, {"rows": 0}):
+        assert append(lib, cache(), **empty) == 0
+        assert read(lib, cache(), **empty) == 0
+        assert prefill(lib, cache(), **empty) == 0
+    assert read(lib, cache(), k=None, v=None) == 0
+    assert decode(lib, cache(), rows=0) == 0
+    assert lib.accel_b200_launch_count() == before
+
+
+@pytest.mark.parametrize("order", [
+    {"seq_stride": 100 * 64, "head_stride": 3 * 100 * 64, "scale_seq_stride": 2, "scale_head_stride": 6},  # heads outside
+    {"slots": 1, "seq_stride": 0, "scale_seq_stride": 0},       # one slot: its stride is never used
+    {"kv_heads": 1, "head_stride": 0, "scale_head_stride": 0},  # one head: the same
+])
+def test_other_orders_of_the_cache_are_taken(lib, order):
+    batch = {"batch": min(3, order.get("slots", 3)), "max_rows": 0}
+    assert append(lib, cache(**order), **batch) == 0
+    assert prefill(lib, cache(**order), **batch) == 0
+
+
+def test_struct_layout_matches_the_header(tmp_path):
+    lines = ['#include <stddef.h>', '#include <stdio.h>', '#include "accel_b200.h"', "int main(void) {",
+             '  printf("size %zu\\n", sizeof(accel_b200_q8_cache));']
+    lines += [f'  printf("{f} %zu\\n", offsetof(accel_b200_q8_cache, {f}));' for f, _ in Q8CacheStruct._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["  return 0;", "}"]) + "\n")
+    subprocess.run(["gcc", "-std=c11", f"-I{ROOT / 'include'}", "-I/usr/local/cuda/include", str(src), "-o", str(exe)],
+                   check=True, capture_output=True, text=True)
+    for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines():
+        name, value = line.split()
+        want = ctypes.sizeof(Q8CacheStruct) if name == "size" else getattr(Q8CacheStruct, name).offset
+        assert int(value) == want, name
+
+
+def test_python_cache_refuses_host_tensors():
+    k = torch.zeros(1, 1, 8, 64, dtype=torch.int8)
+    s = torch.zeros(1, 1, 1)
+    with pytest.raises(ValueError):
+        K.Q8Cache(k, k.clone(), s, s.clone())

@@ -2,16 +2,39 @@
 // cache"), causal, with an optional sliding window and first tokens (sinks)
 // that stay visible: of single rows and of many rows per sequence.
 //
-// The row at position p sees [0, min(sinks, first)) and [first, p], where
-// first = max(0, p - window + 1), or 0 without a window. One CTA takes one
-// row and query head; each warp walks every fourth visible position with an
-// online softmax (running maximum, sum and weighted values in fp32), and the
-// warps' states are merged once.
+// Scores and weighted values run on the tensor cores (mma.sync m16n8k16, fp16
+// operands, fp32 sums) without giving up fp32 results: an int8 key or value is
+// an exact fp16 number, and a query or a weight is the sum of two fp16 numbers
+// (22 bits), whose products with it are exact in fp32. The two parts of 8
+// vectors (query rows x heads that share a kv head) are the 16 rows of one
+// MMA operand, so the pair costs no more than 16 single-precision-less vectors
+// would. Queries are scaled by a power of two to 2^13 and weights to about
+// 2^10, so their second parts stay far above fp16's smallest step.
+//
+// Work split. A warp owns 8 vectors and walks units of 32 tokens, straight from
+// global memory to registers: which lane holds which dimension or token of a
+// sum is free to choose, and is chosen so that a lane's share of an MMA operand
+// is a contiguous run of bytes of the cache and the scores' register layout is
+// the weights' operand layout. No shared memory and no barrier in the loop.
+// Units are dealt to all warps of the S CTAs of a vector group in turn; the
+// next unit's keys load while this one's values are used, and the other way
+// round. Each unit's weighted values are summed on their own and added, times
+// the unit's value scale, to fp32 registers (the tensor core's running sum
+// rounds towards zero, which would drift over a long context).
+//
+// Online softmax in base 2 against a reference that moves only when a score
+// passes it by more than kSlack (a vote; no weight above 2^(kBias + kSlack)).
+// The warps' states merge in shared memory, the CTAs' through distributed
+// shared memory when they are one cluster (S <= 8), else through the
+// workspace by the last CTA to arrive; always in index order, so the result
+// does not depend on scheduling.
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
 #include "accel_b200.h"
+#include "cluster.cuh"
 #include "common.cuh"
 #include "q8_cache.cuh"
 
@@ -20,6 +43,12 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
+constexpr int kUnit = 32;      // tokens per step of a warp
+constexpr int kVec = 8;        // query vectors of a CTA
+constexpr int kMaxCluster = 8; // CTAs whose states merge through distributed shared memory
+constexpr float kSlack = 4.f;  // how far (in powers of two) a score may pass the softmax reference before it moves
+constexpr float kBias = 10.f;  // weights are 2^(score - reference + kBias)
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
   const float* q;
@@ -35,89 +64,476 @@ struct AttnArgs {
   float* out;
   int64_t out_ld;
   int32_t* status;
+  int32_t* counters;  // S > kMaxCluster: arrivals by vector group, then the CTAs' states
+  float* parts;
 };
 
+__device__ __forceinline__ void Mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float Exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 or 8 bytes of the cache, which is read once: not kept in L1.
+__device__ __forceinline__ uint4 LoadStream16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 LoadStream8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// Bytes 0 and 1 (kHi: 2 and 3) of w, each an int8 plus 128, as two fp16
+// numbers: 0x6400 | byte is 1024 + byte, less 1152.
+template <bool kHi>
+__device__ __forceinline__ uint32_t Halves(uint32_t w) {
+  const uint32_t x = __byte_perm(w, 0x64646464u, kHi ? 0x4342 : 0x4140);
+  const uint32_t k1152 = 0x64806480u;
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&k1152));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// (x, y) as fp16 pairs hi + lo, each off by at most 2^-22 of its value.
+__device__ __forceinline__ void SplitPair(float x, float y, uint32_t* hi, uint32_t* lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  *lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// First position that a window ending at pos covers.
+__device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
+
+// The softmax state of a CTA: reference, sum and weighted values of its vectors.
 template <int D>
-__device__ void AttendRow(const AttnArgs& a, int64_t row, int64_t slot, int64_t pos, int h) {
-  constexpr int kE = D / 32;  // elements of a row per lane
+struct alignas(16) State {
+  float m[kVec], l[kVec];
+  float o[kVec][D];
+};
+
+// Grid (split, kv head x vector group, sequence or row). kRuns: a sequence's
+// rows (prefill), else single rows.
+template <int D, bool kRuns>
+__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel(AttnArgs a) {
+  constexpr int kKw = D / 16;      // 32-bit words of a lane's share of a key row
+  constexpr int kTiles = D / 8;    // 8-dimension tiles of the output
+  constexpr int kVw = D / 32;      // words of a lane's share of a value row
+  __shared__ State<D> warp_state[kWarps];
+  __shared__ State<D> cta_state;
+  __shared__ bool last;
+  PdlTrigger();
+  PdlWait();
   const accel_b200_q8_cache& c = a.cache;
-  __shared__ float sm[kWarps], sl[kWarps], so[kWarps][D];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = h / (a.heads / c.kv_heads);
-  const int8_t* kp = c.k + slot * c.seq_stride + g * c.head_stride;
-  const int8_t* vp = c.v + slot * c.seq_stride + g * c.head_stride;
-  const float* ks = c.k_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
-  const float* vs = c.v_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
-  float q[kE], o[kE], m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < kE; ++e) {
-    q[e] = a.q[row * a.q_ld + static_cast<int64_t>(h) * D + lane * kE + e];
-    o[e] = 0.f;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
+  const int S = static_cast<int>(gridDim.x), split = static_cast<int>(blockIdx.x);
+  const int G = a.heads / c.kv_heads;
+  const int g = static_cast<int>(blockIdx.y) % c.kv_heads, group = static_cast<int>(blockIdx.y) / c.kv_heads;
+  const bool reports = split == 0 && blockIdx.y == 0 && tid == 0;
+
+  // The rows: `count` from `first` at positions pos0 + i of `slot`.
+  int64_t first, slot;
+  int count, pos0;
+  if (kRuns) {
+    slot = blockIdx.z;
+    const Run run = RunOf(a.rows, static_cast<int>(slot), c.context, reports, a.status);
+    first = run.first;
+    count = run.count;
+    pos0 = run.pos0;
+  } else {
+    first = blockIdx.z;
+    pos0 = a.row_pos[first];
+    slot = a.row_seq != nullptr ? a.row_seq[first] : first;
+    count = pos0 >= 0 ? 1 : 0;
+    if (count > 0 && (pos0 >= c.context || slot < 0 || slot >= c.slots)) {
+      if (reports && a.status != nullptr) atomicOr(a.status, ACCEL_B200_STATUS_BAD_POSITION);
+      count = 0;
+    }
   }
-  const int64_t near = a.window > 0 ? Max64(0, pos + 1 - a.window) : 0;
-  const int64_t sinks = Min64(a.sinks, near), seen = sinks + pos + 1 - near;
-  for (int64_t i = warp; i < seen; i += kWarps) {
-    const int64_t t = i < sinks ? i : near + (i - sinks);
-    float s = 0.f;
+  // Vectors v0 .. v0 + 7 of the run's count * G (row v / G, head v % G). A
+  // whole cluster leaves here or none of it.
+  const int64_t v0 = static_cast<int64_t>(group) * kVec, vectors = static_cast<int64_t>(count) * G;
+  if (v0 >= vectors) return;
+  const int row_lo = static_cast<int>(v0 / G);
+  const int row_hi = static_cast<int>(Min64(v0 + kVec - 1, vectors - 1) / G);
+  const bool mine = v0 + gid < vectors;
+  const int my_row = mine ? static_cast<int>((v0 + gid) / G) : row_hi;
+  const int my_pos = pos0 + my_row, my_near = NearOf(my_pos, a.window);
+  const int pos_lo = pos0 + row_lo, pos_hi = pos0 + row_hi;
+  const int near_lo = NearOf(pos_lo, a.window), near_hi = NearOf(pos_hi, a.window);
+
+  // Units that some vector sees: sinks before the windows, then the windows.
+  const int unit0 = near_lo / kUnit;
+  const int sink_units = min((a.sinks + 0ll + kUnit - 1) / kUnit, static_cast<long long>(unit0));
+  const int units = sink_units + pos_hi / kUnit - unit0 + 1;
+  const int step = S * kWarps;
+
+  const int8_t* kp = c.k + slot * c.seq_stride + g * c.head_stride + tig * 16;
+  const int8_t* vp = c.v + slot * c.seq_stride + g * c.head_stride + gid * (D / 8);
+  const float* ksp = c.k_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
+  const float* vsp = c.v_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
+  const int per_block = c.block / kUnit;
+
+  // Keys: tile i's token gid, D / 4 bytes (dimensions 16 tig .. + 15, and 64 +
+  // the same). Values: for each half of the unit, tokens 2 tig, 2 tig + 1, 2
+  // tig + 8, 2 tig + 9, bytes gid * D / 8 on. Rows are clamped to the context.
+  uint32_t kw[4][kKw], vw[2][4][kVw];
+  float ks = 0.f, vs = 0.f;
+  const auto unit_of = [&](int u) { return u < sink_units ? u : unit0 + (u - sink_units); };
+  const auto load_keys = [&](int u) {
+    const int t0 = unit_of(u) * kUnit;
+    ks = ksp[unit_of(u) / per_block];
 #pragma unroll
-    for (int e = 0; e < kE; ++e) s = fmaf(q[e], static_cast<float>(kp[t * D + lane * kE + e]), s);
-    s = WarpSum(s) * (a.scale * ks[t / c.block]);
-    const float mx = fmaxf(m, s);
-    const float corr = expf(m - mx), p = expf(s - mx);
-    m = mx;
-    l = l * corr + p;
-    const float pv = p * vs[t / c.block];
+    for (int i = 0; i < 4; ++i) {
+      const int8_t* p = kp + static_cast<int64_t>(min(t0 + 8 * i + gid, c.context - 1)) * D;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = fmaf(pv, static_cast<float>(vp[t * D + lane * kE + e]), o[e] * corr);
+      for (int w = 0; w < kKw / 4; ++w) {
+        const uint4 x = LoadStream16(p + 64 * w);
+        kw[i][4 * w] = x.x;
+        kw[i][4 * w + 1] = x.y;
+        kw[i][4 * w + 2] = x.z;
+        kw[i][4 * w + 3] = x.w;
+      }
+    }
+  };
+  const auto load_values = [&](int u) {
+    const int t0 = unit_of(u) * kUnit;
+    vs = vsp[unit_of(u) / per_block];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = t0 + 16 * h + 2 * tig + (r & 1) + 8 * (r >> 1);
+        const int8_t* p = vp + static_cast<int64_t>(min(t, c.context - 1)) * D;
+        if (D == 64) {
+          const uint2 x = LoadStream8(p);
+          vw[h][r][0] = x.x;
+          vw[h][r][1] = x.y;
+        } else {
+          const uint4 x = LoadStream16(p);
+          vw[h][r][0] = x.x;
+          vw[h][r][1] = x.y;
+          vw[h][r][kVw - 2] = x.z;
+          vw[h][r][kVw - 1] = x.w;
+        }
+      }
+    }
+  };
+  int u = split * kWarps + warp;
+  if (u < units) {
+    load_keys(u);
+    load_values(u);
   }
+
+  // This lane's share of its query vector, as the two fp16 parts of q * 2^e.
+  uint32_t qa[kKw][4];
+  float factor;  // raw sums to scores in base 2 (without the key scale)
+  {
+    float x[kKw][4];
+    uint32_t amax = 0;
+    const float* q = a.q + (first + my_row) * a.q_ld + static_cast<int64_t>(g * G + (v0 + gid) % G) * D + tig * 16;
 #pragma unroll
-  for (int e = 0; e < kE; ++e) so[warp][lane * kE + e] = o[e];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+    for (int j = 0; j < kKw; ++j) {
+      const float4 y = mine ? *reinterpret_cast<const float4*>(q + (j / 4) * 64 + (j % 4) * 4)
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[j][0] = y.x;
+      x[j][1] = y.y;
+      x[j][2] = y.z;
+      x[j][3] = y.w;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) amax = max(amax, __float_as_uint(x[j][k]) & 0x7fffffffu);
+    }
+    amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
+    amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
+    const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);  // the largest to 2^13 .. 2^14
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
+#pragma unroll
+    for (int j = 0; j < kKw; ++j) {
+      SplitPair(x[j][0] * up, x[j][1] * up, &qa[j][0], &qa[j][1]);
+      SplitPair(x[j][2] * up, x[j][3] * up, &qa[j][2], &qa[j][3]);
+    }
+  }
+
+  float m = -INFINITY, l = 0.f, o[kTiles][2];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = 0.f;
+
+  for (; u < units; u += step) {
+    const int t0 = unit_of(u) * kUnit;
+    // Scores: tile i holds tokens 8 i + 2 tig and + 1 of vector gid.
+    float s[4][2];
+    {
+      const float f = factor * ks;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kKw; ++j) {
+          const uint32_t w = kw[i][j] ^ 0x80808080u;
+          Mma16816(acc, qa[j], Halves<false>(w), Halves<true>(w));
+        }
+        s[i][0] = (acc[0] + acc[2]) * f;
+        s[i][1] = (acc[1] + acc[3]) * f;
+      }
+    }
+    if (u + step < units) load_keys(u + step);
+    // A unit that not every vector sees whole.
+    if (t0 + kUnit - 1 > pos_lo || (t0 < near_hi && t0 + kUnit > a.sinks)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int t = t0 + 8 * i + 2 * tig + k;
+          if (t > my_pos || (t < my_near && t >= a.sinks)) s[i][k] = -INFINITY;
+        }
+      }
+    }
+    float top = fmaxf(s[0][0], s[0][1]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) top = fmaxf(top, fmaxf(s[i][0], s[i][1]));
+    if (__any_sync(kFull, top > m + kSlack)) {
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+      const float now = fmaxf(m, top);
+      const float corr = now == -INFINITY ? 1.f : Exp2(m - now);
+      m = now;
+      l *= corr;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        o[i][0] *= corr;
+        o[i][1] *= corr;
+      }
+    }
+    // Weights, in the layout of an MMA operand. A vector that has seen nothing
+    // yet has scores of -inf alone.
+    const float ref = (m == -INFINITY ? 0.f : m) - kBias;
+    uint32_t pa[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float p0 = Exp2(s[2 * h][0] - ref), p1 = Exp2(s[2 * h][1] - ref);
+      const float p2 = Exp2(s[2 * h + 1][0] - ref), p3 = Exp2(s[2 * h + 1][1] - ref);
+      l += (p0 + p1) + (p2 + p3);
+      SplitPair(p0, p1, &pa[h][0], &pa[h][1]);
+      SplitPair(p2, p3, &pa[h][2], &pa[h][3]);
+    }
+    // Weighted values, four dimensions of this lane's run at a time.
+#pragma unroll
+    for (int w = 0; w < kVw; ++w) {
+      float acc[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[k][i] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t x[2], y[2];  // tokens (2 tig, + 1) and (2 tig + 8, + 9): dimensions 0 and 1, 2 and 3
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t w0 = vw[h][2 * r][w] ^ 0x80808080u, w1 = vw[h][2 * r + 1][w] ^ 0x80808080u;
+          x[r] = __byte_perm(w0, w1, 0x5140);
+          y[r] = __byte_perm(w0, w1, 0x7362);
+        }
+        Mma16816(acc[0], pa[h], Halves<false>(x[0]), Halves<false>(x[1]));
+        Mma16816(acc[1], pa[h], Halves<true>(x[0]), Halves<true>(x[1]));
+        Mma16816(acc[2], pa[h], Halves<false>(y[0]), Halves<false>(y[1]));
+        Mma16816(acc[3], pa[h], Halves<true>(y[0]), Halves<true>(y[1]));
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[4 * w + k][0] = fmaf(vs, acc[k][0] + acc[k][2], o[4 * w + k][0]);
+        o[4 * w + k][1] = fmaf(vs, acc[k][1] + acc[k][3], o[4 * w + k][1]);
+      }
+    }
+    if (u + step < units) load_values(u + step);
+  }
+
+  // The warps' states to one, in order. Lane (gid, tig) holds dimensions
+  // (2 tig + k) * D / 8 + i of vector gid.
+  l += __shfl_xor_sync(kFull, l, 1);
+  l += __shfl_xor_sync(kFull, l, 2);
+  State<D>& ws = warp_state[warp];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+#pragma unroll
+    for (int i = 0; i < kTiles; i += 4) {
+      *reinterpret_cast<float4*>(&ws.o[gid][(2 * tig + k) * (D / 8) + i]) =
+          make_float4(o[i][k], o[i + 1][k], o[i + 2][k], o[i + 3][k]);
+    }
+  }
+  if (tig == 0) {
+    ws.m[gid] = m;
+    ws.l[gid] = l;
   }
   __syncthreads();
-  if (threadIdx.x < D) {
+  const auto store = [&](int e, float sum, float acc) {
+    const int64_t v = v0 + e / D;
+    if (v < vectors) {
+      a.out[(first + v / G) * a.out_ld + (g * G + v % G) * D + e % D] = acc / sum;
+    }
+  };
+  for (int e = tid; e < kVec * D; e += kThreads) {
+    const int vec = e / D, d = e % D;
     float mx = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm[w]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, warp_state[w].m[vec]);
+#pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (sm[w] == -INFINITY) continue;
-      const float f = expf(sm[w] - mx);
-      sum = fmaf(sl[w], f, sum);
-      acc = fmaf(so[w][threadIdx.x], f, acc);
+      // A warp that saw nothing counts for nothing; one of NaN scores has
+      // reference -inf too, and a NaN sum that must survive.
+      const float f = warp_state[w].m[vec] == -INFINITY ? 1.f : Exp2(warp_state[w].m[vec] - mx);
+      sum = fmaf(warp_state[w].l[vec], f, sum);
+      acc = fmaf(warp_state[w].o[vec][d], f, acc);
     }
-    a.out[row * a.out_ld + static_cast<int64_t>(h) * D + threadIdx.x] = acc / sum;
+    if (S == 1) {
+      store(e, sum, acc);
+    } else {
+      cta_state.o[vec][d] = acc;
+      if (d == 0) {
+        cta_state.m[vec] = mx;
+        cta_state.l[vec] = sum;
+      }
+    }
   }
-}
+  if (S == 1) return;
 
-// Grid (row, head).
-template <int D>
-__global__ void __launch_bounds__(kThreads) AttnDecodeQ8Kernel(AttnArgs a) {
-  PdlTrigger();
-  PdlWait();
-  const int64_t r = blockIdx.x;
-  const int64_t pos = a.row_pos[r];
-  if (pos < 0) return;
-  const int64_t slot = a.row_seq != nullptr ? a.row_seq[r] : r;
-  if (pos >= a.cache.context || slot < 0 || slot >= a.cache.slots) {
-    if (blockIdx.y == 0 && threadIdx.x == 0 && a.status != nullptr) {
-      atomicOr(a.status, ACCEL_B200_STATUS_BAD_POSITION);
+  if (S <= kMaxCluster) {
+    ClusterSync();  // every CTA's state is there
+    // CTA `split` merges elements split * kThreads + tid on, all peers' loads in flight.
+    for (int e = split * kThreads + tid; e < kVec * D; e += S * kThreads) {
+      const int vec = e / D, d = e % D;
+      float pm[kMaxCluster], pl[kMaxCluster], po[kMaxCluster], mx = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int p = 0; p < kMaxCluster; ++p) {
+        if (p < S) {
+          pm[p] = LoadPeer(&cta_state.m[vec], static_cast<uint32_t>(p));
+          pl[p] = LoadPeer(&cta_state.l[vec], static_cast<uint32_t>(p));
+          po[p] = LoadPeer(&cta_state.o[vec][d], static_cast<uint32_t>(p));
+          mx = fmaxf(mx, pm[p]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < kMaxCluster; ++p) {
+        if (p < S) {
+          const float f = pm[p] == -INFINITY ? 1.f : Exp2(pm[p] - mx);
+          sum = fmaf(pl[p], f, sum);
+          acc = fmaf(po[p], f, acc);
+        }
+      }
+      store(e, sum, acc);
     }
+    ClusterSync();  // no CTA leaves while a peer may still read its state
     return;
   }
-  AttendRow<D>(a, r, slot, pos, blockIdx.y);
+
+  // Through the workspace: states [group][split], the last CTA merges them.
+  constexpr int kFloats = sizeof(State<D>) / 4;
+  const int64_t at = blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z;
+  __syncthreads();
+  const float* mine_state = reinterpret_cast<const float*>(&cta_state);
+  float* part = a.parts + (at * S + split) * kFloats;
+  for (int e = tid; e < kFloats; e += kThreads) part[e] = mine_state[e];
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(a.counters + at, 1) == S - 1;
+  __syncthreads();
+  if (!last) return;
+  if (tid == 0) a.counters[at] = 0;
+  __threadfence();
+  const float* parts = a.parts + at * S * kFloats;
+  for (int e = tid; e < kVec * D; e += kThreads) {
+    const int vec = e / D;
+    float mx = -INFINITY, sum = 0.f, acc = 0.f;
+    for (int p = 0; p < S; ++p) mx = fmaxf(mx, __ldcg(parts + static_cast<int64_t>(p) * kFloats + vec));
+    for (int p = 0; p < S; ++p) {
+      const float* q = parts + static_cast<int64_t>(p) * kFloats;
+      const float pm = __ldcg(q + vec);
+      const float f = pm == -INFINITY ? 1.f : Exp2(pm - mx);
+      sum = fmaf(__ldcg(q + kVec + vec), f, sum);
+      acc = fmaf(__ldcg(q + 2 * kVec + e), f, acc);
+    }
+    store(e, sum, acc);
+  }
 }
 
-// Grid (row of the sequence, head, sequence).
-template <int D>
-__global__ void __launch_bounds__(kThreads) AttnPrefillQ8Kernel(AttnArgs a) {
-  PdlTrigger();
-  PdlWait();
-  const int b = blockIdx.z;
-  const Run run = RunOf(a.rows, b, a.cache.context, blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0, a.status);
-  const int i = blockIdx.x;
-  if (i >= run.count) return;
-  AttendRow<D>(a, run.first + i, b, static_cast<int64_t>(run.pos0) + i, blockIdx.y);
+// How the vector groups of a call split the tokens they see.
+struct Split {
+  int64_t groups;  // grid y * z
+  int vec_groups;  // per (sequence or row, kv head)
+  int s;
+  size_t workspace;
+};
+
+Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run, int32_t heads, int32_t window,
+               int32_t sinks) {
+  Split p{};
+  p.vec_groups = static_cast<int>(CeilDiv(rows_per_run * (heads / c.kv_heads), kVec));
+  p.groups = runs * c.kv_heads * p.vec_groups;
+  // CTAs that are resident at once; each of their warps gets a unit at least.
+  const int64_t resident = kSms * (c.head_dim == 64 ? 4 : 2);
+  const int64_t seen = window > 0 ? Min64(c.context, static_cast<int64_t>(window) + sinks + rows_per_run) : c.context;
+  const int64_t most = Max64(1, CeilDiv(seen, kUnit) / kWarps);
+  int64_t s = Max64(1, Min64(resident / Max64(1, p.groups), most));
+  if (p.groups > kMaxCounters) s = Min64(s, kMaxCluster);
+  p.s = static_cast<int>(s);
+  if (s > kMaxCluster) {
+    const size_t state = static_cast<size_t>(2 * kVec + kVec * c.head_dim) * sizeof(float);
+    p.workspace = kCounterRegion + static_cast<size_t>(p.groups) * static_cast<size_t>(s) * state;
+  }
+  return p;
+}
+
+template <int D, bool kRuns>
+int LaunchVectors(AttnArgs a, const Split& p, int64_t runs, void* workspace, cudaStream_t stream, const char* what) {
+  if (p.workspace > 0) {
+    a.counters = static_cast<int32_t*>(workspace);
+    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterRegion);
+  }
+  const dim3 grid(static_cast<unsigned>(p.s), static_cast<unsigned>(a.cache.kv_heads * p.vec_groups),
+                  static_cast<unsigned>(runs));
+  const unsigned cluster = p.s <= kMaxCluster ? static_cast<unsigned>(p.s) : 1u;
+  return CheckLaunchEx(LaunchK(AttnVectorsQ8Kernel<D, kRuns>, grid, dim3(kThreads), 0, stream, cluster, 1u, a), what);
+}
+
+int CheckWorkspace(const Split& p, const void* workspace, size_t bytes, const std::string& what) {
+  if (p.workspace == 0) return ACCEL_B200_OK;
+  if (workspace == nullptr || bytes < p.workspace) return SetError(ACCEL_B200_EINVAL, what + ": workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+    return SetError(ACCEL_B200_EINVAL, what + ": the workspace must be 16-byte aligned");
+  }
+  return ACCEL_B200_OK;
+}
+
+AttnArgs ArgsOf(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, const RaggedRows& rows,
+                const int32_t* row_seq, const int32_t* row_pos, int32_t heads, int32_t window, int32_t sinks,
+                float* out, int64_t out_ld, int32_t* status) {
+  AttnArgs a{};
+  a.q = q;
+  a.q_ld = q_ld;
+  a.cache = *cache;
+  a.rows = rows;
+  a.row_seq = row_seq;
+  a.row_pos = row_pos;
+  a.heads = heads;
+  a.window = window;
+  a.sinks = sinks;
+  a.scale = 1.f / sqrtf(static_cast<float>(cache->head_dim));
+  a.out = out;
+  a.out_ld = out_ld;
+  a.status = status;
+  return a;
 }
 
 int CheckAttention(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, int32_t heads, int32_t window,
@@ -145,8 +561,11 @@ extern "C" {
 
 ACCEL_B200_API size_t accel_b200_attention_decode_q8_workspace(const accel_b200_q8_cache* cache, int64_t rows,
                                                                int32_t heads, int32_t window, int32_t sinks) {
-  (void)cache, (void)rows, (void)heads, (void)window, (void)sinks;
-  return 0;
+  if (CheckQ8Cache(cache, "attention_decode_q8_workspace") != ACCEL_B200_OK || rows <= 0 || heads <= 0 ||
+      heads % cache->kv_heads != 0 || window < 0 || sinks < 0) {
+    return 0;
+  }
+  return SplitFor(*cache, rows, 1, heads, window, sinks).workspace;
 }
 
 ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
@@ -154,8 +573,7 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
                                                   int32_t heads, int32_t window, int32_t sinks, float* out,
                                                   int64_t out_ld, void* workspace, size_t workspace_bytes,
                                                   int32_t* status, void* stream) {
-  (void)workspace, (void)workspace_bytes;
-  const int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, "attention_decode_q8");
+  int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, "attention_decode_q8");
   if (rc != ACCEL_B200_OK) return rc;
   if (rows < 0 || row_pos == nullptr) return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: bad arguments");
   if (row_seq == nullptr && rows > cache->slots) {
@@ -163,20 +581,26 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
   }
   if (rows == 0) return ClearError();
   if (rows > 65535) return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: more than 65535 rows");
-  const AttnArgs a{q,      q_ld,  *cache, RaggedRows{}, row_seq, row_pos, heads,
-                   window, sinks, 1.f / sqrtf(static_cast<float>(cache->head_dim)), out, out_ld, status};
-  const dim3 grid(static_cast<unsigned>(rows), static_cast<unsigned>(heads));
-  auto launch = [&](auto kernel) {
-    return CheckLaunchEx(LaunchK(kernel, grid, dim3(kThreads), 0, AsStream(stream), 1u, 1u, a), "attention_decode_q8");
-  };
-  return cache->head_dim == 64 ? launch(AttnDecodeQ8Kernel<64>) : launch(AttnDecodeQ8Kernel<128>);
+  const Split p = SplitFor(*cache, rows, 1, heads, window, sinks);
+  if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
+    return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: grid too large");
+  }
+  rc = CheckWorkspace(p, workspace, workspace_bytes, "attention_decode_q8");
+  if (rc != ACCEL_B200_OK) return rc;
+  const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{}, row_seq, row_pos, heads, window, sinks, out, out_ld, status);
+  const char* what = "attention_decode_q8";
+  if (cache->head_dim == 64) return LaunchVectors<64, false>(a, p, rows, workspace, AsStream(stream), what);
+  return LaunchVectors<128, false>(a, p, rows, workspace, AsStream(stream), what);
 }
 
 ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200_q8_cache* cache, int32_t batch,
                                                                 int32_t max_rows, int32_t heads, int32_t window,
                                                                 int32_t sinks) {
-  (void)cache, (void)batch, (void)max_rows, (void)heads, (void)window, (void)sinks;
-  return 0;
+  if (CheckQ8Cache(cache, "attention_prefill_q8_workspace") != ACCEL_B200_OK || batch <= 0 || max_rows <= 0 ||
+      heads <= 0 || heads % cache->kv_heads != 0 || window < 0 || sinks < 0) {
+    return 0;
+  }
+  return SplitFor(*cache, batch, Min64(max_rows, cache->context), heads, window, sinks).workspace;
 }
 
 ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
@@ -185,8 +609,7 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
                                                    int32_t window, int32_t sinks, float* out, int64_t out_ld,
                                                    void* workspace, size_t workspace_bytes, int32_t* status,
                                                    void* stream) {
-  (void)workspace, (void)workspace_bytes;
-  const int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, "attention_prefill_q8");
+  int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, "attention_prefill_q8");
   if (rc != ACCEL_B200_OK) return rc;
   if (rows < 0 || batch < 0 || max_rows < 0 || first == nullptr || count == nullptr || pos0 == nullptr) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: bad arguments");
@@ -195,13 +618,17 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
   if (rows == 0 || batch == 0 || max_rows == 0) return ClearError();
   if (batch > 65535) return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: more than 65535 sequences");
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));  // a longer run does not fit
-  const AttnArgs a{q,      q_ld,  *cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads,
-                   window, sinks, 1.f / sqrtf(static_cast<float>(cache->head_dim)), out, out_ld, status};
-  const dim3 grid(static_cast<unsigned>(max_rows), static_cast<unsigned>(heads), static_cast<unsigned>(batch));
-  auto launch = [&](auto kernel) {
-    return CheckLaunchEx(LaunchK(kernel, grid, dim3(kThreads), 0, AsStream(stream), 1u, 1u, a), "attention_prefill_q8");
-  };
-  return cache->head_dim == 64 ? launch(AttnPrefillQ8Kernel<64>) : launch(AttnPrefillQ8Kernel<128>);
+  const Split p = SplitFor(*cache, batch, max_rows, heads, window, sinks);
+  if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
+    return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: grid too large");
+  }
+  rc = CheckWorkspace(p, workspace, workspace_bytes, "attention_prefill_q8");
+  if (rc != ACCEL_B200_OK) return rc;
+  const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads,
+                            window, sinks, out, out_ld, status);
+  const char* what = "attention_prefill_q8";
+  if (cache->head_dim == 64) return LaunchVectors<64, true>(a, p, batch, workspace, AsStream(stream), what);
+  return LaunchVectors<128, true>(a, p, batch, workspace, AsStream(stream), what);
 }
 
 }  // extern "C"

@@ -35,6 +35,7 @@ inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
   if (c->slots <= 0 || c->kv_heads <= 0 || c->context <= 0) {
     return SetError(ACCEL_B200_EINVAL, w + ": the cache has no slots, heads or context");
   }
+  if (c->context > (1 << 30)) return SetError(ACCEL_B200_EINVAL, w + ": more than 2^30 positions");
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 != 0 || c->seq_stride % 16 != 0 ||
       c->head_stride % 16 != 0) {
     return SetError(ACCEL_B200_EINVAL, w + ": cache rows must be 16-byte aligned");

@@ -73,7 +73,13 @@ def attend(cache, q, slot, pos, window=0, sinks=0):
     Weights: exp and its argument in base 2 add 2^-22 of (1 + |score|), the 22
     bits of a weight 2^-22. Numerator and denominator are each off by that
     share of their magnitudes, their sums of n terms by n roundings at most, of
-    which a tile's partial sums bound n by 32 + visible / 32."""
+    which a tile's partial sums bound n by 32 + visible / 32.
+    Weights are held as two fp16 numbers in a unit in which the largest of a
+    row is at least 2^10 (2^(score - reference + 10), and the reference is one
+    of the scores). fp16's smallest step is 2^-24, so besides its 22 bits a
+    weight may be off by 2^-25 / 2^10 = 2^-35 of the largest one. That matters
+    where the largest weight meets a value of zero: it is 2^-35 times the sum
+    of |v|, whatever the other weights."""
     heads, d = q.shape
     kv = cache.q["k"].shape[1]
     t = visible(pos, window, sinks)
@@ -89,5 +95,5 @@ def attend(cache, q, slot, pos, window=0, sinks=0):
         out[h] = p @ v
         share = 2 * (d + 2) * 2.0 ** -24 * size.max() + 2.0 ** -22 * (2 + 2 * np.abs(s).max())
         share += (34 + len(t) / 32) * 2.0 ** -24
-        tol[h] = 2 * share * (p @ np.abs(v)) + 1e-30
+        tol[h] = 2 * share * (p @ np.abs(v)) + 2 * 2.0 ** -35 * p.max() * np.abs(v).sum(0) + 1e-30
     return out, tol

@@ -360,7 +360,7 @@ class Q8Cache:
             raise ValueError("a (slot, head) run of the cache must be contiguous")
         self.k, self.v, self.k_scale, self.v_scale, self.block = k, v, k_scale, v_scale, block
         self.slots, self.kv_heads, self.context, self.head_dim = slots, kv_heads, context, head_dim
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.native = Q8CacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k.stride(0),
                                     k.stride(1), k_scale.stride(0), k_scale.stride(1), slots, kv_heads, head_dim,
                                     context, block)
@@ -373,36 +373,51 @@ class Q8Cache:
         return cls(*planes, *scales, block)
 
 
-def _rows(name, t, device, width=None):
-    """The row stride of a 2-D fp32 tensor on `device`."""
-    if t.dtype != torch.float32 or t.dim() != 2 or t.device != device or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"{name} must be 2-D fp32 with contiguous rows on {device}")
-    if width is not None and t.shape[1] != width:
-        raise ValueError(f"{name} must have {width} columns")
+def _rows(name, t, index, width):
+    """(rows, row stride) of a 2-D fp32 tensor of `width` columns on device `index`."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not torch.float32 or t.get_device() != index or len(shape) != 2 or shape[1] != width or stride[1] != 1:
+        raise ValueError(f"{name} must be fp32 [rows, {width}] with contiguous rows on cuda:{index}")
     # One row has no stride that matters (torch may report any).
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return shape[0], stride[0] if shape[0] > 1 else max(stride[0], width)
 
 
-def _i32(device, n, **tensors):
-    for name, t in tensors.items():
-        if t is not None and (t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != n or
-                              not t.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous int32 vector of {n} on {device}")
+def _i32(name, t, index, n):
+    """The address of a contiguous int32 vector of n on device `index` (None: 0)."""
+    if t is None:
+        return 0
+    if t.dtype is not torch.int32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 vector of {n} on cuda:{index}")
+    return t.data_ptr()
 
 
 def _table(name, t, cache):
-    if (t.dtype != torch.float32 or t.device != cache.device or t.dim() != 2 or t.shape[0] < cache.context or
-            t.shape[1] != cache.head_dim or not t.is_contiguous()):
-        raise ValueError(f"{name} must be contiguous fp32 [context, head_dim] on {cache.device}")
+    shape = t.shape
+    if (t.dtype is not torch.float32 or t.get_device() != cache.index or len(shape) != 2 or
+            shape[0] < cache.context or shape[1] != cache.head_dim or not t.is_contiguous()):
+        raise ValueError(f"{name} must be contiguous fp32 [context, head_dim] on cuda:{cache.index}")
+    return t.data_ptr()
 
 
-def _call(device, fn, *args):
-    """fn(*args, stream) with `device` current, on its current stream."""
-    if torch.cuda.current_device() == device.index:
-        check(fn(*args, _s()))
+def _bytes(ws, index):
+    """(address, size) of a workspace on device `index` (None: none)."""
+    if ws is None:
+        return 0, 0
+    if ws.dtype is not torch.uint8 or ws.get_device() != index or not ws.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on cuda:{index}")
+    return ws.data_ptr(), ws.numel()
+
+
+def _call(index, fn, *args):
+    """fn(*args, stream) with device `index` current, on its current stream. (A
+    decode step makes these calls once per layer: the raw stream and device
+    numbers spare the objects that torch's public calls build.)"""
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        check(fn(*args, stream))
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, _s()))
+        with torch.cuda.device(index):
+            check(fn(*args, stream))
 
 
 def rope_append_q8(qkv, cache, first, count, pos0, heads, max_rows, cos_t, sin_t, q_out=None, status=None):
@@ -410,52 +425,50 @@ def rope_append_q8(qkv, cache, first, count, pos0, heads, max_rows, cos_t, sin_t
     of qkv [rows, (heads + 2 kv_heads) * head_dim] at positions pos0[b] + i of
     slot b (int32 device vectors; count[b] <= max_rows). Returns the roped
     queries [rows, heads * head_dim] (q_out; rows of no sequence are left)."""
-    dev, d = cache.device, cache.head_dim
-    ld = _rows("qkv", qkv, dev, (heads + 2 * cache.kv_heads) * d)
-    rows, batch = qkv.shape[0], first.shape[0]
-    _i32(dev, batch, first=first, count=count, pos0=pos0)
-    _i32(dev, 1, status=status)
-    _table("cos_t", cos_t, cache)
-    _table("sin_t", sin_t, cache)
+    index, d = cache.index, cache.head_dim
+    rows, ld = _rows("qkv", qkv, index, (heads + 2 * cache.kv_heads) * d)
+    batch = first.shape[0]
     if q_out is None:
-        q_out = torch.zeros(rows, heads * d, dtype=torch.float32, device=dev)
-    q_ld = _rows("q_out", q_out, dev, heads * d)
-    if q_out.shape[0] != rows:
+        q_out = torch.zeros(rows, heads * d, dtype=torch.float32, device=cache.device)
+    q_rows, q_ld = _rows("q_out", q_out, index, heads * d)
+    if q_rows != rows:
         raise ValueError("q_out must have a row for each row of qkv")
-    _call(dev, load().accel_b200_rope_append_q8, _p(qkv), ld, rows, cache._ref, _p(first), _p(count), _p(pos0), batch,
-          max_rows, heads, _p(cos_t), _p(sin_t), _p(q_out), q_ld, _p(status))
+    _call(index, load().accel_b200_rope_append_q8, qkv.data_ptr(), ld, rows, cache._ref,
+          _i32("first", first, index, batch), _i32("count", count, index, batch), _i32("pos0", pos0, index, batch),
+          batch, max_rows, heads, _table("cos_t", cos_t, cache), _table("sin_t", sin_t, cache), q_out.data_ptr(), q_ld,
+          _i32("status", status, index, 1))
     return q_out
 
 
 def cache_rows_q8(cache, first, count, pos0, max_rows, k_out=None, v_out=None, status=None):
     """Cache positions pos0[b] + i of slot b as fp32 into rows first[b] + i of
     k_out and v_out [rows, kv_heads * head_dim] (either may be None)."""
-    dev = cache.device
-    _i32(dev, first.shape[0], first=first, count=count, pos0=pos0)
-    _i32(dev, 1, status=status)
-    given = [t for t in (k_out, v_out) if t is not None]
-    lds = [_rows("k_out / v_out", t, dev, cache.kv_heads * cache.head_dim) for t in given]
-    if not given or len({t.shape[0] for t in given}) != 1 or len(set(lds)) != 1:
+    index, width, batch = cache.index, cache.kv_heads * cache.head_dim, first.shape[0]
+    k = v = None
+    if k_out is not None:
+        k = _rows("k_out", k_out, index, width)
+    if v_out is not None:
+        v = _rows("v_out", v_out, index, width)
+    if (k or v) is None or (k is not None and v is not None and k != v):
         raise ValueError("k_out and v_out must have the same rows and strides, and one must be given")
-    _call(dev, load().accel_b200_cache_rows_q8, cache._ref, _p(first), _p(count), _p(pos0), first.shape[0], max_rows,
-          _p(k_out), _p(v_out), lds[0], given[0].shape[0], _p(status))
+    rows, ld = k or v
+    _call(index, load().accel_b200_cache_rows_q8, cache._ref, _i32("first", first, index, batch),
+          _i32("count", count, index, batch), _i32("pos0", pos0, index, batch), batch, max_rows,
+          0 if k is None else k_out.data_ptr(), 0 if v is None else v_out.data_ptr(), ld, rows,
+          _i32("status", status, index, 1))
     return k_out, v_out
 
 
 def _attention_io(q, cache, heads, out):
-    dev, width = cache.device, heads * cache.head_dim
-    q_ld = _rows("q", q, dev, width)
+    """(rows, q's row stride, out, out's row stride)."""
+    width = heads * cache.head_dim
+    rows, q_ld = _rows("q", q, cache.index, width)
     if out is None:
-        out = torch.zeros(q.shape[0], width, dtype=torch.float32, device=dev)
-    out_ld = _rows("out", out, dev, width)
-    if out.shape[0] != q.shape[0]:
+        out = torch.zeros(rows, width, dtype=torch.float32, device=cache.device)
+    out_rows, out_ld = _rows("out", out, cache.index, width)
+    if out_rows != rows:
         raise ValueError("out must have a row for each row of q")
-    return q_ld, out, out_ld
-
-
-def _bytes(name, ws, device):
-    if ws is not None and (ws.device != device or ws.dtype != torch.uint8 or not ws.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous uint8 tensor on {device}")
+    return rows, q_ld, out, out_ld
 
 
 def attention_decode_q8_workspace(cache, rows, heads, window=0, sinks=0):
@@ -471,16 +484,14 @@ def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=
     position row_pos[r] of slot row_seq[r] (None: slot r), over an int8 cache.
     window: how many of the last tokens a row sees (0: all); sinks: first
     tokens it sees besides. Rows with row_pos < 0 are left."""
-    dev = cache.device
-    q_ld, out, out_ld = _attention_io(q, cache, heads, out)
-    _i32(dev, q.shape[0], row_pos=row_pos, row_seq=row_seq)
-    _i32(dev, 1, status=status)
+    index = cache.index
+    rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
     if workspace is None:
-        workspace = attention_decode_q8_workspace(cache, q.shape[0], heads, window, sinks)
-    _bytes("workspace", workspace, dev)
-    _call(dev, load().accel_b200_attention_decode_q8, _p(q), q_ld, cache._ref, _p(row_seq), _p(row_pos), q.shape[0],
-          heads, window, sinks, _p(out), out_ld, _p(workspace), 0 if workspace is None else workspace.numel(),
-          _p(status))
+        workspace = attention_decode_q8_workspace(cache, rows, heads, window, sinks)
+    ws, ws_bytes = _bytes(workspace, index)
+    _call(index, load().accel_b200_attention_decode_q8, q.data_ptr(), q_ld, cache._ref,
+          _i32("row_seq", row_seq, index, rows), _i32("row_pos", row_pos, index, rows), rows, heads, window, sinks,
+          out.data_ptr(), out_ld, ws, ws_bytes, _i32("status", status, index, 1))
     return out
 
 
@@ -496,15 +507,13 @@ def attention_prefill_q8(q, cache, first, count, pos0, heads, max_rows, window=0
     """Causal attention of sequence b's rows first[b] .. + count[b] - 1 of q
     (roped) at positions pos0[b] + i over slot b of an int8 cache that holds
     their keys and values. window and sinks as in attention_decode_q8."""
-    dev = cache.device
-    q_ld, out, out_ld = _attention_io(q, cache, heads, out)
-    batch = first.shape[0]
-    _i32(dev, batch, first=first, count=count, pos0=pos0)
-    _i32(dev, 1, status=status)
+    index, batch = cache.index, first.shape[0]
+    rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
     if workspace is None:
         workspace = attention_prefill_q8_workspace(cache, batch, max_rows, heads, window, sinks)
-    _bytes("workspace", workspace, dev)
-    _call(dev, load().accel_b200_attention_prefill_q8, _p(q), q_ld, cache._ref, _p(first), _p(count), _p(pos0), batch,
-          max_rows, q.shape[0], heads, window, sinks, _p(out), out_ld, _p(workspace),
-          0 if workspace is None else workspace.numel(), _p(status))
+    ws, ws_bytes = _bytes(workspace, index)
+    _call(index, load().accel_b200_attention_prefill_q8, q.data_ptr(), q_ld, cache._ref,
+          _i32("first", first, index, batch), _i32("count", count, index, batch), _i32("pos0", pos0, index, batch),
+          batch, max_rows, rows, heads, window, sinks, out.data_ptr(), out_ld, ws, ws_bytes,
+          _i32("status", status, index, 1))
     return out

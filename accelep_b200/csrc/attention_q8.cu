@@ -11,16 +11,19 @@
 // would. Queries are scaled by a power of two to 2^13 and weights to about
 // 2^10, so their second parts stay far above fp16's smallest step.
 //
-// Work split. A warp owns 8 vectors and walks units of 32 tokens, straight from
-// global memory to registers: which lane holds which dimension or token of a
-// sum is free to choose, and is chosen so that a lane's share of an MMA operand
-// is a contiguous run of bytes of the cache and the scores' register layout is
-// the weights' operand layout. No shared memory and no barrier in the loop.
-// Units are dealt to all warps of the S CTAs of a vector group in turn; the
-// next unit's keys load while this one's values are used, and the other way
-// round. Each unit's weighted values are summed on their own and added, times
-// the unit's value scale, to fp32 registers (the tensor core's running sum
-// rounds towards zero, which would drift over a long context).
+// Work split. A warp owns 8 vectors and walks units of 32 tokens, which TMA
+// brings into the warp's own queue in shared memory; no barrier but the copy's
+// own in the loop. Which lane stands for which dimension or token of a sum is
+// free to choose, and is chosen so that a lane's share of an MMA operand is a
+// run of bytes, the shared-memory reads have no bank conflicts under TMA's
+// swizzle, and the scores' register layout is the weights' operand layout.
+// (Measured at 4 sequences of 40001..65536 tokens, 8 kv heads of 128: 88 us,
+// 4.9 TB/s. With loads to registers 128 us and with per-lane cp.async 132 us:
+// an SM keeps too few of those in flight.) Units are dealt to all warps of the
+// S CTAs of a vector group in turn. Each unit's weighted values are summed on
+// their own and added, times the unit's value scale, to fp32 registers (the
+// tensor core's running sum rounds towards zero, which would drift over a long
+// context).
 //
 // Online softmax in base 2 against a reference that moves only when a score
 // passes it by more than kSlack (a vote; no weight above 2^(kBias + kSlack)).
@@ -37,6 +40,7 @@
 #include "cluster.cuh"
 #include "common.cuh"
 #include "q8_cache.cuh"
+#include "tensor_map.cuh"
 
 namespace accel_b200 {
 namespace {
@@ -48,6 +52,9 @@ constexpr int kVec = 8;        // query vectors of a CTA
 constexpr int kMaxCluster = 8; // CTAs whose states merge through distributed shared memory
 constexpr float kSlack = 4.f;  // how far (in powers of two) a score may pass the softmax reference before it moves
 constexpr float kBias = 10.f;  // weights are 2^(score - reference + kBias)
+constexpr int kWarpUnits = 2;  // units a warp gets at least before the tokens are split further
+template <int D>
+constexpr int kResident = D == 64 ? 3 : 2;  // CTAs per SM
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnArgs {
@@ -81,20 +88,6 @@ __device__ __forceinline__ float Exp2(float x) {
   return y;
 }
 
-// 16 or 8 bytes of the cache, which is read once: not kept in L1.
-__device__ __forceinline__ uint4 LoadStream16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 LoadStream8(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
 // Bytes 0 and 1 (kHi: 2 and 3) of w, each an int8 plus 128, as two fp16
 // numbers: 0x6400 | byte is 1024 + byte, less 1152.
 template <bool kHi>
@@ -117,6 +110,21 @@ __device__ __forceinline__ void SplitPair(float x, float y, uint32_t* hi, uint32
 // First position that a window ending at pos covers.
 __device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
+// Shared memory: each warp's own queue of kStages units (32 key rows, then 32
+// value rows, as TMA writes them with the swizzle of their row length), the
+// barriers behind them, and after the loop, in the queues' bytes, the warps'
+// states. The swizzle is computed from address bits up to 1024.
+template <int D>
+struct Queue {
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kPlaneBytes = kUnit * D;
+  static constexpr int kUnitBytes = 2 * kPlaneBytes;
+  static constexpr int kWarpBytes = kStages * kUnitBytes;
+  static constexpr int kBarriers = kWarps * kWarpBytes;
+  static constexpr int kBytes = kBarriers + kWarps * kStages * 8;
+  static constexpr int kAlign = 1024;
+};
+
 // The softmax state of a CTA: reference, sum and weighted values of its vectors.
 template <int D>
 struct alignas(16) State {
@@ -127,12 +135,17 @@ struct alignas(16) State {
 // Grid (split, kv head x vector group, sequence or row). kRuns: a sequence's
 // rows (prefill), else single rows.
 template <int D, bool kRuns>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
+    const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const AttnArgs a) {
   constexpr int kKw = D / 16;      // 32-bit words of a lane's share of a key row
   constexpr int kTiles = D / 8;    // 8-dimension tiles of the output
   constexpr int kVw = D / 32;      // words of a lane's share of a value row
-  __shared__ State<D> warp_state[kWarps];
-  __shared__ State<D> cta_state;
+  using Qu = Queue<D>;
+  extern __shared__ char smem_raw[];
+  char* smem = smem_raw + ((Qu::kAlign - (SmemAddr(smem_raw) & (Qu::kAlign - 1))) & (Qu::kAlign - 1));
+  static_assert(sizeof(State<D>) * (kWarps + 1) <= Qu::kBarriers, "the states fit the queues' bytes");
+  State<D>* warp_state = reinterpret_cast<State<D>*>(smem);
+  State<D>& cta_state = warp_state[kWarps];
   __shared__ bool last;
   PdlTrigger();
   PdlWait();
@@ -143,7 +156,18 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
   const int g = static_cast<int>(blockIdx.y) % c.kv_heads, group = static_cast<int>(blockIdx.y) / c.kv_heads;
   const bool reports = split == 0 && blockIdx.y == 0 && tid == 0;
 
-  // The rows: `count` from `first` at positions pos0 + i of `slot`.
+  // The rows: `count` from `first` at positions pos0 + i of `slot`. A single
+  // row's query does not wait for its position.
+  float x[kKw][4];
+  const auto load_query = [&](int64_t row, int64_t vec, bool some) {
+    const float* q = a.q + row * a.q_ld + static_cast<int64_t>(g * G + vec % G) * D + tig * 16;
+#pragma unroll
+    for (int j = 0; j < kKw; ++j) {
+      *reinterpret_cast<float4*>(x[j]) = some ? *reinterpret_cast<const float4*>(q + (j / 4) * 64 + (j % 4) * 4)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  if (!kRuns) load_query(blockIdx.z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
   int64_t first, slot;
   int count, pos0;
   if (kRuns) {
@@ -180,78 +204,59 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
   const int units = sink_units + pos_hi / kUnit - unit0 + 1;
   const int step = S * kWarps;
 
-  const int8_t* kp = c.k + slot * c.seq_stride + g * c.head_stride + tig * 16;
-  const int8_t* vp = c.v + slot * c.seq_stride + g * c.head_stride + gid * (D / 8);
   const float* ksp = c.k_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
   const float* vsp = c.v_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
   const int per_block = c.block / kUnit;
+  const int plane_row = static_cast<int>((slot * c.seq_stride + g * c.head_stride) / D);
 
-  // Keys: tile i's token gid, D / 4 bytes (dimensions 16 tig .. + 15, and 64 +
-  // the same). Values: for each half of the unit, tokens 2 tig, 2 tig + 1, 2
-  // tig + 8, 2 tig + 9, bytes gid * D / 8 on. Rows are clamped to the context.
-  uint32_t kw[4][kKw], vw[2][4][kVw];
-  float ks = 0.f, vs = 0.f;
+  // One lane of the warp copies its units; rows behind the context are of the
+  // next run or zeros, and hidden.
   const auto unit_of = [&](int u) { return u < sink_units ? u : unit0 + (u - sink_units); };
-  const auto load_keys = [&](int u) {
-    const int t0 = unit_of(u) * kUnit;
-    ks = ksp[unit_of(u) / per_block];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int8_t* p = kp + static_cast<int64_t>(min(t0 + 8 * i + gid, c.context - 1)) * D;
-#pragma unroll
-      for (int w = 0; w < kKw / 4; ++w) {
-        const uint4 x = LoadStream16(p + 64 * w);
-        kw[i][4 * w] = x.x;
-        kw[i][4 * w + 1] = x.y;
-        kw[i][4 * w + 2] = x.z;
-        kw[i][4 * w + 3] = x.w;
-      }
+  char* queue = smem + warp * Qu::kWarpBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Qu::kBarriers) + warp * Qu::kStages;
+  const auto issue = [&](int u, int stage) {
+    if (lane == 0 && u < units) {
+      const int row = plane_row + unit_of(u) * kUnit;
+      char* dst = queue + stage * Qu::kUnitBytes;
+      MbarArriveExpectTx(&full[stage], Qu::kUnitBytes);
+      TmaLoad2D(dst, &tk, 0, row, &full[stage]);
+      TmaLoad2D(dst + Qu::kPlaneBytes, &tv, 0, row, &full[stage]);
     }
   };
-  const auto load_values = [&](int u) {
-    const int t0 = unit_of(u) * kUnit;
-    vs = vsp[unit_of(u) / per_block];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = t0 + 16 * h + 2 * tig + (r & 1) + 8 * (r >> 1);
-        const int8_t* p = vp + static_cast<int64_t>(min(t, c.context - 1)) * D;
-        if (D == 64) {
-          const uint2 x = LoadStream8(p);
-          vw[h][r][0] = x.x;
-          vw[h][r][1] = x.y;
-        } else {
-          const uint4 x = LoadStream16(p);
-          vw[h][r][0] = x.x;
-          vw[h][r][1] = x.y;
-          vw[h][r][kVw - 2] = x.z;
-          vw[h][r][kVw - 1] = x.w;
-        }
-      }
-    }
-  };
-  int u = split * kWarps + warp;
-  if (u < units) {
-    load_keys(u);
-    load_values(u);
+  if (lane == 0) {
+    for (int i = 0; i < Qu::kStages; ++i) MbarInit(&full[i], 1);
+    FenceBarrierInit();
   }
+  int u = split * kWarps + warp;
+#pragma unroll
+  for (int i = 0; i < Qu::kStages - 1; ++i) issue(u + i * step, i);
+
+  // Which token, and which dimensions, a lane's place in an MMA operand stands
+  // for is free, as long as keys and queries, and weights and values, agree. It
+  // is chosen so that a lane's share is a run of bytes and each shared-memory
+  // phase of 8 (or 16) lanes covers all banks under the swizzle: column gid of
+  // a score tile is token (gid / 2) + 4 (gid % 2), its low bit flipped for odd
+  // gid; tig's share of a key row is the 16-byte pieces tig and tig + 4; gid's
+  // share of a value row is 16-byte piece gid / 2 + 4 (gid % 2), or for 64
+  // dimensions the 8-byte half gid % 2 of piece 2 ((gid / 2) % 2) + gid / 4.
+  const auto token_of = [](int n) { return ((n >> 1) + 4 * (n & 1)) ^ (n & 1); };
+  const auto dim_of = [](int n) {
+    return D == 128 ? 16 * ((n >> 1) + 4 * (n & 1)) : 16 * (2 * ((n >> 1) & 1) + (n >> 2)) + 8 * (n & 1);
+  };
+  const auto piece_at = [](int row, int byte) {  // offset of a byte of a row under the swizzle
+    return row * D + (byte ^ ((D == 128 ? row & 7 : (row >> 1) & 3) << 4));
+  };
+  const int key_at0 = piece_at(token_of(gid), 16 * tig), key_at1 = piece_at(token_of(gid), 64 % D + 16 * tig);
+  const int value_at0 = piece_at(token_of(2 * tig), dim_of(gid)), value_at1 = piece_at(token_of(2 * tig + 1), dim_of(gid));
 
   // This lane's share of its query vector, as the two fp16 parts of q * 2^e.
   uint32_t qa[kKw][4];
   float factor;  // raw sums to scores in base 2 (without the key scale)
   {
-    float x[kKw][4];
     uint32_t amax = 0;
-    const float* q = a.q + (first + my_row) * a.q_ld + static_cast<int64_t>(g * G + (v0 + gid) % G) * D + tig * 16;
+    if (kRuns) load_query(first + my_row, v0 + gid, mine);
 #pragma unroll
     for (int j = 0; j < kKw; ++j) {
-      const float4 y = mine ? *reinterpret_cast<const float4*>(q + (j / 4) * 64 + (j % 4) * 4)
-                            : make_float4(0.f, 0.f, 0.f, 0.f);
-      x[j][0] = y.x;
-      x[j][1] = y.y;
-      x[j][2] = y.z;
-      x[j][3] = y.w;
 #pragma unroll
       for (int k = 0; k < 4; ++k) amax = max(amax, __float_as_uint(x[j][k]) & 0x7fffffffu);
     }
@@ -271,9 +276,24 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) o[i][0] = o[i][1] = 0.f;
 
+  int stage = 0;
+  uint32_t parity = 0;
+  bool ok = true;
   for (; u < units; u += step) {
     const int t0 = unit_of(u) * kUnit;
-    // Scores: tile i holds tokens 8 i + 2 tig and + 1 of vector gid.
+    const float ks = ksp[unit_of(u) / per_block], vs = vsp[unit_of(u) / per_block];
+    // The stage behind the last one read is free: every lane has read it.
+    __syncwarp();
+    issue(u + (Qu::kStages - 1) * step, stage == 0 ? Qu::kStages - 1 : stage - 1);
+    ok = __all_sync(kFull, MbarWait(&full[stage], parity));
+    if (!ok) break;
+    const char* keys = queue + stage * Qu::kUnitBytes;
+    const char* values = keys + Qu::kPlaneBytes;
+    if (++stage == Qu::kStages) {
+      stage = 0;
+      parity ^= 1;
+    }
+    // Scores: tile i's columns 2 tig and 2 tig + 1 of vector gid.
     float s[4][2];
     {
       const float f = factor * ks;
@@ -281,22 +301,23 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
       for (int i = 0; i < 4; ++i) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < kKw; ++j) {
-          const uint32_t w = kw[i][j] ^ 0x80808080u;
-          Mma16816(acc, qa[j], Halves<false>(w), Halves<true>(w));
+        for (int w = 0; w < D / 64; ++w) {
+          const uint4 x = *reinterpret_cast<const uint4*>(keys + i * 8 * D + (w == 0 ? key_at0 : key_at1));
+          const uint32_t k4[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) Mma16816(acc, qa[4 * w + j], Halves<false>(k4[j]), Halves<true>(k4[j]));
         }
         s[i][0] = (acc[0] + acc[2]) * f;
         s[i][1] = (acc[1] + acc[3]) * f;
       }
     }
-    if (u + step < units) load_keys(u + step);
     // A unit that not every vector sees whole.
     if (t0 + kUnit - 1 > pos_lo || (t0 < near_hi && t0 + kUnit > a.sinks)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const int t = t0 + 8 * i + 2 * tig + k;
+          const int t = t0 + 8 * i + token_of(2 * tig + k);
           if (t > my_pos || (t < my_near && t >= a.sinks)) s[i][k] = -INFINITY;
         }
       }
@@ -330,6 +351,23 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
       SplitPair(p2, p3, &pa[h][2], &pa[h][3]);
     }
     // Weighted values, four dimensions of this lane's run at a time.
+    // Row 4 h + 2 t + k of vw: column 2 tig + k of score tile 2 h + t.
+    uint32_t vw[8][kVw];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const char* p = values + (r >> 1) * 8 * D + ((r & 1) == 0 ? value_at0 : value_at1);
+      if (D == 64) {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        vw[r][0] = x.x ^ 0x80808080u;
+        vw[r][1] = x.y ^ 0x80808080u;
+      } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        vw[r][0] = x.x ^ 0x80808080u;
+        vw[r][1] = x.y ^ 0x80808080u;
+        vw[r][kVw - 2] = x.z ^ 0x80808080u;
+        vw[r][kVw - 1] = x.w ^ 0x80808080u;
+      }
+    }
 #pragma unroll
     for (int w = 0; w < kVw; ++w) {
       float acc[4][4];
@@ -339,10 +377,10 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
         for (int i = 0; i < 4; ++i) acc[k][i] = 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t x[2], y[2];  // tokens (2 tig, + 1) and (2 tig + 8, + 9): dimensions 0 and 1, 2 and 3
+        uint32_t x[2], y[2];  // tile 2 h + r's two tokens: dimensions 0 and 1, 2 and 3
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const uint32_t w0 = vw[h][2 * r][w] ^ 0x80808080u, w1 = vw[h][2 * r + 1][w] ^ 0x80808080u;
+          const uint32_t w0 = vw[4 * h + 2 * r][w], w1 = vw[4 * h + 2 * r + 1][w];
           x[r] = __byte_perm(w0, w1, 0x5140);
           y[r] = __byte_perm(w0, w1, 0x7362);
         }
@@ -357,11 +395,24 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
         o[4 * w + k][1] = fmaf(vs, acc[k][1] + acc[k][3], o[4 * w + k][1]);
       }
     }
-    if (u + step < units) load_values(u + step);
   }
+  if (!ok) {
+    // A copy did not land: say so, give NaN, and let the copies still in
+    // flight land before the bytes are used again (bounded waits).
+    if (lane == 0 && a.status != nullptr) atomicOr(a.status, ACCEL_B200_STATUS_COPY_TIMEOUT);
+    l = __int_as_float(0x7fc00000);
+    for (int i = 0; i < Qu::kStages && u < units; ++i, u += step) {
+      MbarWait(&full[stage], parity);
+      if (++stage == Qu::kStages) {
+        stage = 0;
+        parity ^= 1;
+      }
+    }
+  }
+  __syncthreads();  // the queues' bytes become the states'
 
   // The warps' states to one, in order. Lane (gid, tig) holds dimensions
-  // (2 tig + k) * D / 8 + i of vector gid.
+  // dim_of(2 tig + k) + i of vector gid.
   l += __shfl_xor_sync(kFull, l, 1);
   l += __shfl_xor_sync(kFull, l, 2);
   State<D>& ws = warp_state[warp];
@@ -369,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
   for (int k = 0; k < 2; ++k) {
 #pragma unroll
     for (int i = 0; i < kTiles; i += 4) {
-      *reinterpret_cast<float4*>(&ws.o[gid][(2 * tig + k) * (D / 8) + i]) =
+      *reinterpret_cast<float4*>(&ws.o[gid][dim_of(2 * tig + k) + i]) =
           make_float4(o[i][k], o[i + 1][k], o[i + 2][k], o[i + 3][k]);
     }
   }
@@ -378,29 +429,44 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
     ws.l[gid] = l;
   }
   __syncthreads();
-  const auto store = [&](int e, float sum, float acc) {
+  // Element e of the CTA's vectors, four at a time.
+  const auto store = [&](int e, float sum, float4 acc) {
     const int64_t v = v0 + e / D;
     if (v < vectors) {
-      a.out[(first + v / G) * a.out_ld + (g * G + v % G) * D + e % D] = acc / sum;
+      *reinterpret_cast<float4*>(a.out + (first + v / G) * a.out_ld + (g * G + v % G) * D + e % D) =
+          make_float4(acc.x / sum, acc.y / sum, acc.z / sum, acc.w / sum);
     }
   };
-  for (int e = tid; e < kVec * D; e += kThreads) {
-    const int vec = e / D, d = e % D;
-    float mx = -INFINITY, sum = 0.f, acc = 0.f;
+  // acc += f * x. A state that saw nothing (reference -inf) counts for nothing
+  // with factor 1; one of NaN scores has reference -inf too, and a NaN sum
+  // that must survive.
+  const auto factor_of = [](float m_part, float m_all) { return m_part == -INFINITY ? 1.f : Exp2(m_part - m_all); };
+  const auto add4 = [](float4* acc, float f, const float4& x) {
+    acc->x = fmaf(x.x, f, acc->x);
+    acc->y = fmaf(x.y, f, acc->y);
+    acc->z = fmaf(x.z, f, acc->z);
+    acc->w = fmaf(x.w, f, acc->w);
+  };
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, warp_state[w].m[vec]);
+  for (int e = 4 * tid; e < kVec * D; e += 4 * kThreads) {
+    const int vec = e / D, d = e % D;
+    float pm[kWarps], mx = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      // A warp that saw nothing counts for nothing; one of NaN scores has
-      // reference -inf too, and a NaN sum that must survive.
-      const float f = warp_state[w].m[vec] == -INFINITY ? 1.f : Exp2(warp_state[w].m[vec] - mx);
+      pm[w] = warp_state[w].m[vec];
+      mx = fmaxf(mx, pm[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = factor_of(pm[w], mx);
       sum = fmaf(warp_state[w].l[vec], f, sum);
-      acc = fmaf(warp_state[w].o[vec][d], f, acc);
+      add4(&acc, f, *reinterpret_cast<const float4*>(&warp_state[w].o[vec][d]));
     }
     if (S == 1) {
       store(e, sum, acc);
     } else {
-      cta_state.o[vec][d] = acc;
+      *reinterpret_cast<float4*>(&cta_state.o[vec][d]) = acc;
       if (d == 0) {
         cta_state.m[vec] = mx;
         cta_state.l[vec] = sum;
@@ -411,25 +477,26 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
 
   if (S <= kMaxCluster) {
     ClusterSync();  // every CTA's state is there
-    // CTA `split` merges elements split * kThreads + tid on, all peers' loads in flight.
-    for (int e = split * kThreads + tid; e < kVec * D; e += S * kThreads) {
+    // CTA `split` merges every S-th group of 4 elements, all peers' loads in flight.
+    for (int e = 4 * (split + S * tid); e < kVec * D; e += 4 * S * kThreads) {
       const int vec = e / D, d = e % D;
-      float pm[kMaxCluster], pl[kMaxCluster], po[kMaxCluster], mx = -INFINITY, sum = 0.f, acc = 0.f;
+      float pm[kMaxCluster], pl[kMaxCluster], mx = -INFINITY, sum = 0.f;
+      float4 po[kMaxCluster], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int p = 0; p < kMaxCluster; ++p) {
         if (p < S) {
           pm[p] = LoadPeer(&cta_state.m[vec], static_cast<uint32_t>(p));
           pl[p] = LoadPeer(&cta_state.l[vec], static_cast<uint32_t>(p));
-          po[p] = LoadPeer(&cta_state.o[vec][d], static_cast<uint32_t>(p));
+          po[p] = LoadPeer4(&cta_state.o[vec][d], static_cast<uint32_t>(p));
           mx = fmaxf(mx, pm[p]);
         }
       }
 #pragma unroll
       for (int p = 0; p < kMaxCluster; ++p) {
         if (p < S) {
-          const float f = pm[p] == -INFINITY ? 1.f : Exp2(pm[p] - mx);
+          const float f = factor_of(pm[p], mx);
           sum = fmaf(pl[p], f, sum);
-          acc = fmaf(po[p], f, acc);
+          add4(&acc, f, po[p]);
         }
       }
       store(e, sum, acc);
@@ -442,9 +509,10 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
   constexpr int kFloats = sizeof(State<D>) / 4;
   const int64_t at = blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z;
   __syncthreads();
-  const float* mine_state = reinterpret_cast<const float*>(&cta_state);
   float* part = a.parts + (at * S + split) * kFloats;
-  for (int e = tid; e < kFloats; e += kThreads) part[e] = mine_state[e];
+  for (int e = tid; e < kFloats / 4; e += kThreads) {
+    reinterpret_cast<float4*>(part)[e] = reinterpret_cast<const float4*>(&cta_state)[e];
+  }
   __threadfence();
   __syncthreads();
   if (tid == 0) last = atomicAdd(a.counters + at, 1) == S - 1;
@@ -453,18 +521,35 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 4 : 2) AttnVectorsQ8Kernel
   if (tid == 0) a.counters[at] = 0;
   __threadfence();
   const float* parts = a.parts + at * S * kFloats;
-  for (int e = tid; e < kVec * D; e += kThreads) {
-    const int vec = e / D;
-    float mx = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int p = 0; p < S; ++p) mx = fmaxf(mx, __ldcg(parts + static_cast<int64_t>(p) * kFloats + vec));
-    for (int p = 0; p < S; ++p) {
+  // The factor and the sum of each (vector, CTA), then the weighted values with
+  // eight CTAs' loads in flight.
+  float* factors = reinterpret_cast<float*>(smem);  // [S][kVec], then the sums of the vectors
+  float* sums = factors + S * kVec;
+  for (int vec = warp; vec < kVec; vec += kWarps) {
+    float mx = -INFINITY, sum = 0.f;
+    for (int p = lane; p < S; p += 32) mx = fmaxf(mx, __ldcg(parts + static_cast<int64_t>(p) * kFloats + vec));
+    mx = WarpMax(mx);
+    for (int p = lane; p < S; p += 32) {
       const float* q = parts + static_cast<int64_t>(p) * kFloats;
       const float pm = __ldcg(q + vec);
-      const float f = pm == -INFINITY ? 1.f : Exp2(pm - mx);
+      const float f = factor_of(pm, mx);
+      factors[p * kVec + vec] = f;
       sum = fmaf(__ldcg(q + kVec + vec), f, sum);
-      acc = fmaf(__ldcg(q + 2 * kVec + e), f, acc);
     }
-    store(e, sum, acc);
+    sum = WarpSum(sum);
+    if (lane == 0) sums[vec] = sum;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 4 * tid; e < kVec * D; e += 4 * kThreads) {
+    const int vec = e / D;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = 0; p < S; ++p) {
+      add4(&acc, factors[p * kVec + vec],
+           __ldcg(reinterpret_cast<const float4*>(parts + static_cast<int64_t>(p) * kFloats + 2 * kVec + e)));
+    }
+    store(e, sums[vec], acc);
   }
 }
 
@@ -481,10 +566,11 @@ Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run,
   Split p{};
   p.vec_groups = static_cast<int>(CeilDiv(rows_per_run * (heads / c.kv_heads), kVec));
   p.groups = runs * c.kv_heads * p.vec_groups;
-  // CTAs that are resident at once; each of their warps gets a unit at least.
-  const int64_t resident = kSms * (c.head_dim == 64 ? 4 : 2);
+  // As many splits as fill the CTAs that are resident at once (a second wave
+  // costs more than it balances), while a warp gets kWarpUnits units.
+  const int64_t resident = kSms * (c.head_dim == 64 ? kResident<64> : kResident<128>);
   const int64_t seen = window > 0 ? Min64(c.context, static_cast<int64_t>(window) + sinks + rows_per_run) : c.context;
-  const int64_t most = Max64(1, CeilDiv(seen, kUnit) / kWarps);
+  const int64_t most = CeilDiv(CeilDiv(seen, kUnit), kWarps * kWarpUnits);
   int64_t s = Max64(1, Min64(resident / Max64(1, p.groups), most));
   if (p.groups > kMaxCounters) s = Min64(s, kMaxCluster);
   p.s = static_cast<int>(s);
@@ -504,7 +590,19 @@ int LaunchVectors(AttnArgs a, const Split& p, int64_t runs, void* workspace, cud
   const dim3 grid(static_cast<unsigned>(p.s), static_cast<unsigned>(a.cache.kv_heads * p.vec_groups),
                   static_cast<unsigned>(runs));
   const unsigned cluster = p.s <= kMaxCluster ? static_cast<unsigned>(p.s) : 1u;
-  return CheckLaunchEx(LaunchK(AttnVectorsQ8Kernel<D, kRuns>, grid, dim3(kThreads), 0, stream, cluster, 1u, a), what);
+  constexpr int kSmem = Queue<D>::kBytes + Queue<D>::kAlign;
+  const cudaError_t err = cudaFuncSetAttribute(AttnVectorsQ8Kernel<D, kRuns>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (err != cudaSuccess) return CheckLaunchEx(err, what);
+  const CUtensorMapSwizzle swizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  const uint64_t plane_rows = static_cast<uint64_t>(PlaneRows(a.cache));
+  CUtensorMap tk{}, tv{};
+  if (!Encode2D(&tk, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.cache.k, D, plane_rows, D, D, kUnit, swizzle) ||
+      !Encode2D(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.cache.v, D, plane_rows, D, D, kUnit, swizzle)) {
+    return SetError(ACCEL_B200_EINVAL, std::string(what) + ": cache tensor map rejected");
+  }
+  return CheckLaunchEx(
+      LaunchK(AttnVectorsQ8Kernel<D, kRuns>, grid, dim3(kThreads), kSmem, stream, cluster, 1u, tk, tv, a), what);
 }
 
 int CheckWorkspace(const Split& p, const void* workspace, size_t bytes, const std::string& what) {

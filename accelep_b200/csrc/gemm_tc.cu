@@ -76,6 +76,7 @@
 #include "common.cuh"
 #include "fixed_point.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.cuh"
 #include "tma.cuh"
 
 namespace accel_b200 {
@@ -146,14 +147,6 @@ struct TcArgs {
   Epilogue ep;
   PeerOut peers;  // copies of C on other GPUs (n = 0: none)
 };
-
-__device__ __forceinline__ void TmaLoad2D(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          SmemAddr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(SmemAddr(bar))
-      : "memory");
-}
 
 __device__ __forceinline__ void TmaLoad3D(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
                                           uint64_t* bar) {
@@ -954,20 +947,6 @@ TcPlan MakeTcPlan(int64_t m, int64_t k, int64_t n, bool silu, bool norm) {
   return p;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 EncodeFn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess) {
-      cudaGetLastError();
-      ptr = nullptr;
-    }
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }();
-  return fn;
-}
-
 template <int R, int ST, int M>
 int LaunchTc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& tu, const TcArgs& g, const TcPlan& p,
              cudaStream_t s) {
@@ -1004,16 +983,6 @@ int LaunchTcPlanes(const CUtensorMap& tw, const CUtensorMap& tx, const TcArgs& g
     case 32: return LaunchTc<32, 3, kAPlanes>(tw, tx, tx, g, p, s);
     default: return LaunchTc<64, 2, kAPlanes>(tw, tx, tx, g, p, s);
   }
-}
-
-bool Encode2D(CUtensorMap* map, CUtensorMapDataType type, const void* base, uint64_t inner, uint64_t outer,
-              uint64_t row_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {row_bytes};
-  const cuuint32_t box[2] = {box_inner, box_outer};
-  const cuuint32_t estr[2] = {1, 1};
-  return EncodeFn()(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace

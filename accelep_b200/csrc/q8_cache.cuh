@@ -20,6 +20,14 @@ inline bool Disjoint(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t inn
   return (s1 >= inner && s0 / n1 >= s1) || (s0 >= inner && s1 / n0 >= s0);
 }
 
+// Rows of head_dim bytes from the first of a plane to behind its last run; row
+// t of (slot s, head g) is (s * seq_stride + g * head_stride) / head_dim + t.
+inline int64_t PlaneRows(const accel_b200_q8_cache& c) {
+  const int64_t last = (c.slots > 1 ? (c.slots - 1) * c.seq_stride : 0) +
+                       (c.kv_heads > 1 ? (c.kv_heads - 1) * c.head_stride : 0);
+  return last / c.head_dim + c.context;
+}
+
 // ACCEL_B200_OK, or EINVAL with a message that begins with `what`.
 inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
   const std::string w(what);
@@ -36,9 +44,9 @@ inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
     return SetError(ACCEL_B200_EINVAL, w + ": the cache has no slots, heads or context");
   }
   if (c->context > (1 << 30)) return SetError(ACCEL_B200_EINVAL, w + ": more than 2^30 positions");
-  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 != 0 || c->seq_stride % 16 != 0 ||
-      c->head_stride % 16 != 0) {
-    return SetError(ACCEL_B200_EINVAL, w + ": cache rows must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) % 16 != 0 || c->seq_stride % c->head_dim != 0 ||
+      c->head_stride % c->head_dim != 0) {
+    return SetError(ACCEL_B200_EINVAL, w + ": the planes must be 16-byte aligned, their strides whole rows");
   }
   if ((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) % 4 != 0) {
     return SetError(ACCEL_B200_EINVAL, w + ": cache scales must be 4-byte aligned");
@@ -49,6 +57,7 @@ inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
       !Disjoint(c->slots, c->scale_seq_stride, c->kv_heads, c->scale_head_stride, blocks)) {
     return SetError(ACCEL_B200_EINVAL, w + ": cache strides do not hold the context");
   }
+  if (PlaneRows(*c) > (int64_t{1} << 31) - 256) return SetError(ACCEL_B200_EINVAL, w + ": more than 2^31 cache rows");
   return ACCEL_B200_OK;
 }
 

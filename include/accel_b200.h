@@ -450,8 +450,8 @@ ACCEL_B200_API int accel_b200_decode_attention_prefetch(
    head_stride + t * head_dim + d] and stands for that integer times
    k_scale[s * scale_seq_stride + g * scale_head_stride + t / block]; v the
    same. The planes are 16-byte aligned with strides that are multiples of
-   16, the scales 4-byte aligned; no two (slot, head) runs overlap, in either
-   order of slots and heads. head_dim is 64 or 128, block 32, 64 or 128 tokens.
+   head_dim, the scales 4-byte aligned; no two (slot, head) runs overlap, in
+   either order of slots and heads, and a plane spans less than 2^31 rows. head_dim is 64 or 128, block 32, 64 or 128 tokens.
    Device memory of the current device throughout. */
 typedef struct accel_b200_q8_cache {
   int8_t* k;

@@ -31,12 +31,12 @@
 // shared memory when they are one cluster (S <= 8), else through the
 // workspace by the last CTA to arrive; always in index order, so the result
 // does not depend on scheduling.
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
 
 #include "accel_b200.h"
+#include "attention_q8.cuh"
 #include "cluster.cuh"
 #include "common.cuh"
 #include "q8_cache.cuh"
@@ -50,30 +50,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnit = 32;      // tokens per step of a warp
 constexpr int kVec = 8;        // query vectors of a CTA
 constexpr int kMaxCluster = 8; // CTAs whose states merge through distributed shared memory
-constexpr float kSlack = 4.f;  // how far (in powers of two) a score may pass the softmax reference before it moves
-constexpr float kBias = 10.f;  // weights are 2^(score - reference + kBias)
 constexpr int kWarpUnits = 2;  // units a warp gets at least before the tokens are split further
 template <int D>
 constexpr int kResident = D == 64 ? 3 : 2;  // CTAs per SM
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttnArgs {
-  const float* q;
-  int64_t q_ld;
-  accel_b200_q8_cache cache;
-  RaggedRows rows;         // prefill: rows by sequence
-  const int32_t* row_seq;  // single rows: slot (null: the row's number) and position
-  const int32_t* row_pos;
-  int32_t heads;
-  int32_t window;
-  int32_t sinks;
-  float scale;
-  float* out;
-  int64_t out_ld;
-  int32_t* status;
-  int32_t* counters;  // S > kMaxCluster: arrivals by vector group, then the CTAs' states
-  float* parts;
-};
 
 __device__ __forceinline__ void Mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -81,34 +60,6 @@ __device__ __forceinline__ void Mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-__device__ __forceinline__ float Exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Bytes 0 and 1 (kHi: 2 and 3) of w, each an int8 plus 128, as two fp16
-// numbers: 0x6400 | byte is 1024 + byte, less 1152.
-template <bool kHi>
-__device__ __forceinline__ uint32_t Halves(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, kHi ? 0x4342 : 0x4140);
-  const uint32_t k1152 = 0x64806480u;
-  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&k1152));
-  return *reinterpret_cast<const uint32_t*>(&y);
-}
-
-// (x, y) as fp16 pairs hi + lo, each off by at most 2^-22 of its value.
-__device__ __forceinline__ void SplitPair(float x, float y, uint32_t* hi, uint32_t* lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-  *hi = *reinterpret_cast<const uint32_t*>(&h);
-  *lo = *reinterpret_cast<const uint32_t*>(&l);
-}
-
-// First position that a window ending at pos covers.
-__device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
 // Shared memory: each warp's own queue of kStages units (32 key rows, then 32
 // value rows, as TMA writes them with the swizzle of their row length), the
@@ -614,6 +565,12 @@ int CheckWorkspace(const Split& p, const void* workspace, size_t bytes, const st
   return ACCEL_B200_OK;
 }
 
+// Sequences of more vectors than this per kv head take 256-vector tiles.
+constexpr int64_t kMostVectors = 64;
+bool TakesTiles(const accel_b200_q8_cache& c, int64_t max_rows, int32_t heads) {
+  return max_rows * (heads / c.kv_heads) > kMostVectors;
+}
+
 AttnArgs ArgsOf(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, const RaggedRows& rows,
                 const int32_t* row_seq, const int32_t* row_pos, int32_t heads, int32_t window, int32_t sinks,
                 float* out, int64_t out_ld, int32_t* status) {
@@ -698,7 +655,9 @@ ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200
       heads <= 0 || heads % cache->kv_heads != 0 || window < 0 || sinks < 0) {
     return 0;
   }
-  return SplitFor(*cache, batch, Min64(max_rows, cache->context), heads, window, sinks).workspace;
+  max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));
+  if (TakesTiles(*cache, max_rows, heads)) return 0;
+  return SplitFor(*cache, batch, max_rows, heads, window, sinks).workspace;
 }
 
 ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
@@ -716,14 +675,15 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
   if (rows == 0 || batch == 0 || max_rows == 0) return ClearError();
   if (batch > 65535) return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: more than 65535 sequences");
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));  // a longer run does not fit
+  const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads,
+                            window, sinks, out, out_ld, status);
+  if (TakesTiles(*cache, max_rows, heads)) return LaunchTilesQ8(a, batch, max_rows, AsStream(stream));
   const Split p = SplitFor(*cache, batch, max_rows, heads, window, sinks);
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: grid too large");
   }
   rc = CheckWorkspace(p, workspace, workspace_bytes, "attention_prefill_q8");
   if (rc != ACCEL_B200_OK) return rc;
-  const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads,
-                            window, sinks, out, out_ld, status);
   const char* what = "attention_prefill_q8";
   if (cache->head_dim == 64) return LaunchVectors<64, true>(a, p, batch, workspace, AsStream(stream), what);
   return LaunchVectors<128, true>(a, p, batch, workspace, AsStream(stream), what);

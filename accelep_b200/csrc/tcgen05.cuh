@@ -68,6 +68,38 @@ __device__ __forceinline__ void MmaS8(uint32_t tmem_d, uint64_t adesc, uint64_t 
       : "memory");
 }
 
+// Instruction descriptor of kind::f16 with fp16 A and B, fp32 D, M = 128; A
+// K-major, B K-major or (b_mn) N-contiguous. n: the MMA N (16..256, % 16).
+__host__ __device__ constexpr uint32_t InstrDescF16(uint32_t n, bool b_mn) {
+  return (1u << 4)                    // D format: f32; A and B format 0: f16
+         | ((b_mn ? 1u : 0u) << 16)   // B major
+         | ((n >> 3) << 17)           // N >> 3
+         | ((128u >> 4) << 24);       // M >> 4
+}
+
+// D[tmem] (+)= A[smem] x B[smem], fp16 operands, fp32 sums, issued by one thread.
+__device__ __forceinline__ void MmaF16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The same with A in TMEM: lane r holds row r, each 32-bit column two
+// consecutive elements of K.
+__device__ __forceinline__ void MmaF16FromTmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
 // Arrives on `bar` once every tensor-core operation this thread issued so far
 // has completed.
 __device__ __forceinline__ void MmaCommit(uint64_t* bar) {
@@ -87,6 +119,33 @@ __device__ __forceinline__ void TmemLoad16Raw(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
+
+// 32 consecutive 32-bit columns of this thread's TMEM lane, as above.
+__device__ __forceinline__ void TmemLoad32Raw(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 16 registers to 16 consecutive columns of this thread's TMEM lane, without
+// waiting: TmemWaitStores() before another thread is told of them.
+__device__ __forceinline__ void TmemStore16Raw(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void TmemWaitStores() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void TmemWaitLoads() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 

@@ -19,9 +19,9 @@
 // of the tile's blocks are folded into the weights relative to the largest.
 //
 // Roles: warps 0..3 and 4..7 the softmax of the two halves (while one half
-// computes, the tensor core works for the other); warps 8..10 turn the int8
+// computes, the tensor core works for the other); warps 8..11 turn the int8
 // tiles that TMA brings into fp16 operands with the 128-byte swizzle; one
-// thread of warp 11 issues every MMA. Bound by the tensor core at 128
+// thread of warp 12 issues every MMA. Bound by the tensor core at 128
 // dimensions (two fp16 products in place of one) and by the softmax's issue
 // slots at 64.
 //
@@ -32,6 +32,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
 #include "accel_b200.h"
 #include "attention_q8.cuh"
@@ -43,13 +44,15 @@
 namespace accel_b200 {
 namespace {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kHalf = 128;         // vectors of a half: TMEM lanes
 constexpr int kTile = 128;         // tokens per tile
-constexpr int kConverters = 3;     // warps
+constexpr int kConverters = 4;     // warps
+constexpr int kMmaWarp = 8 + kConverters;
 constexpr int kChunk = 32;         // tokens whose scores a thread holds at a time: one scale block at most
 constexpr int kChunks = kTile / kChunk;
 constexpr uint32_t kTmemCols = 512;
+constexpr float kMostLift = 6.f;    // scales of a tile further apart than 2^6 are applied one by one
 constexpr int kPanel = 128 * 128;  // bytes of 128 rows x 64 fp16, the swizzle's row length
 
 template <int D>
@@ -82,6 +85,7 @@ struct Bars {
   uint64_t drain;             // after a failure
   uint32_t tmem;
   int32_t failed;
+  int32_t apart[2];           // the half's tile sums each chunk's values on its own
 };
 static_assert(sizeof(Bars) <= 256, "");
 
@@ -107,6 +111,20 @@ __device__ __forceinline__ bool SeesAll(const Range& r, int t, int n, int sinks)
   return t + n - 1 <= r.pos_lo && (t >= r.near_hi || t + n <= sinks);
 }
 
+// Registers of a warpgroup's threads from here on. 512 threads start with 128
+// each; the two softmax groups, whose threads hold D sums and a run of scores,
+// take what the other two give: 256 * kMore + 256 * kLess = 512 * 128.
+constexpr int kMore = 208, kLess = 48;
+static_assert(kMore + kLess == 2 * 128, "");
+template <int kRegs>
+__device__ __forceinline__ void RegsUp() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void RegsDown() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
 // Barrier of the converter warps; whether any thread passed true.
 __device__ __forceinline__ bool ConvertersAny(bool any) {
   uint32_t r;
@@ -129,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ char smem_raw[];
   char* smem = smem_raw + ((L::kAlign - (SmemAddr(smem_raw) & (L::kAlign - 1))) & (L::kAlign - 1));
   Bars& bars = *reinterpret_cast<Bars*>(smem + L::kBars);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kFull, tid >> 5, 0);
   const accel_b200_q8_cache& c = a.cache;
   const int G = a.heads / c.kv_heads, g = blockIdx.y, b = blockIdx.z;
   PdlWait();
@@ -160,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // TMEM is taken behind the wait for the previous kernel, and the next kernel
   // is let in behind that: neither can hold the columns the other waits for.
-  if (warp == 11) TmemAlloc(&bars.tmem, kTmemCols);
+  if (warp == kMmaWarp) TmemAlloc(&bars.tmem, kTmemCols);
   TcFenceBeforeSync();
   __syncthreads();
   TcFenceAfterSync();
@@ -175,57 +193,84 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n = sink_tiles + all.pos_hi / kTile - tile0 + 1;
   const auto token_of = [&](int j) { return (j < sink_tiles ? j : tile0 + (j - sink_tiles)) * kTile; };
   const bool second = v0 + kHalf < vectors;
-  const Range half_range[2] = {RangeOf(v0, Min64(v0 + kHalf - 1, v_last), G, run.pos0, a.window),
-                               RangeOf(second ? v0 + kHalf : v_last, v_last, G, run.pos0, a.window)};
-  const auto needed = [&](int w, int j) {
-    return (w == 0 || second) && SeesSome(half_range[w], token_of(j), kTile, a.sinks);
+  // Half w's vectors, and whether they see any of tile j.
+  const auto half_range = [&](int w) {
+    const int64_t lo = Min64(v0 + w * kHalf, v_last);
+    return RangeOf(lo, Min64(lo + kHalf - 1, v_last), G, run.pos0, a.window);
+  };
+  const auto needed = [&](const Range& range, int w, int j) {
+    return (w == 0 || second) && SeesSome(range, token_of(j), kTile, a.sinks);
   };
   volatile int32_t* failed = &bars.failed;
   // A bounded wait; false, and every role's cue to stop, once any ran out.
   const auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (MbarWait(bar, parity)) return true;
+    if (MbarWaitSleep(bar, parity)) return true;
     *failed = 1;
     return false;
   };
 
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
+    RegsUp<kMore>();
     const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // half, vector of the half
-    const Range& range = half_range[w];
+    const Range range = half_range(w);
     const int64_t v = v0 + w * kHalf + r;
     const bool mine = v < vectors;
     const int my_pos = mine ? run.pos0 + static_cast<int>(v / G) : range.pos_hi;
     const int my_near = NearOf(my_pos, a.window);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t my_scores = tmem + lanes + L::kScores + w * kTile, my_out = tmem + lanes + L::kOut + w * D;
-    float factor;
+    // The queries as two fp16 parts of q * 2^e, their largest element at 2^13.
+    // The warp loads its 32 vectors one after another, a vector over its lanes.
+    float factor = 0.f;
     {
-      // The query as two fp16 parts of q * 2^e, its largest element at 2^13.
-      const float* q = a.q + (run.first + (mine ? v / G : 0)) * a.q_ld + static_cast<int64_t>(g * G + (mine ? v % G : 0)) * D;
-      uint32_t amax = 0;
-#pragma unroll 8
-      for (int d = 0; d < D; d += 4) {
-        const float4 x = mine ? *reinterpret_cast<const float4*>(q + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        amax = max(max(amax, __float_as_uint(x.x) & 0x7fffffffu), __float_as_uint(x.y) & 0x7fffffffu);
-        amax = max(max(amax, __float_as_uint(x.z) & 0x7fffffffu), __float_as_uint(x.w) & 0x7fffffffu);
-      }
-      const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
-      char* dst = smem + L::kQ + w * 2 * L::kOperand + r * 128;
-#pragma unroll 2
-      for (int d = 0; d < D; d += 8) {
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (mine) {
-          const float4 x = *reinterpret_cast<const float4*>(q + d), y = *reinterpret_cast<const float4*>(q + d + 4);
-          SplitPair(x.x * up, x.y * up, &hi.x, &lo.x);
-          SplitPair(x.z * up, x.w * up, &hi.y, &lo.y);
-          SplitPair(y.x * up, y.y * up, &hi.z, &lo.z);
-          SplitPair(y.z * up, y.w * up, &hi.w, &lo.w);
+      constexpr int kPer = D / 32;  // elements of a vector per lane
+      const int64_t vw = v0 + w * kHalf + (warp & 3) * 32;
+      char* dst = smem + L::kQ + w * 2 * L::kOperand;
+      const int at0 = (kPer * lane / 64) * kPanel, piece = (kPer * lane % 64) / 8, in = kPer * lane % 8 * 2;
+      constexpr int kBatch = 8;  // vectors whose loads are in flight together
+      int64_t row_at = vw / G;
+      int head_at = static_cast<int>(vw - row_at * G);
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += kBatch) {
+        float x[kBatch][kPer];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const float* q = a.q + (run.first + row_at) * a.q_ld + (g * G + head_at) * D + kPer * lane;
+          const bool some = vw + i0 + i < vectors;
+          if (++head_at == G) {
+            head_at = 0;
+            ++row_at;
+          }
+          if constexpr (D == 128) {
+            *reinterpret_cast<float4*>(x[i]) =
+                some ? *reinterpret_cast<const float4*>(q) : make_float4(0.f, 0.f, 0.f, 0.f);
+          } else {
+            *reinterpret_cast<float2*>(x[i]) = some ? *reinterpret_cast<const float2*>(q) : make_float2(0.f, 0.f);
+          }
         }
-        const int at = (d / 64) * kPanel + ((((d % 64) / 8) ^ (r & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst + at) = hi;
-        *reinterpret_cast<uint4*>(dst + L::kOperand + at) = lo;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          uint32_t amax = 0;
+#pragma unroll
+          for (int k = 0; k < kPer; ++k) amax = max(amax, __float_as_uint(x[i][k]) & 0x7fffffffu);
+          amax = __reduce_max_sync(kFull, amax);
+          const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+          if (lane == i0 + i) factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
+          uint32_t hi[kPer / 2], lo[kPer / 2];
+#pragma unroll
+          for (int k = 0; k < kPer; k += 2) SplitPair(x[i][k] * up, x[i][k + 1] * up, &hi[k / 2], &lo[k / 2]);
+          const int row = (warp & 3) * 32 + i0 + i;
+          char* p = dst + at0 + row * 128 + ((piece ^ (row & 7)) << 4) + in;
+          if constexpr (D == 128) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[kPer / 2 - 1]);
+            *reinterpret_cast<uint2*>(p + L::kOperand) = make_uint2(lo[0], lo[kPer / 2 - 1]);
+          } else {
+            *reinterpret_cast<uint32_t*>(p) = hi[0];
+            *reinterpret_cast<uint32_t*>(p + L::kOperand) = lo[0];
+          }
+        }
       }
       FenceProxyAsyncSmem();
       __syncwarp();
@@ -248,26 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < 16; ++i) o[d + i] = fmaf(v_ref, __uint_as_float(x[i]), o[d + i]);
       }
     };
-    int taken = 0;  // tiles this half has gone through
-    bool ok = true;
-    for (int j = 0; j < n && ok; ++j) {
-      if (!needed(w, j)) continue;
-      const int t0 = token_of(j);
-      // Scales of the tile's chunks; one that nobody sees has weight 0 whatever
-      // its scale says.
-      float ks[kChunks], vs[kChunks], v_now = 0.f;
-#pragma unroll
-      for (int k = 0; k < kChunks; ++k) {
-        const bool seen = SeesSome(range, t0 + k * kChunk, kChunk, a.sinks);
-        ks[k] = seen ? ksp[(t0 + k * kChunk) / c.block] : 0.f;
-        vs[k] = seen ? vsp[(t0 + k * kChunk) / c.block] : 0.f;
-        v_now = fmaxf(v_now, vs[k]);
-      }
-      const bool whole = SeesAll(range, t0, kTile, a.sinks);
-      ok = __all_sync(kFull, wait(&bars.scores[w], taken & 1));
-      if (!ok) break;
-      TcFenceAfterSync();
-      const auto hidden = [&](int t) { return t > my_pos || (t < my_near && t >= a.sinks); };
+    // The tile's scores: their maximum, and then the weights in their place.
+    // kWhole: every vector of the half sees all of the tile.
+    const auto maximum = [&](auto whole, int t0, const float (&ks)[kChunks]) {
+      constexpr bool kWhole = decltype(whole)::value;
       float top = -INFINITY;
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
@@ -275,62 +304,130 @@ __global__ void __launch_bounds__(kThreads, 1)
         TmemLoad32Raw(my_scores + k * kChunk, x);
         TmemWaitLoads();
         float mx = -INFINITY;
-        if (whole) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, hidden(t0 + k * kChunk + i) ? -INFINITY : __uint_as_float(x[i]));
+        for (int i = 0; i < 32; ++i) {
+          const int t = t0 + k * kChunk + i;
+          if (kWhole || !(t > my_pos || (t < my_near && t >= a.sinks))) mx = fmaxf(mx, __uint_as_float(x[i]));
         }
         // A chunk with no visible token stays at -inf (its scale may be 0).
-        if (mx != -INFINITY) top = fmaxf(top, mx * (factor * ks[k]));
+        if (kWhole || mx != -INFINITY) top = fmaxf(top, mx * (factor * ks[k]));
       }
-      const bool moves = __any_sync(kFull, top > m + kSlack);
-      const float now = moves ? fmaxf(m, top) : m;
-      if (taken > 0) {
-        ok = __all_sync(kFull, wait(&bars.out[w], (taken - 1) & 1));
+      return top;
+    };
+    const auto weigh = [&](auto whole, int t0, const float (&ks)[kChunks], const float (&lift)[kChunks],
+                           float ref) {
+      constexpr bool kWhole = decltype(whole)::value;
+      // 16 tokens at a time: an MMA step's 8 columns of hi and 8 of lo.
+      // The next 16 scores load while these are worked on, where registers allow.
+      constexpr bool kAhead = D == 64;
+      uint32_t x[2][16], y[16];
+      TmemLoad16Raw(my_scores, x[0]);
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k) {
+        const float f = factor * ks[k / 2], shift = ref - lift[k / 2];
+        float sum = 0.f;
+        TmemWaitLoads();
+        if (kAhead && k + 1 < kTile / 16) TmemLoad16Raw(my_scores + 16 * (k + 1), x[(k + 1) & 1]);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          float p0 = Exp2(fmaf(__uint_as_float(x[kAhead ? k & 1 : 0][i]), f, -shift));
+          float p1 = Exp2(fmaf(__uint_as_float(x[kAhead ? k & 1 : 0][i + 1]), f, -shift));
+          if (!kWhole) {
+            const int t = t0 + 16 * k + i;
+            p0 = t > my_pos || (t < my_near && t >= a.sinks) ? 0.f : p0;
+            p1 = t + 1 > my_pos || (t + 1 < my_near && t + 1 >= a.sinks) ? 0.f : p1;
+          }
+          sum += p0 + p1;
+          SplitPair(p0, p1, &y[i / 2], &y[8 + i / 2]);
+        }
+        l = fmaf(sum, Exp2(-lift[k / 2]), l);
+        TmemStore16Raw(my_scores + 16 * k, y);
+        if (!kAhead && k + 1 < kTile / 16) TmemLoad16Raw(my_scores + 16 * (k + 1), x[0]);
+      }
+    };
+    int taken = 0, outs = 0;  // tiles whose scores, and MMA groups whose values, were taken
+    bool pending = false;     // weighted values of the last tile are still to be taken
+    bool ok = true;
+    for (int j = 0; j < n && ok; ++j) {
+      if (!needed(range, w, j)) continue;
+      const int t0 = token_of(j);
+      // Scales of the tile's chunks. Weights carry their chunk's value scale
+      // relative to the tile's largest, as a shift of the exponent, and the sum
+      // of weights takes it out again. Where scales are so far apart that the
+      // smaller ones' weights would lose bits, each chunk is summed on its own.
+      float ks[kChunks], lift[kChunks], v_now = 0.f;
+      bool apart = false;
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        const bool seen = SeesSome(range, t0 + k * kChunk, kChunk, a.sinks);
+        ks[k] = seen ? ksp[(t0 + k * kChunk) / c.block] : 0.f;
+        lift[k] = seen ? vsp[(t0 + k * kChunk) / c.block] : -1.f;
+        v_now = fmaxf(v_now, lift[k]);
+      }
+      const float v_inv = 1.f / v_now;
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k) {
+        lift[k] = lift[k] == -1.f ? 0.f : __log2f(lift[k] * v_inv);
+        apart = apart || !(lift[k] >= -kMostLift);
+      }
+      if (apart) {
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) lift[k] = 0.f;
+      }
+      if (pending) {
+        // The last tile's weighted values, while the tensor core sums this one's scores.
+        ok = __all_sync(kFull, wait(&bars.out[w], outs & 1));
         if (!ok) break;
         TcFenceAfterSync();
         take_out();
+        ++outs;
       }
-      if (moves) {
+      v_ref = v_now;
+      const bool whole = SeesAll(range, t0, kTile, a.sinks);
+      ok = __all_sync(kFull, wait(&bars.scores[w], taken & 1));
+      if (!ok) break;
+      TcFenceAfterSync();
+      const float top = whole ? maximum(std::true_type{}, t0, ks) : maximum(std::false_type{}, t0, ks);
+      if (__any_sync(kFull, top > m + kSlack)) {
+        const float now = fmaxf(m, top);
         const float corr = now == -INFINITY ? 1.f : Exp2(m - now);
         m = now;
         l *= corr;
 #pragma unroll
         for (int d = 0; d < D; ++d) o[d] *= corr;
       }
-      v_ref = v_now;
       const float ref = (m == -INFINITY ? 0.f : m) - kBias;
-      const float v_inv = v_now > 0.f ? 1.f / v_now : 0.f;
-      // Weights, 16 tokens at a time: an MMA step's 8 columns of hi and 8 of lo.
-#pragma unroll
-      for (int k = 0; k < kTile / 16; ++k) {
-        const float f = factor * ks[k / 2], scale = vs[k / 2];
-        const float ratio = scale == v_now ? 1.f : scale * v_inv;
-        uint32_t x[16], y[16];
-        TmemLoad16Raw(my_scores + 16 * k, x);
-        TmemWaitLoads();
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float p0 = Exp2(fmaf(__uint_as_float(x[i]), f, -ref)), p1 = Exp2(fmaf(__uint_as_float(x[i + 1]), f, -ref));
-          if (!whole) {
-            p0 = hidden(t0 + 16 * k + i) ? 0.f : p0;
-            p1 = hidden(t0 + 16 * k + i + 1) ? 0.f : p1;
-          }
-          l += p0 + p1;
-          SplitPair(p0 * ratio, p1 * ratio, &y[i / 2], &y[8 + i / 2]);
-        }
-        TmemStore16Raw(my_scores + 16 * k, y);
+      if (whole) {
+        weigh(std::true_type{}, t0, ks, lift, ref);
+      } else {
+        weigh(std::false_type{}, t0, ks, lift, ref);
       }
       TmemWaitStores();
-      TcFenceBeforeSync();
-      __syncwarp();
-      if (lane == 0) MbarArrive(&bars.weights[w]);
+      const auto tell = [&] {
+        TcFenceBeforeSync();
+        __syncwarp();
+        if (lane == 0) MbarArrive(&bars.weights[w]);
+      };
+      if (lane == 0) bars.apart[w] = apart ? 1 : 0;  // the same of all four warps
+      tell();
       ++taken;
+      pending = !apart;
+      if (apart) {
+#pragma unroll 1
+        for (int k = 0; k < kChunks && ok; ++k) {
+          const bool seen = SeesSome(range, t0 + k * kChunk, kChunk, a.sinks);
+          v_ref = seen ? vsp[(t0 + k * kChunk) / c.block] : 0.f;
+          ok = __all_sync(kFull, wait(&bars.out[w], outs & 1));
+          if (!ok) break;
+          TcFenceAfterSync();
+          take_out();
+          ++outs;
+          if (k + 1 < kChunks) tell();
+        }
+      }
     }
-    if (ok && taken > 0) {
-      ok = __all_sync(kFull, wait(&bars.out[w], (taken - 1) & 1));
+    if (ok && pending) {
+      ok = __all_sync(kFull, wait(&bars.out[w], outs & 1));
       if (ok) {
         TcFenceAfterSync();
         take_out();
@@ -346,11 +443,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp < 8 + kConverters) {
     // ---------------------------------------------------------- int8 -> fp16
+    RegsDown<kLess>();
     const int ct = tid - 256;
-    const int row0 = static_cast<int>((b * c.seq_stride + g * c.head_stride) / D);
+    const int plane_row = static_cast<int>((b * c.seq_stride + g * c.head_stride) / D);
     const auto fetch = [&](int plane, int j) {
       MbarArriveExpectTx(&bars.raw_full[plane], L::kRawBytes);
-      TmaLoad2D(smem + L::kRaw + plane * L::kRawBytes, plane == 0 ? &tk : &tv, 0, row0 + token_of(j),
+      TmaLoad2D(smem + L::kRaw + plane * L::kRawBytes, plane == 0 ? &tk : &tv, 0, plane_row + token_of(j),
                 &bars.raw_full[plane]);
     };
     if (ct == 0) {
@@ -368,15 +466,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = wait(&bars.raw_full[plane], j & 1) && wait(&bars.empty[plane][stage], lap ^ 1);
         const char* src = smem + L::kRaw + plane * L::kRawBytes;
         char* dst = smem + (plane == 0 ? L::kK : L::kV) + stage * L::kOperand;
-        constexpr int kPieces = D / 8;  // 8-element pieces of a row
-#pragma unroll 4
-        for (int i = ct; i < kTile * kPieces; i += kConverters * 32) {
-          uint2 x = *reinterpret_cast<const uint2*>(src + i * 8);
-          x.x ^= 0x80808080u;
-          x.y ^= 0x80808080u;
-          const int row = i / kPieces, piece = i % kPieces;
-          *reinterpret_cast<uint4*>(dst + (piece / 8) * kPanel + row * 128 + (((piece % 8) ^ (row & 7)) << 4)) =
-              make_uint4(Halves<false>(x.x), Halves<true>(x.x), Halves<false>(x.y), Halves<true>(x.y));
+        // 8 elements at a time. The threads are whole multiples of 8 rows, so a
+        // thread's swizzle and piece stay the same from row to row.
+        constexpr int kPieces = D / 8, kStep = kConverters * 32 / kPieces;  // pieces of a row, rows per pass
+        static_assert(kStep % 8 == 0, "");
+        constexpr int kBatch = 8;  // pieces a thread has in flight
+        const int row0 = ct / kPieces, piece = ct % kPieces;
+        src += ct * 8;
+        dst += (piece / 8) * kPanel + row0 * 128 + (((piece % 8) ^ (row0 & 7)) << 4);
+#pragma unroll 1
+        for (int r = 0; r < kTile; r += kBatch * kStep, src += kBatch * kStep * D, dst += kBatch * kStep * 128) {
+          uint2 x[kBatch];
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) x[k] = *reinterpret_cast<const uint2*>(src + k * kStep * D);
+#pragma unroll
+          for (int k = 0; k < kBatch; ++k) {
+            const uint32_t u = x[k].x ^ 0x80808080u, v = x[k].y ^ 0x80808080u;
+            *reinterpret_cast<uint4*>(dst + k * kStep * 128) =
+                make_uint4(Halves<false>(u), Halves<true>(u), Halves<false>(v), Halves<true>(v));
+          }
         }
         FenceProxyAsyncSmem();
         __syncwarp();
@@ -394,7 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ MMA
-    if (lane == 0) {
+    RegsDown<kLess>();
+    if (warp == kMmaWarp && ElectOne()) {
       constexpr uint32_t kQkDesc = InstrDescF16(kTile, false), kPvDesc = InstrDescF16(D, true);
       const uint32_t q_at = SmemAddr(smem + L::kQ), k_at = SmemAddr(smem + L::kK), v_at = SmemAddr(smem + L::kV);
       const auto scores = [&](int w, int stage) {
@@ -411,24 +520,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         MmaCommit(&bars.scores[w]);
       };
-      const auto values = [&](int w, int stage) {
+      // Weighted values of tokens 16 s0 .. 16 (s0 + kSteps) - 1 of the tile.
+      const auto values = [&](int w, int stage, int s0, auto steps) {
+        constexpr int kSteps = decltype(steps)::value;
 #pragma unroll 1
         for (int part = 1; part >= 0; --part) {
-          const uint32_t pa = tmem + L::kScores + w * kTile + part * 8, vb = v_at + stage * L::kOperand;
+          // A step: 16 tokens, 8 columns of weights, 16 rows of values.
+          const uint32_t pa = tmem + L::kScores + w * kTile + part * 8 + s0 * 16;
+          const uint32_t vb = v_at + stage * L::kOperand + s0 * 2048;
 #pragma unroll
-          for (int s = 0; s < kTile / 16; ++s) {
-            // Step s: 16 tokens, 8 columns of weights, 16 rows of values.
-            MmaF16FromTmem(tmem + L::kOut + w * D, pa + s * 16,
-                           SmemDescSw128(vb + s * 2048, kPanel, 1024), kPvDesc, part == 0 || s > 0);
+          for (int s = 0; s < kSteps; ++s) {
+            MmaF16FromTmem(tmem + L::kOut + w * D, pa + s * 16, SmemDescSw128(vb + s * 2048, kPanel, 1024), kPvDesc,
+                           part == 0 || s > 0);
           }
         }
         MmaCommit(&bars.out[w]);
       };
+      const Range range0 = half_range(0), range1 = half_range(1);
       int done[2] = {0, 0};  // weights taken from each half
       bool ok = true;
       // Scores of tile j for half w, once the half's queries and the keys are there.
       const auto next_scores = [&](int w, int j) {
-        if (!ok || !needed(w, j)) return;
+        if (!ok || !needed(w == 0 ? range0 : range1, w, j)) return;
         ok = wait(&bars.queries[w], 0) && wait(&bars.full[0][j % L::kStages], (j / L::kStages) & 1);
         if (!ok) return;
         TcFenceAfterSync();
@@ -438,18 +551,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       next_scores(1, 0);
       if (ok) MmaCommit(&bars.empty[0][0]);
       for (int j = 0; j < n && ok; ++j) {
-        for (int w = 0; w < 2 && ok; ++w) {
-          if (needed(w, j)) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (ok && needed(w == 0 ? range0 : range1, w, j)) {
             ok = wait(&bars.weights[w], done[w] & 1) && wait(&bars.full[1][j % L::kStages], (j / L::kStages) & 1);
-            if (!ok) break;
+            if (!ok) continue;
             ++done[w];
             TcFenceAfterSync();
-            values(w, j % L::kStages);
+            if (*reinterpret_cast<volatile int32_t*>(&bars.apart[w]) == 0) {
+              values(w, j % L::kStages, 0, std::integral_constant<int, kTile / 16>{});
+            } else {
+              for (int k = 0; k < kChunks && ok; ++k) {
+                if (k > 0) {
+                  ok = wait(&bars.weights[w], done[w] & 1);
+                  if (!ok) break;
+                  ++done[w];
+                  TcFenceAfterSync();
+                }
+                values(w, j % L::kStages, k * (kChunk / 16), std::integral_constant<int, kChunk / 16>{});
+              }
+            }
           }
+          // The values are free before the next scores are.
+          if (ok && w == 1) MmaCommit(&bars.empty[1][j % L::kStages]);
           if (j + 1 < n) next_scores(w, j + 1);
         }
         if (!ok) break;
-        MmaCommit(&bars.empty[1][j % L::kStages]);
         if (j + 1 < n) MmaCommit(&bars.empty[0][(j + 1) % L::kStages]);
       }
       if (!ok) {
@@ -465,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (*failed != 0 && tid == 0) {
     if (a.status != nullptr) atomicOr(a.status, ACCEL_B200_STATUS_COPY_TIMEOUT);
   }
-  if (warp == 11) TmemDealloc(tmem, kTmemCols);
+  if (warp == kMmaWarp) TmemDealloc(tmem, kTmemCols);
 }
 
 template <int D>

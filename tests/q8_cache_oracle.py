@@ -79,7 +79,10 @@ def attend(cache, q, slot, pos, window=0, sinks=0):
     of the scores). fp16's smallest step is 2^-24, so besides its 22 bits a
     weight may be off by 2^-25 / 2^10 = 2^-35 of the largest one. That matters
     where the largest weight meets a value of zero: it is 2^-35 times the sum
-    of |v|, whatever the other weights."""
+    of |v|, whatever the other weights. A prefill's weights also carry their
+    block's value scale relative to the largest of a tile, up to a ratio of
+    2^6 (beyond it blocks are summed one by one): as much more, at most.
+    """
     heads, d = q.shape
     kv = cache.q["k"].shape[1]
     t = visible(pos, window, sinks)
@@ -95,5 +98,7 @@ def attend(cache, q, slot, pos, window=0, sinks=0):
         out[h] = p @ v
         share = 2 * (d + 2) * 2.0 ** -24 * size.max() + 2.0 ** -22 * (2 + 2 * np.abs(s).max())
         share += (34 + len(t) / 32) * 2.0 ** -24
-        tol[h] = 2 * share * (p @ np.abs(v)) + 2 * 2.0 ** -35 * p.max() * np.abs(v).sum(0) + 1e-30
+        used = cache.s["v"][slot, g, np.unique(t // cache.block)]
+        spread = min(64.0, used.max() / used[used > 0].min()) if (used > 0).any() else 1.0
+        tol[h] = 2 * share * (p @ np.abs(v)) + 2 * 2.0 ** -35 * spread * p.max() * np.abs(v).sum(0) + 1e-30
     return out, tol

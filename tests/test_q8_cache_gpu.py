@@ -355,6 +355,30 @@ def test_queries_and_scales_of_any_size(lib, cuda, size):
     check_rows(c, q, got, [(0, 0, 199), (1, 1, 150)], heads, 0, 0)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("apart", [2.0 ** 5, 2.0 ** 9, 2.0 ** 40, np.inf])
+def test_value_scales_far_apart(lib, cuda, d, apart):
+    """Blocks of one tile whose value scales differ by 2^5 to 2^40, or are zero,
+    where the small ones have all of the weight, half of it or none."""
+    rng = np.random.default_rng(int(d + min(apart, 1e6)))
+    heads, kv, block, context, n = 4, 1, 32, 320, 60
+    c = filled(rng, 1, kv, context, d, block)
+    q = rng.standard_normal((n, heads * d), dtype=np.float32)
+    q[:, :d] *= 30  # one head of large scores
+    small = np.arange(context // block) % 3 == 1
+    c.s["v"][0, 0] = np.where(small, 0.0 if np.isinf(apart) else 1.0 / apart, 1.0)
+    direction = np.sign(q[:, d:2 * d].sum(0))  # tokens of small blocks that head 1 looks at
+    for j in np.flatnonzero(small):
+        c.q["k"][0, 0, j * block:(j + 1) * block] = direction * rng.integers(60, 127, (block, 1))
+    dev = device_cache(c)
+    for first_pos in (4, 250):
+        got = H(K.attention_prefill_q8(T(q), dev, I([0]), I([n]), I([first_pos]), heads, n))
+        check_rows(c, q, got, [(r, 0, first_pos + r) for r in range(0, n, 3)], heads, 0, 0)
+    rows = min(n, 3)
+    got = H(K.attention_decode_q8(T(q[:rows]), dev, I([40, 200, 319]), heads, row_seq=I([0] * rows)))
+    check_rows(c, q, got, [(0, 0, 40), (1, 0, 200), (2, 0, 319)], heads, 0, 0)
+
+
 def test_nan_queries_stay_in_their_head(lib, cuda):
     rng = np.random.default_rng(13)
     heads, kv, d = 6, 2, 64

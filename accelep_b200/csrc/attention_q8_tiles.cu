@@ -294,55 +294,61 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     // The tile's scores: their maximum, and then the weights in their place.
-    // kWhole: every vector of the half sees all of the tile.
+    // Chunks in a loop that is not unrolled: the code of a tile stays small
+    // (every CTA fetches it anew). kWhole: every vector of the half sees all of
+    // the tile; else bit i of a chunk's mask says whether it sees token i.
+    const auto pick = [](const float (&x)[kChunks], int k) {
+      return k < 2 ? (k == 0 ? x[0] : x[1]) : (k == 2 ? x[2] : x[3]);
+    };
+    const auto mask_of = [&](int t) {
+      const auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };  // bits 0 .. n - 1
+      return below(my_pos + 1 - t) & (~below(my_near - t) | below(a.sinks - t));
+    };
     const auto maximum = [&](auto whole, int t0, const float (&ks)[kChunks]) {
       constexpr bool kWhole = decltype(whole)::value;
       float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
       for (int k = 0; k < kChunks; ++k) {
         uint32_t x[32];
         TmemLoad32Raw(my_scores + k * kChunk, x);
+        const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
         TmemWaitLoads();
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          const int t = t0 + k * kChunk + i;
-          if (kWhole || !(t > my_pos || (t < my_near && t >= a.sinks))) mx = fmaxf(mx, __uint_as_float(x[i]));
+          if (kWhole || (mask >> i & 1u) != 0) mx = fmaxf(mx, __uint_as_float(x[i]));
         }
         // A chunk with no visible token stays at -inf (its scale may be 0).
-        if (kWhole || mx != -INFINITY) top = fmaxf(top, mx * (factor * ks[k]));
+        if (kWhole || mx != -INFINITY) top = fmaxf(top, mx * (factor * pick(ks, k)));
       }
       return top;
     };
-    const auto weigh = [&](auto whole, int t0, const float (&ks)[kChunks], const float (&lift)[kChunks],
-                           float ref) {
+    const auto weigh = [&](auto whole, int t0, const float (&ks)[kChunks], const float (&lift)[kChunks], float ref) {
       constexpr bool kWhole = decltype(whole)::value;
-      // 16 tokens at a time: an MMA step's 8 columns of hi and 8 of lo.
-      // The next 16 scores load while these are worked on, where registers allow.
-      constexpr bool kAhead = D == 64;
-      uint32_t x[2][16], y[16];
-      TmemLoad16Raw(my_scores, x[0]);
-#pragma unroll
-      for (int k = 0; k < kTile / 16; ++k) {
-        const float f = factor * ks[k / 2], shift = ref - lift[k / 2];
+#pragma unroll 1
+      for (int k = 0; k < kChunks; ++k) {
+        const float f = factor * pick(ks, k), up = pick(lift, k), shift = ref - up;
+        const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
         float sum = 0.f;
-        TmemWaitLoads();
-        if (kAhead && k + 1 < kTile / 16) TmemLoad16Raw(my_scores + 16 * (k + 1), x[(k + 1) & 1]);
+        // 16 tokens at a time: an MMA step's 8 columns of hi and 8 of lo.
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          float p0 = Exp2(fmaf(__uint_as_float(x[kAhead ? k & 1 : 0][i]), f, -shift));
-          float p1 = Exp2(fmaf(__uint_as_float(x[kAhead ? k & 1 : 0][i + 1]), f, -shift));
-          if (!kWhole) {
-            const int t = t0 + 16 * k + i;
-            p0 = t > my_pos || (t < my_near && t >= a.sinks) ? 0.f : p0;
-            p1 = t + 1 > my_pos || (t + 1 < my_near && t + 1 >= a.sinks) ? 0.f : p1;
+        for (int h = 0; h < 2; ++h) {
+          uint32_t x[16], y[16];
+          TmemLoad16Raw(my_scores + k * kChunk + 16 * h, x);
+          TmemWaitLoads();
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float p0 = Exp2(fmaf(__uint_as_float(x[i]), f, -shift)), p1 = Exp2(fmaf(__uint_as_float(x[i + 1]), f, -shift));
+            if (!kWhole) {
+              p0 = (mask >> (16 * h + i) & 1u) != 0 ? p0 : 0.f;
+              p1 = (mask >> (16 * h + i + 1) & 1u) != 0 ? p1 : 0.f;
+            }
+            sum += p0 + p1;
+            SplitPair(p0, p1, &y[i / 2], &y[8 + i / 2]);
           }
-          sum += p0 + p1;
-          SplitPair(p0, p1, &y[i / 2], &y[8 + i / 2]);
+          TmemStore16Raw(my_scores + k * kChunk + 16 * h, y);
         }
-        l = fmaf(sum, Exp2(-lift[k / 2]), l);
-        TmemStore16Raw(my_scores + 16 * k, y);
-        if (!kAhead && k + 1 < kTile / 16) TmemLoad16Raw(my_scores + 16 * (k + 1), x[0]);
+        l = fmaf(sum, Exp2(-up), l);
       }
     };
     int taken = 0, outs = 0;  // tiles whose scores, and MMA groups whose values, were taken

@@ -125,6 +125,40 @@ __device__ __forceinline__ void RegsDown() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
+// Two fp32 numbers in a register pair, and sm_100's paired arithmetic on them:
+// one issue slot for both.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair MakePair(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+__device__ __forceinline__ float2 Split2(Pair p) {
+  float2 v;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ Pair Fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Pair Mul2(Pair a, Pair b) {
+  Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Pair Add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float Max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Barrier of the converter warps; whether any thread passed true.
 __device__ __forceinline__ bool ConvertersAny(bool any) {
   uint32_t r;
@@ -228,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t vw = v0 + w * kHalf + (warp & 3) * 32;
       char* dst = smem + L::kQ + w * 2 * L::kOperand;
       const int at0 = (kPer * lane / 64) * kPanel, piece = (kPer * lane % 64) / 8, in = kPer * lane % 8 * 2;
-      constexpr int kBatch = 8;  // vectors whose loads are in flight together
+      constexpr int kBatch = D == 64 ? 32 : 16;  // vectors whose loads are in flight together
       int64_t row_at = vw / G;
       int head_at = static_cast<int>(vw - row_at * G);
 #pragma unroll 1
@@ -277,20 +311,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) MbarArrive(&bars.queries[w]);
     }
 
-    float m = -INFINITY, l = 0.f, v_ref = 0.f, o[D];
+    float m = -INFINITY, l = 0.f, v_ref = 0.f;
+    Pair o[D / 2];  // weighted values of dimensions 2 d and 2 d + 1
 #pragma unroll
-    for (int d = 0; d < D; ++d) o[d] = 0.f;
+    for (int d = 0; d < D / 2; ++d) o[d] = 0;
     const float* ksp = c.k_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
     const float* vsp = c.v_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
     // registers += v_ref * the last tile's weighted values.
     const auto take_out = [&] {
+      const Pair ref2 = MakePair(v_ref, v_ref);
 #pragma unroll
       for (int d = 0; d < D; d += 16) {
         uint32_t x[16];
         TmemLoad16Raw(my_out + d, x);
         TmemWaitLoads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[d + i] = fmaf(v_ref, __uint_as_float(x[i]), o[d + i]);
+        for (int i = 0; i < 16; i += 2) {
+          o[(d + i) / 2] = Fma2(ref2, MakePair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), o[(d + i) / 2]);
+        }
       }
     };
     // The tile's scores: their maximum, and then the weights in their place.
@@ -315,8 +353,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         TmemWaitLoads();
         float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (kWhole || (mask >> i & 1u) != 0) mx = fmaxf(mx, __uint_as_float(x[i]));
+        for (int i = 0; i < 32; i += 2) {
+          const float x0 = kWhole || (mask >> i & 1u) != 0 ? __uint_as_float(x[i]) : -INFINITY;
+          const float x1 = kWhole || (mask >> (i + 1) & 1u) != 0 ? __uint_as_float(x[i + 1]) : -INFINITY;
+          mx = Max3(mx, x0, x1);
         }
         // A chunk with no visible token stays at -inf (its scale may be 0).
         if (kWhole || mx != -INFINITY) top = fmaxf(top, mx * (factor * pick(ks, k)));
@@ -329,7 +369,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; k < kChunks; ++k) {
         const float f = factor * pick(ks, k), up = pick(lift, k), shift = ref - up;
         const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
-        float sum = 0.f;
+        const Pair f2 = MakePair(f, f), shift2 = MakePair(-shift, -shift), minus2 = MakePair(-1.f, -1.f);
+        Pair sum2 = 0;
         // 16 tokens at a time: an MMA step's 8 columns of hi and 8 of lo.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -338,16 +379,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           TmemWaitLoads();
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float p0 = Exp2(fmaf(__uint_as_float(x[i]), f, -shift)), p1 = Exp2(fmaf(__uint_as_float(x[i + 1]), f, -shift));
+            const float2 e =
+                Split2(Fma2(MakePair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), f2, shift2));
+            float2 p = make_float2(Exp2(e.x), Exp2(e.y));
             if (!kWhole) {
-              p0 = (mask >> (16 * h + i) & 1u) != 0 ? p0 : 0.f;
-              p1 = (mask >> (16 * h + i + 1) & 1u) != 0 ? p1 : 0.f;
+              p.x = (mask >> (16 * h + i) & 1u) != 0 ? p.x : 0.f;
+              p.y = (mask >> (16 * h + i + 1) & 1u) != 0 ? p.y : 0.f;
             }
-            sum += p0 + p1;
-            SplitPair(p0, p1, &y[i / 2], &y[8 + i / 2]);
+            const Pair p2 = MakePair(p.x, p.y);
+            sum2 = Add2(sum2, p2);
+            const __half2 hi = __floats2half2_rn(p.x, p.y);
+            const float2 back = __half22float2(hi);
+            const float2 rest = Split2(Fma2(MakePair(back.x, back.y), minus2, p2));
+            const __half2 lo = __floats2half2_rn(rest.x, rest.y);
+            y[i / 2] = *reinterpret_cast<const uint32_t*>(&hi);
+            y[8 + i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
           }
           TmemStore16Raw(my_scores + k * kChunk + 16 * h, y);
         }
+        const float2 sums = Split2(sum2);
+        const float sum = sums.x + sums.y;
         l = fmaf(sum, Exp2(-up), l);
       }
     };
@@ -399,8 +450,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float corr = now == -INFINITY ? 1.f : Exp2(m - now);
         m = now;
         l *= corr;
+        const Pair corr2 = MakePair(corr, corr);
 #pragma unroll
-        for (int d = 0; d < D; ++d) o[d] *= corr;
+        for (int d = 0; d < D / 2; ++d) o[d] = Mul2(o[d], corr2);
       }
       const float ref = (m == -INFINITY ? 0.f : m) - kBias;
       if (whole) {
@@ -444,7 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       float* dst = a.out + (run.first + v / G) * a.out_ld + static_cast<int64_t>(g * G + v % G) * D;
 #pragma unroll
       for (int d = 0; d < D; d += 4) {
-        *reinterpret_cast<float4*>(dst + d) = make_float4(o[d] / l, o[d + 1] / l, o[d + 2] / l, o[d + 3] / l);
+        const float2 x = Split2(o[d / 2]), y = Split2(o[d / 2 + 1]);
+        *reinterpret_cast<float4*>(dst + d) = make_float4(x.x / l, x.y / l, y.x / l, y.y / l);
       }
     }
   } else if (warp < 8 + kConverters) {

@@ -18,10 +18,10 @@
 // the value scale and the softmax reference change from tile to tile. Scales
 // of the tile's blocks are folded into the weights relative to the largest.
 //
-// Roles: warps 0..3 and 4..7 the softmax of the two halves (while one half
-// computes, the tensor core works for the other); warps 8..11 turn the int8
-// tiles that TMA brings into fp16 operands with the 128-byte swizzle; one
-// thread of warp 12 issues every MMA. Bound by the tensor core at 128
+// Roles: the first warps are the softmax of the two halves (while one half
+// computes, the tensor core works for the other); four turn the int8 tiles that
+// TMA brings into fp16 operands with the 128-byte swizzle; one thread of the
+// next issues every MMA. Bound by the tensor core at 128
 // dimensions (two fp16 products in place of one) and by the softmax's issue
 // slots at 64.
 //
@@ -44,11 +44,9 @@
 namespace accel_b200 {
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kHalf = 128;         // vectors of a half: TMEM lanes
 constexpr int kTile = 128;         // tokens per tile
 constexpr int kConverters = 4;     // warps
-constexpr int kMmaWarp = 8 + kConverters;
 constexpr int kChunk = 32;         // tokens whose scores a thread holds at a time: one scale block at most
 constexpr int kChunks = kTile / kChunk;
 constexpr uint32_t kTmemCols = 512;
@@ -57,6 +55,18 @@ constexpr int kPanel = 128 * 128;  // bytes of 128 rows x 64 fp16, the swizzle's
 
 template <int D>
 struct Tiles {
+  // Threads that share a vector, each with half of a tile's tokens and half of
+  // the dimensions: two where the sums of 64 dimensions leave the registers
+  // for it (one is left waiting for its own instructions most of the time).
+  static constexpr int kParts = D == 64 ? 2 : 1;
+  static constexpr int kSoftWarps = 8 * kParts, kMmaWarp = kSoftWarps + kConverters;
+  static constexpr int kThreads = (kSoftWarps + 8) * 32;  // whole warpgroups
+  // Registers of the softmax threads and of the others from their start on:
+  // in all no more than the launch gives out, 65536 / kThreads each (down to a
+  // multiple of 8).
+  static constexpr int kLaunch = 65536 / kThreads / 8 * 8;
+  static constexpr int kLess = 48, kMore = kLaunch + (kLaunch - kLess) * 256 / (kSoftWarps * 32);
+  static_assert(kMore % 8 == 0 && kSoftWarps * 32 * kMore + 256 * kLess <= kThreads * kLaunch, "");
   static constexpr int kPanels = D / 64;
   static constexpr int kOperand = kPanels * kPanel;     // a 128 x D fp16 operand
   static constexpr int kStages = D == 64 ? 2 : 1;       // fp16 key and value tiles
@@ -66,7 +76,8 @@ struct Tiles {
   static constexpr int kRaw = kV + kStages * kOperand;  // int8 tiles as they come: keys, values
   static constexpr int kRawBytes = kTile * D;
   static constexpr int kBars = kRaw + 2 * kRawBytes;
-  static constexpr int kBytes = kBars + 256;
+  static constexpr int kShared = kBars + 256;           // float [half][vector] and [2][half][part][vector]
+  static constexpr int kBytes = kShared + (kParts > 1 ? (2 + 4 * kParts) * 128 * 4 : 0);
   static constexpr int kAlign = 1024;
   static_assert(kBytes + kAlign <= 227 * 1024, "shared memory of a CTA");
   // TMEM columns: scores (then weights) and weighted values of the halves.
@@ -111,11 +122,7 @@ __device__ __forceinline__ bool SeesAll(const Range& r, int t, int n, int sinks)
   return t + n - 1 <= r.pos_lo && (t >= r.near_hi || t + n <= sinks);
 }
 
-// Registers of a warpgroup's threads from here on. 512 threads start with 128
-// each; the two softmax groups, whose threads hold D sums and a run of scores,
-// take what the other two give: 256 * kMore + 256 * kLess = 512 * 128.
-constexpr int kMore = 208, kLess = 48;
-static_assert(kMore + kLess == 2 * 128, "");
+// Registers of a warpgroup's threads from here on.
 template <int kRegs>
 __device__ __forceinline__ void RegsUp() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
@@ -159,23 +166,25 @@ __device__ __forceinline__ float Max3(float a, float b, float c) {
   return d;
 }
 
-// Barrier of the converter warps; whether any thread passed true.
-__device__ __forceinline__ bool ConvertersAny(bool any) {
+// Barrier `id` of `threads` threads; whether any of them passed true. What ends
+// one warp's loop (a wait that ran out) goes through here, so that warps that
+// meet at a barrier leave their loops together.
+__device__ __forceinline__ bool MeetAny(int id, int threads, bool any) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.or.pred q, 1, %2, p;\n\t"
+      "barrier.cta.red.or.pred q, %2, %3, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(any ? 1u : 0u), "n"(kConverters * 32)
+      : "r"(any ? 1u : 0u), "r"(id), "r"(threads)
       : "memory");
   return r != 0;
 }
 
 // Grid (256-vector tile, kv head, sequence).
 template <int D>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
     AttnTilesQ8Kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const AttnArgs a) {
   using L = Tiles<D>;
   extern __shared__ char smem_raw[];
@@ -201,9 +210,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         MbarInit(&bars.full[i][s], kConverters);
         MbarInit(&bars.empty[i][s], 1);
       }
-      MbarInit(&bars.queries[i], 4);
+      MbarInit(&bars.queries[i], 4 * L::kParts);
       MbarInit(&bars.scores[i], 1);
-      MbarInit(&bars.weights[i], 4);
+      MbarInit(&bars.weights[i], 4 * L::kParts);
       MbarInit(&bars.out[i], 1);
     }
     MbarInit(&bars.drain, 1);
@@ -212,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // TMEM is taken behind the wait for the previous kernel, and the next kernel
   // is let in behind that: neither can hold the columns the other waits for.
-  if (warp == kMmaWarp) TmemAlloc(&bars.tmem, kTmemCols);
+  if (warp == L::kMmaWarp) TmemAlloc(&bars.tmem, kTmemCols);
   TcFenceBeforeSync();
   __syncthreads();
   TcFenceAfterSync();
@@ -220,6 +229,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = bars.tmem;
 
   // The tiles: those of the sinks before the windows, then the windows.
+  const int64_t row_of_v0 = v0 / G;
+  const uint32_t head_of_v0 = static_cast<uint32_t>(v0 - row_of_v0 * G);
   const int64_t v_last = Min64(v0 + 2 * kHalf, vectors) - 1;
   const Range all = RangeOf(v0, v_last, G, run.pos0, a.window);
   const int tile0 = all.near_lo / kTile;
@@ -243,85 +254,101 @@ __global__ void __launch_bounds__(kThreads, 1)
     return false;
   };
 
-  if (warp < 8) {
+  if (warp < L::kSoftWarps) {
     // ------------------------------------------------------------- softmax
-    RegsUp<kMore>();
-    const int w = warp >> 2, r = (warp & 3) * 32 + lane;  // half, vector of the half
+    RegsUp<L::kMore>();
+    constexpr int kParts = L::kParts;
+    const int w = warp / (4 * kParts), part = (warp >> 2) % kParts;  // half, and which tokens and dimensions of it
+    const int quad = warp & 3, r = quad * 32 + lane;                  // vector of the half: its TMEM lane
     const Range range = half_range(w);
-    const int64_t v = v0 + w * kHalf + r;
-    const bool mine = v < vectors;
-    const int my_pos = mine ? run.pos0 + static_cast<int>(v / G) : range.pos_hi;
+    const bool mine = v0 + w * kHalf + r < vectors;
+    const int64_t my_row = row_of_v0 + (head_of_v0 + w * kHalf + r) / static_cast<uint32_t>(G);
+    const int my_head = g * G + static_cast<int>((head_of_v0 + w * kHalf + r) % static_cast<uint32_t>(G));
+    const int my_pos = mine ? run.pos0 + static_cast<int>(my_row) : range.pos_hi;
     const int my_near = NearOf(my_pos, a.window);
-    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t my_scores = tmem + lanes + L::kScores + w * kTile, my_out = tmem + lanes + L::kOut + w * D;
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    constexpr int kOwn = kTile / kParts, kOwnChunks = kChunks / kParts, kDims = D / kParts;
+    const uint32_t my_scores = tmem + lanes + L::kScores + w * kTile + part * kOwn;
+    const uint32_t my_out = tmem + lanes + L::kOut + w * D + part * kDims;
+    // What the threads of a vector tell each other, over a barrier of their two warps.
+    float* factors = reinterpret_cast<float*>(smem + L::kShared) + w * kHalf;
+    float* tops = reinterpret_cast<float*>(smem + L::kShared) + 2 * kHalf + w * kParts * kHalf;
+    const auto meet = [&](bool bad) { return MeetAny(2 + w * 4 + quad, kParts * 32, bad); };
     // The queries as two fp16 parts of q * 2^e, their largest element at 2^13.
-    // The warp loads its 32 vectors one after another, a vector over its lanes.
+    // Four lanes load a vector, a warp 8 at a time.
     float factor = 0.f;
     {
-      constexpr int kPer = D / 32;  // elements of a vector per lane
-      const int64_t vw = v0 + w * kHalf + (warp & 3) * 32;
+      constexpr int kLoads = D / 16;  // 16-byte pieces of a vector per lane
+      constexpr int kBatches = 4 / kParts, kTogether = D == 64 ? 2 : 1;
       char* dst = smem + L::kQ + w * 2 * L::kOperand;
-      const int at0 = (kPer * lane / 64) * kPanel, piece = (kPer * lane % 64) / 8, in = kPer * lane % 8 * 2;
-      constexpr int kBatch = D == 64 ? 32 : 16;  // vectors whose loads are in flight together
-      int64_t row_at = vw / G;
-      int head_at = static_cast<int>(vw - row_at * G);
 #pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += kBatch) {
-        float x[kBatch][kPer];
+      for (int b0 = 0; b0 < kBatches; b0 += kTogether) {
+        float4 x[kTogether][kLoads];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const float* q = a.q + (run.first + row_at) * a.q_ld + (g * G + head_at) * D + kPer * lane;
-          const bool some = vw + i0 + i < vectors;
-          if (++head_at == G) {
-            head_at = 0;
-            ++row_at;
-          }
-          if constexpr (D == 128) {
-            *reinterpret_cast<float4*>(x[i]) =
-                some ? *reinterpret_cast<const float4*>(q) : make_float4(0.f, 0.f, 0.f, 0.f);
-          } else {
-            *reinterpret_cast<float2*>(x[i]) = some ? *reinterpret_cast<const float2*>(q) : make_float2(0.f, 0.f);
+        for (int i = 0; i < kTogether; ++i) {
+          const int row = quad * 32 + (part * kBatches + b0 + i) * 8 + (lane >> 2);
+          const uint32_t at = head_of_v0 + w * kHalf + row, down = at / static_cast<uint32_t>(G);
+          const float* q = a.q + (run.first + row_of_v0 + down) * a.q_ld +
+                           static_cast<int64_t>(g * G + (at - down * G)) * D + (lane & 3) * 4;
+          const bool some = v0 + w * kHalf + row < vectors;
+#pragma unroll
+          for (int k = 0; k < kLoads; ++k) {
+            x[i][k] = some ? *reinterpret_cast<const float4*>(q + 16 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
+        for (int i = 0; i < kTogether; ++i) {
+          const int batch = part * kBatches + b0 + i, row = quad * 32 + batch * 8 + (lane >> 2);
           uint32_t amax = 0;
 #pragma unroll
-          for (int k = 0; k < kPer; ++k) amax = max(amax, __float_as_uint(x[i][k]) & 0x7fffffffu);
-          amax = __reduce_max_sync(kFull, amax);
+          for (int k = 0; k < kLoads; ++k) {
+            amax = max(max(amax, __float_as_uint(x[i][k].x) & 0x7fffffffu), __float_as_uint(x[i][k].y) & 0x7fffffffu);
+            amax = max(max(amax, __float_as_uint(x[i][k].z) & 0x7fffffffu), __float_as_uint(x[i][k].w) & 0x7fffffffu);
+          }
+          amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
+          amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
           const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);
           const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-          if (lane == i0 + i) factor = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
-          uint32_t hi[kPer / 2], lo[kPer / 2];
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
+          if (kParts == 1) {
+            const float theirs = __shfl_sync(kFull, down, (lane & 7) * 4);
+            if ((lane >> 3) == batch) factor = theirs;
+          } else if ((lane & 3) == 0) {
+            factors[row] = down;
+          }
 #pragma unroll
-          for (int k = 0; k < kPer; k += 2) SplitPair(x[i][k] * up, x[i][k + 1] * up, &hi[k / 2], &lo[k / 2]);
-          const int row = (warp & 3) * 32 + i0 + i;
-          char* p = dst + at0 + row * 128 + ((piece ^ (row & 7)) << 4) + in;
-          if constexpr (D == 128) {
-            *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[kPer / 2 - 1]);
-            *reinterpret_cast<uint2*>(p + L::kOperand) = make_uint2(lo[0], lo[kPer / 2 - 1]);
-          } else {
-            *reinterpret_cast<uint32_t*>(p) = hi[0];
-            *reinterpret_cast<uint32_t*>(p + L::kOperand) = lo[0];
+          for (int k = 0; k < kLoads; ++k) {
+            uint2 hi, lo;
+            SplitPair(x[i][k].x * up, x[i][k].y * up, &hi.x, &lo.x);
+            SplitPair(x[i][k].z * up, x[i][k].w * up, &hi.y, &lo.y);
+            // Elements 16 k + 4 (lane % 4) on: half a 16-byte piece.
+            const int piece = 2 * (k % 4) + ((lane & 3) >> 1);
+            char* p = dst + (k / 4) * kPanel + row * 128 + ((piece ^ (row & 7)) << 4) + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(p) = hi;
+            *reinterpret_cast<uint2*>(p + L::kOperand) = lo;
           }
         }
       }
       FenceProxyAsyncSmem();
       __syncwarp();
       if (lane == 0) MbarArrive(&bars.queries[w]);
+      if (kParts > 1) {
+        meet(false);
+        factor = factors[r];
+      }
     }
 
     float m = -INFINITY, l = 0.f, v_ref = 0.f;
-    Pair o[D / 2];  // weighted values of dimensions 2 d and 2 d + 1
+    Pair o[kDims / 2];  // weighted values of dimensions 2 d and 2 d + 1 of this part
 #pragma unroll
-    for (int d = 0; d < D / 2; ++d) o[d] = 0;
+    for (int d = 0; d < kDims / 2; ++d) o[d] = 0;
     const float* ksp = c.k_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
     const float* vsp = c.v_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
     // registers += v_ref * the last tile's weighted values.
     const auto take_out = [&] {
       const Pair ref2 = MakePair(v_ref, v_ref);
 #pragma unroll
-      for (int d = 0; d < D; d += 16) {
+      for (int d = 0; d < kDims; d += 16) {
         uint32_t x[16];
         TmemLoad16Raw(my_out + d, x);
         TmemWaitLoads();
@@ -346,9 +373,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr bool kWhole = decltype(whole)::value;
       float top = -INFINITY;
 #pragma unroll 1
-      for (int k = 0; k < kChunks; ++k) {
+      for (int i0 = 0; i0 < kOwnChunks; ++i0) {
+        const int k = part * kOwnChunks + i0;
         uint32_t x[32];
-        TmemLoad32Raw(my_scores + k * kChunk, x);
+        TmemLoad32Raw(my_scores + i0 * kChunk, x);
         const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
         TmemWaitLoads();
         float mx = -INFINITY;
@@ -366,7 +394,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto weigh = [&](auto whole, int t0, const float (&ks)[kChunks], const float (&lift)[kChunks], float ref) {
       constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll 1
-      for (int k = 0; k < kChunks; ++k) {
+      for (int i0 = 0; i0 < kOwnChunks; ++i0) {
+        const int k = part * kOwnChunks + i0;
         const float f = factor * pick(ks, k), up = pick(lift, k), shift = ref - up;
         const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
         const Pair f2 = MakePair(f, f), shift2 = MakePair(-shift, -shift), minus2 = MakePair(-1.f, -1.f);
@@ -375,8 +404,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t x[16], y[16];
-          TmemLoad16Raw(my_scores + k * kChunk + 16 * h, x);
-          TmemWaitLoads();
+          TmemLoad16Raw(my_scores + i0 * kChunk + 16 * h, x);
+          TmemWaitLoads(x);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             const float2 e =
@@ -395,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             y[i / 2] = *reinterpret_cast<const uint32_t*>(&hi);
             y[8 + i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
           }
-          TmemStore16Raw(my_scores + k * kChunk + 16 * h, y);
+          TmemStore16Raw(my_scores + i0 * kChunk + 16 * h, y);
         }
         const float2 sums = Split2(sum2);
         const float sum = sums.x + sums.y;
@@ -434,17 +463,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (pending) {
         // The last tile's weighted values, while the tensor core sums this one's scores.
         ok = __all_sync(kFull, wait(&bars.out[w], outs & 1));
-        if (!ok) break;
-        TcFenceAfterSync();
-        take_out();
-        ++outs;
+        if (ok) {
+          TcFenceAfterSync();
+          take_out();
+          ++outs;
+        }
       }
       v_ref = v_now;
       const bool whole = SeesAll(range, t0, kTile, a.sinks);
-      ok = __all_sync(kFull, wait(&bars.scores[w], taken & 1));
+      ok = ok && __all_sync(kFull, wait(&bars.scores[w], taken & 1));
+      float top = -INFINITY;
+      if (ok) {
+        TcFenceAfterSync();
+        top = whole ? maximum(std::true_type{}, t0, ks) : maximum(std::false_type{}, t0, ks);
+      }
+      if (kParts > 1) {
+        // Every other tile's exchange has its own place: the last one may still be read.
+        float* t = tops + (taken & 1) * 2 * kParts * kHalf;
+        t[part * kHalf + r] = top;
+        ok = !meet(!ok);
+        top = fmaxf(top, t[(part ^ 1) * kHalf + r]);
+      }
       if (!ok) break;
-      TcFenceAfterSync();
-      const float top = whole ? maximum(std::true_type{}, t0, ks) : maximum(std::false_type{}, t0, ks);
       if (__any_sync(kFull, top > m + kSlack)) {
         const float now = fmaxf(m, top);
         const float corr = now == -INFINITY ? 1.f : Exp2(m - now);
@@ -452,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l *= corr;
         const Pair corr2 = MakePair(corr, corr);
 #pragma unroll
-        for (int d = 0; d < D / 2; ++d) o[d] = Mul2(o[d], corr2);
+        for (int d = 0; d < kDims / 2; ++d) o[d] = Mul2(o[d], corr2);
       }
       const float ref = (m == -INFINITY ? 0.f : m) - kBias;
       if (whole) {
@@ -482,6 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++outs;
           if (k + 1 < kChunks) tell();
         }
+        if (kParts > 1) ok = !meet(!ok);
       }
     }
     if (ok && pending) {
@@ -492,18 +533,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     if (!ok) l = __int_as_float(0x7fc00000);
+    if (kParts > 1) {
+      // The sum of all of the tokens' weights.
+      float* t = tops + (taken & 1) * 2 * kParts * kHalf;
+      t[part * kHalf + r] = l;
+      meet(false);
+      l += t[(part ^ 1) * kHalf + r];
+    }
     if (mine) {
-      float* dst = a.out + (run.first + v / G) * a.out_ld + static_cast<int64_t>(g * G + v % G) * D;
+      float* dst = a.out + (run.first + my_row) * a.out_ld + static_cast<int64_t>(my_head) * D + part * kDims;
 #pragma unroll
-      for (int d = 0; d < D; d += 4) {
+      for (int d = 0; d < kDims; d += 4) {
         const float2 x = Split2(o[d / 2]), y = Split2(o[d / 2 + 1]);
         *reinterpret_cast<float4*>(dst + d) = make_float4(x.x / l, x.y / l, y.x / l, y.y / l);
       }
     }
-  } else if (warp < 8 + kConverters) {
+  } else if (warp < L::kMmaWarp) {
     // ---------------------------------------------------------- int8 -> fp16
-    RegsDown<kLess>();
-    const int ct = tid - 256;
+    RegsDown<L::kLess>();
+    const int ct = tid - L::kSoftWarps * 32;
     const int plane_row = static_cast<int>((b * c.seq_stride + g * c.head_stride) / D);
     const auto fetch = [&](int plane, int j) {
       MbarArriveExpectTx(&bars.raw_full[plane], L::kRawBytes);
@@ -550,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) MbarArrive(&bars.full[plane][stage]);
         // Every converter has read the int8 tile: its bytes take the next one.
         // One whose wait ran out takes all of them out of the loop together.
-        ok = !ConvertersAny(!ok);
+        ok = !MeetAny(1, kConverters * 32, !ok);
         if (ct == 0 && ok && j + 1 < n) fetch(plane, j + 1);
         if (ok) ++fetched[plane];
       }
@@ -561,8 +609,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------ MMA
-    RegsDown<kLess>();
-    if (warp == kMmaWarp && ElectOne()) {
+    RegsDown<L::kLess>();
+    if (warp == L::kMmaWarp && ElectOne()) {
       constexpr uint32_t kQkDesc = InstrDescF16(kTile, false), kPvDesc = InstrDescF16(D, true);
       const uint32_t q_at = SmemAddr(smem + L::kQ), k_at = SmemAddr(smem + L::kK), v_at = SmemAddr(smem + L::kV);
       const auto scores = [&](int w, int stage) {
@@ -651,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (*failed != 0 && tid == 0) {
     if (a.status != nullptr) atomicOr(a.status, ACCEL_B200_STATUS_COPY_TIMEOUT);
   }
-  if (warp == kMmaWarp) TmemDealloc(tmem, kTmemCols);
+  if (warp == L::kMmaWarp) TmemDealloc(tmem, kTmemCols);
 }
 
 template <int D>
@@ -669,7 +717,7 @@ int Launch(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stre
   const int64_t vectors = static_cast<int64_t>(max_rows) * (a.heads / a.cache.kv_heads);
   const dim3 grid(static_cast<unsigned>(CeilDiv(vectors, 2 * kHalf)), static_cast<unsigned>(a.cache.kv_heads),
                   static_cast<unsigned>(batch));
-  return CheckLaunchEx(LaunchK(AttnTilesQ8Kernel<D>, grid, dim3(kThreads), kSmem, stream, 1u, 1u, tk, tv, a),
+  return CheckLaunchEx(LaunchK(AttnTilesQ8Kernel<D>, grid, dim3(Tiles<D>::kThreads), kSmem, stream, 1u, 1u, tk, tv, a),
                        "attention_prefill_q8");
 }
 

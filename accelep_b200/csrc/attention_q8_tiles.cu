@@ -222,11 +222,14 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
   // TMEM is taken behind the wait for the previous kernel, and the next kernel
   // is let in behind that: neither can hold the columns the other waits for.
   if (warp == L::kMmaWarp) TmemAlloc(&bars.tmem, kTmemCols);
-  TcFenceBeforeSync();
-  __syncthreads();
-  TcFenceAfterSync();
-  PdlTrigger();
-  const uint32_t tmem = bars.tmem;
+  // Every role passes here once, the softmax with its queries' loads in flight.
+  const auto set_up = [&] {
+    TcFenceBeforeSync();
+    __syncthreads();
+    TcFenceAfterSync();
+    PdlTrigger();
+    return bars.tmem;
+  };
 
   // The tiles: those of the sinks before the windows, then the windows.
   const int64_t row_of_v0 = v0 / G;
@@ -262,14 +265,11 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
     const int quad = warp & 3, r = quad * 32 + lane;                  // vector of the half: its TMEM lane
     const Range range = half_range(w);
     const bool mine = v0 + w * kHalf + r < vectors;
-    const int64_t my_row = row_of_v0 + (head_of_v0 + w * kHalf + r) / static_cast<uint32_t>(G);
-    const int my_head = g * G + static_cast<int>((head_of_v0 + w * kHalf + r) % static_cast<uint32_t>(G));
-    const int my_pos = mine ? run.pos0 + static_cast<int>(my_row) : range.pos_hi;
+    const int my_pos =
+        mine ? run.pos0 + static_cast<int>(row_of_v0 + (head_of_v0 + w * kHalf + r) / static_cast<uint32_t>(G)) : range.pos_hi;
     const int my_near = NearOf(my_pos, a.window);
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     constexpr int kOwn = kTile / kParts, kOwnChunks = kChunks / kParts, kDims = D / kParts;
-    const uint32_t my_scores = tmem + lanes + L::kScores + w * kTile + part * kOwn;
-    const uint32_t my_out = tmem + lanes + L::kOut + w * D + part * kDims;
     // What the threads of a vector tell each other, over a barrier of their two warps.
     float* factors = reinterpret_cast<float*>(smem + L::kShared) + w * kHalf;
     float* tops = reinterpret_cast<float*>(smem + L::kShared) + 2 * kHalf + w * kParts * kHalf;
@@ -277,56 +277,55 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
     // The queries as two fp16 parts of q * 2^e, their largest element at 2^13.
     // Four lanes load a vector, a warp 8 at a time.
     float factor = 0.f;
+    uint32_t tmem;
     {
       constexpr int kLoads = D / 16;  // 16-byte pieces of a vector per lane
-      constexpr int kBatches = 4 / kParts, kTogether = D == 64 ? 2 : 1;
+      constexpr int kBatches = 4 / kParts;
       char* dst = smem + L::kQ + w * 2 * L::kOperand;
-#pragma unroll 1
-      for (int b0 = 0; b0 < kBatches; b0 += kTogether) {
-        float4 x[kTogether][kLoads];
+      float4 x[kBatches][kLoads];
 #pragma unroll
-        for (int i = 0; i < kTogether; ++i) {
-          const int row = quad * 32 + (part * kBatches + b0 + i) * 8 + (lane >> 2);
-          const uint32_t at = head_of_v0 + w * kHalf + row, down = at / static_cast<uint32_t>(G);
-          const float* q = a.q + (run.first + row_of_v0 + down) * a.q_ld +
-                           static_cast<int64_t>(g * G + (at - down * G)) * D + (lane & 3) * 4;
-          const bool some = v0 + w * kHalf + row < vectors;
+      for (int i = 0; i < kBatches; ++i) {
+        const int row = quad * 32 + (part * kBatches + i) * 8 + (lane >> 2);
+        const uint32_t at = head_of_v0 + w * kHalf + row, down = at / static_cast<uint32_t>(G);
+        const float* q = a.q + (run.first + row_of_v0 + down) * a.q_ld +
+                         static_cast<int64_t>(g * G + (at - down * G)) * D + (lane & 3) * 4;
+        const bool some = v0 + w * kHalf + row < vectors;
 #pragma unroll
-          for (int k = 0; k < kLoads; ++k) {
-            x[i][k] = some ? *reinterpret_cast<const float4*>(q + 16 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
+        for (int k = 0; k < kLoads; ++k) {
+          x[i][k] = some ? *reinterpret_cast<const float4*>(q + 16 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      tmem = set_up();
+#pragma unroll
+      for (int i = 0; i < kBatches; ++i) {
+        const int batch = part * kBatches + i, row = quad * 32 + batch * 8 + (lane >> 2);
+        uint32_t amax = 0;
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+          amax = max(max(amax, __float_as_uint(x[i][k].x) & 0x7fffffffu), __float_as_uint(x[i][k].y) & 0x7fffffffu);
+          amax = max(max(amax, __float_as_uint(x[i][k].z) & 0x7fffffffu), __float_as_uint(x[i][k].w) & 0x7fffffffu);
+        }
+        amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
+        amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
+        const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
+        if (kParts == 1) {
+          const float theirs = __shfl_sync(kFull, down, (lane & 7) * 4);
+          if ((lane >> 3) == batch) factor = theirs;
+        } else if ((lane & 3) == 0) {
+          factors[row] = down;
         }
 #pragma unroll
-        for (int i = 0; i < kTogether; ++i) {
-          const int batch = part * kBatches + b0 + i, row = quad * 32 + batch * 8 + (lane >> 2);
-          uint32_t amax = 0;
-#pragma unroll
-          for (int k = 0; k < kLoads; ++k) {
-            amax = max(max(amax, __float_as_uint(x[i][k].x) & 0x7fffffffu), __float_as_uint(x[i][k].y) & 0x7fffffffu);
-            amax = max(max(amax, __float_as_uint(x[i][k].z) & 0x7fffffffu), __float_as_uint(x[i][k].w) & 0x7fffffffu);
-          }
-          amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
-          amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
-          const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);
-          const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
-          if (kParts == 1) {
-            const float theirs = __shfl_sync(kFull, down, (lane & 7) * 4);
-            if ((lane >> 3) == batch) factor = theirs;
-          } else if ((lane & 3) == 0) {
-            factors[row] = down;
-          }
-#pragma unroll
-          for (int k = 0; k < kLoads; ++k) {
-            uint2 hi, lo;
-            SplitPair(x[i][k].x * up, x[i][k].y * up, &hi.x, &lo.x);
-            SplitPair(x[i][k].z * up, x[i][k].w * up, &hi.y, &lo.y);
-            // Elements 16 k + 4 (lane % 4) on: half a 16-byte piece.
-            const int piece = 2 * (k % 4) + ((lane & 3) >> 1);
-            char* p = dst + (k / 4) * kPanel + row * 128 + ((piece ^ (row & 7)) << 4) + (lane & 1) * 8;
-            *reinterpret_cast<uint2*>(p) = hi;
-            *reinterpret_cast<uint2*>(p + L::kOperand) = lo;
-          }
+        for (int k = 0; k < kLoads; ++k) {
+          uint2 hi, lo;
+          SplitPair(x[i][k].x * up, x[i][k].y * up, &hi.x, &lo.x);
+          SplitPair(x[i][k].z * up, x[i][k].w * up, &hi.y, &lo.y);
+          // Elements 16 k + 4 (lane % 4) on: half a 16-byte piece.
+          const int piece = 2 * (k % 4) + ((lane & 3) >> 1);
+          char* p = dst + (k / 4) * kPanel + row * 128 + ((piece ^ (row & 7)) << 4) + (lane & 1) * 8;
+          *reinterpret_cast<uint2*>(p) = hi;
+          *reinterpret_cast<uint2*>(p + L::kOperand) = lo;
         }
       }
       FenceProxyAsyncSmem();
@@ -338,6 +337,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
       }
     }
 
+    const uint32_t my_scores = tmem + lanes + L::kScores + w * kTile + part * kOwn;
+    const uint32_t my_out = tmem + lanes + L::kOut + w * D + part * kDims;
     float m = -INFINITY, l = 0.f, v_ref = 0.f;
     Pair o[kDims / 2];  // weighted values of dimensions 2 d and 2 d + 1 of this part
 #pragma unroll
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
       for (int d = 0; d < kDims; d += 16) {
         uint32_t x[16];
         TmemLoad16Raw(my_out + d, x);
-        TmemWaitLoads();
+        TmemWaitLoads(x);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           o[(d + i) / 2] = Fma2(ref2, MakePair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), o[(d + i) / 2]);
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
         uint32_t x[32];
         TmemLoad32Raw(my_scores + i0 * kChunk, x);
         const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
-        TmemWaitLoads();
+        TmemWaitLoads(x);
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -434,22 +435,35 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
     int taken = 0, outs = 0;  // tiles whose scores, and MMA groups whose values, were taken
     bool pending = false;     // weighted values of the last tile are still to be taken
     bool ok = true;
-    for (int j = 0; j < n && ok; ++j) {
-      if (!needed(range, w, j)) continue;
-      const int t0 = token_of(j);
-      // Scales of the tile's chunks. Weights carry their chunk's value scale
-      // relative to the tile's largest, as a shift of the exponent, and the sum
-      // of weights takes it out again. Where scales are so far apart that the
-      // smaller ones' weights would lose bits, each chunk is summed on its own.
+    // Scales of a tile's chunks, one per lane: keys' in lanes 0 .. 3, values' in
+    // 4 .. 7; of chunks that nobody sees 0 and -1. They load a tile ahead.
+    const auto next_needed = [&](int j) {
+      while (j < n && !needed(range, w, j)) ++j;
+      return j;
+    };
+    const auto load_scales = [&](int j) {
+      const int t = (j < n ? token_of(j) : 0) + (lane & 3) * kChunk;
+      const bool value = (lane & 4) != 0;
+      if (j >= n || lane >= 2 * kChunks || !SeesSome(range, t, kChunk, a.sinks)) return value ? -1.f : 0.f;
+      return (value ? vsp : ksp)[t / c.block];
+    };
+    int j = next_needed(0);
+    float scales = load_scales(j);
+    while (j < n && ok) {
+      const int t0 = token_of(j), next = next_needed(j + 1);
+      // Weights carry their chunk's value scale relative to the tile's largest,
+      // as a shift of the exponent, and the sum of weights takes it out again.
+      // Where scales are so far apart that the smaller ones' weights would lose
+      // bits, each chunk is summed on its own.
       float ks[kChunks], lift[kChunks], v_now = 0.f;
       bool apart = false;
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
-        const bool seen = SeesSome(range, t0 + k * kChunk, kChunk, a.sinks);
-        ks[k] = seen ? ksp[(t0 + k * kChunk) / c.block] : 0.f;
-        lift[k] = seen ? vsp[(t0 + k * kChunk) / c.block] : -1.f;
+        ks[k] = __shfl_sync(kFull, scales, k);
+        lift[k] = __shfl_sync(kFull, scales, kChunks + k);
         v_now = fmaxf(v_now, lift[k]);
       }
+      scales = load_scales(next);
       const float v_inv = 1.f / v_now;
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
@@ -524,6 +538,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
         }
         if (kParts > 1) ok = !meet(!ok);
       }
+      j = next;
     }
     if (ok && pending) {
       ok = __all_sync(kFull, wait(&bars.out[w], outs & 1));
@@ -540,17 +555,36 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
       meet(false);
       l += t[(part ^ 1) * kHalf + r];
     }
-    if (mine) {
-      float* dst = a.out + (run.first + my_row) * a.out_ld + static_cast<int64_t>(my_head) * D + part * kDims;
+    // Out through the bytes of the half's queries, which nothing reads any more:
+    // a thread's row in, then whole rows out.
+    {
+      constexpr int kRowBytes = kDims * 4, kPieces = kRowBytes / 16;
+      static_assert(32 * kRowBytes * 4 * kParts == 2 * L::kOperand, "");
+      char* mine_rows = smem + L::kQ + w * 2 * L::kOperand + (part * 4 + quad) * 32 * kRowBytes;
+      const Pair inv2 = MakePair(1.f / l, 1.f / l);
 #pragma unroll
-      for (int d = 0; d < kDims; d += 4) {
-        const float2 x = Split2(o[d / 2]), y = Split2(o[d / 2 + 1]);
-        *reinterpret_cast<float4*>(dst + d) = make_float4(x.x / l, x.y / l, y.x / l, y.y / l);
+      for (int k = 0; k < kPieces; ++k) {
+        const float2 x = Split2(Mul2(o[2 * k], inv2)), y = Split2(Mul2(o[2 * k + 1], inv2));
+        *reinterpret_cast<float4*>(mine_rows + lane * kRowBytes + ((k ^ (lane & 7)) << 4)) =
+            make_float4(x.x, x.y, y.x, y.y);
+      }
+      __syncwarp();
+      constexpr int kRows = 32 / kPieces;  // rows that the warp's lanes cover
+#pragma unroll 4
+      for (int i = lane / kPieces; i < 32; i += kRows) {
+        const int piece = lane % kPieces, row = quad * 32 + i;
+        const uint32_t at = head_of_v0 + w * kHalf + row, down = at / static_cast<uint32_t>(G);
+        if (v0 + w * kHalf + row < vectors) {
+          *reinterpret_cast<float4*>(a.out + (run.first + row_of_v0 + down) * a.out_ld +
+                                     static_cast<int64_t>(g * G + (at - down * G)) * D + part * kDims + piece * 4) =
+              *reinterpret_cast<const float4*>(mine_rows + i * kRowBytes + ((piece ^ (i & 7)) << 4));
+        }
       }
     }
   } else if (warp < L::kMmaWarp) {
     // ---------------------------------------------------------- int8 -> fp16
     RegsDown<L::kLess>();
+    set_up();
     const int ct = tid - L::kSoftWarps * 32;
     const int plane_row = static_cast<int>((b * c.seq_stride + g * c.head_stride) / D);
     const auto fetch = [&](int plane, int j) {
@@ -610,6 +644,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
   } else {
     // ------------------------------------------------------------------ MMA
     RegsDown<L::kLess>();
+    const uint32_t tmem = set_up();
     if (warp == L::kMmaWarp && ElectOne()) {
       constexpr uint32_t kQkDesc = InstrDescF16(kTile, false), kPvDesc = InstrDescF16(D, true);
       const uint32_t q_at = SmemAddr(smem + L::kQ), k_at = SmemAddr(smem + L::kK), v_at = SmemAddr(smem + L::kV);
@@ -699,7 +734,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
   if (*failed != 0 && tid == 0) {
     if (a.status != nullptr) atomicOr(a.status, ACCEL_B200_STATUS_COPY_TIMEOUT);
   }
-  if (warp == L::kMmaWarp) TmemDealloc(tmem, kTmemCols);
+  if (warp == L::kMmaWarp) TmemDealloc(bars.tmem, kTmemCols);
 }
 
 template <int D>

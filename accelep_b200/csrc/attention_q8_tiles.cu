@@ -265,8 +265,11 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
     const int quad = warp & 3, r = quad * 32 + lane;                  // vector of the half: its TMEM lane
     const Range range = half_range(w);
     const bool mine = v0 + w * kHalf + r < vectors;
-    const int my_pos =
-        mine ? run.pos0 + static_cast<int>(row_of_v0 + (head_of_v0 + w * kHalf + r) / static_cast<uint32_t>(G)) : range.pos_hi;
+    // Row (from row_of_v0) and head of this lane's vector, for itself and, by
+    // shuffle, for lanes that move its row.
+    const uint32_t my_down = (head_of_v0 + w * kHalf + r) / static_cast<uint32_t>(G);
+    const uint32_t my_place = my_down << 16 | (head_of_v0 + w * kHalf + r - my_down * G);
+    const int my_pos = mine ? run.pos0 + static_cast<int>(row_of_v0 + my_down) : range.pos_hi;
     const int my_near = NearOf(my_pos, a.window);
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     constexpr int kOwn = kTile / kParts, kOwnChunks = kChunks / kParts, kDims = D / kParts;
@@ -282,50 +285,58 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
       constexpr int kLoads = D / 16;  // 16-byte pieces of a vector per lane
       constexpr int kBatches = 4 / kParts;
       char* dst = smem + L::kQ + w * 2 * L::kOperand;
-      float4 x[kBatches][kLoads];
+      constexpr int kTogether = D == 64 ? kBatches : 2;  // as many as registers hold
+      float4 x[kTogether][kLoads];
+      const auto load = [&](int b0) {
 #pragma unroll
-      for (int i = 0; i < kBatches; ++i) {
-        const int row = quad * 32 + (part * kBatches + i) * 8 + (lane >> 2);
-        const uint32_t at = head_of_v0 + w * kHalf + row, down = at / static_cast<uint32_t>(G);
-        const float* q = a.q + (run.first + row_of_v0 + down) * a.q_ld +
-                         static_cast<int64_t>(g * G + (at - down * G)) * D + (lane & 3) * 4;
-        const bool some = v0 + w * kHalf + row < vectors;
+        for (int i = 0; i < kTogether; ++i) {
+          const int row = (part * kBatches + b0 + i) * 8 + (lane >> 2);  // of the quad
+          const uint32_t place = __shfl_sync(kFull, my_place, row);
+          const float* q = a.q + (run.first + row_of_v0 + (place >> 16)) * a.q_ld +
+                           static_cast<int64_t>(g * G + (place & 0xffffu)) * D + (lane & 3) * 4;
+          const bool some = v0 + w * kHalf + quad * 32 + row < vectors;
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) {
-          x[i][k] = some ? *reinterpret_cast<const float4*>(q + 16 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int k = 0; k < kLoads; ++k) {
+            x[i][k] = some ? *reinterpret_cast<const float4*>(q + 16 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
         }
-      }
+      };
+      load(0);
       tmem = set_up();
+#pragma unroll 1
+      for (int b0 = 0; b0 < kBatches; b0 += kTogether) {
+        if (b0 > 0) load(b0);
 #pragma unroll
-      for (int i = 0; i < kBatches; ++i) {
-        const int batch = part * kBatches + i, row = quad * 32 + batch * 8 + (lane >> 2);
-        uint32_t amax = 0;
+        for (int i = 0; i < kTogether; ++i) {
+          const int batch = part * kBatches + b0 + i, row = quad * 32 + batch * 8 + (lane >> 2);
+          uint32_t amax = 0;
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) {
-          amax = max(max(amax, __float_as_uint(x[i][k].x) & 0x7fffffffu), __float_as_uint(x[i][k].y) & 0x7fffffffu);
-          amax = max(max(amax, __float_as_uint(x[i][k].z) & 0x7fffffffu), __float_as_uint(x[i][k].w) & 0x7fffffffu);
-        }
-        amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
-        amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
-        const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);
-        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
-        if (kParts == 1) {
-          const float theirs = __shfl_sync(kFull, down, (lane & 7) * 4);
-          if ((lane >> 3) == batch) factor = theirs;
-        } else if ((lane & 3) == 0) {
-          factors[row] = down;
-        }
+          for (int k = 0; k < kLoads; ++k) {
+            amax = max(max(amax, __float_as_uint(x[i][k].x) & 0x7fffffffu), __float_as_uint(x[i][k].y) & 0x7fffffffu);
+            amax = max(max(amax, __float_as_uint(x[i][k].z) & 0x7fffffffu), __float_as_uint(x[i][k].w) & 0x7fffffffu);
+          }
+          amax = max(amax, __shfl_xor_sync(kFull, amax, 1));
+          amax = max(amax, __shfl_xor_sync(kFull, amax, 2));
+          const int e = min(13 + 127 - static_cast<int>(amax >> 23), 126);
+          const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+          const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23) * (a.scale * kLog2e);
+          if (kParts == 1) {
+            const float theirs = __shfl_sync(kFull, down, (lane & 7) * 4);
+            if ((lane >> 3) == batch) factor = theirs;
+          } else if ((lane & 3) == 0) {
+            factors[row] = down;
+          }
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) {
-          uint2 hi, lo;
-          SplitPair(x[i][k].x * up, x[i][k].y * up, &hi.x, &lo.x);
-          SplitPair(x[i][k].z * up, x[i][k].w * up, &hi.y, &lo.y);
-          // Elements 16 k + 4 (lane % 4) on: half a 16-byte piece.
-          const int piece = 2 * (k % 4) + ((lane & 3) >> 1);
-          char* p = dst + (k / 4) * kPanel + row * 128 + ((piece ^ (row & 7)) << 4) + (lane & 1) * 8;
-          *reinterpret_cast<uint2*>(p) = hi;
-          *reinterpret_cast<uint2*>(p + L::kOperand) = lo;
+          for (int k = 0; k < kLoads; ++k) {
+            uint2 hi, lo;
+            SplitPair(x[i][k].x * up, x[i][k].y * up, &hi.x, &lo.x);
+            SplitPair(x[i][k].z * up, x[i][k].w * up, &hi.y, &lo.y);
+            // Elements 16 k + 4 (lane % 4) on: half a 16-byte piece.
+            const int piece = 2 * (k % 4) + ((lane & 3) >> 1);
+            char* p = dst + (k / 4) * kPanel + row * 128 + ((piece ^ (row & 7)) << 4) + (lane & 1) * 8;
+            *reinterpret_cast<uint2*>(p) = hi;
+            *reinterpret_cast<uint2*>(p + L::kOperand) = lo;
+          }
         }
       }
       FenceProxyAsyncSmem();
@@ -570,13 +581,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
       }
       __syncwarp();
       constexpr int kRows = 32 / kPieces;  // rows that the warp's lanes cover
-#pragma unroll 4
-      for (int i = lane / kPieces; i < 32; i += kRows) {
-        const int piece = lane % kPieces, row = quad * 32 + i;
-        const uint32_t at = head_of_v0 + w * kHalf + row, down = at / static_cast<uint32_t>(G);
-        if (v0 + w * kHalf + row < vectors) {
-          *reinterpret_cast<float4*>(a.out + (run.first + row_of_v0 + down) * a.out_ld +
-                                     static_cast<int64_t>(g * G + (at - down * G)) * D + part * kDims + piece * 4) =
+      float* out = a.out + (run.first + row_of_v0) * a.out_ld + static_cast<int64_t>(g) * G * D + part * kDims;
+#pragma unroll 8
+      for (int i0 = 0; i0 < 32; i0 += kRows) {
+        const int i = i0 + lane / kPieces, piece = lane % kPieces;
+        const uint32_t place = __shfl_sync(kFull, my_place, i);
+        if (v0 + w * kHalf + quad * 32 + i < vectors) {
+          *reinterpret_cast<float4*>(out + static_cast<int64_t>(place >> 16) * a.out_ld + (place & 0xffffu) * D + piece * 4) =
               *reinterpret_cast<const float4*>(mine_rows + i * kRowBytes + ((piece ^ (i & 7)) << 4));
         }
       }

@@ -141,6 +141,7 @@ SIGNATURES = {
     "accel_llama_destroy": (None, [c_vp]),
     "accel_llama_weight": (c_int, [c_vp, c_i32, c_i32, P_f32, c_i64, c_i64]),
     "accel_llama_weight_q8": (c_int, [c_vp, c_i32, c_i32, P_i8, P_f32, c_i64, c_i64]),
+    "accel_llama_cache": (c_int, [c_vp, c_i32, c_i32, c_i32, c_i32]),
     "accel_llama_tokenizer": (c_int, [c_vp, ctypes.c_char_p]),
     "accel_llama_generate": (c_int, [c_vp, P_i32, c_i32, c_i32, c_i32, c_f32, c_u32, c_i32, P_i32, P_i32]),
     "accel_llama_generate_batch": (c_int, [c_vp, P_i32, P_i32, c_i32, c_i32, c_i32, c_f32, c_u32, P_u32, c_i32,

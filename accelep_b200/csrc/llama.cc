@@ -24,6 +24,10 @@
 // accel_llama_cache_rows returns rows in the reference's [context][kv
 // heads][head_dim] layout.
 //
+// With accel_llama_cache the KV cache is int8 with scales per block of tokens
+// and kv head: RoPE and append quantise, and both attentions read int8
+// (optionally through a window), in prefill and decode.
+//
 // Decode: the step (choose the next id of every live sequence, then one
 // forward of one row per sequence) is captured once as a CUDA graph and
 // replayed; ids, positions and lengths stay on the device, so the loop needs
@@ -328,6 +332,36 @@ class Engine {
 
   // ------------------------------------------------------------- generation
 
+  // accel_llama_cache: the present cache and context end.
+  void SetCache(int32_t kind, int32_t block, int32_t window, int32_t sinks) {
+    const bool int8 = kind == ACCEL_CACHE_INT8;
+    if (kind != ACCEL_CACHE_F32 && !int8) throw std::invalid_argument("unknown cache kind");
+    if (window < 0 || sinks < 0) throw std::invalid_argument("invalid attention window");
+    if (!int8 && (block != 0 || window != 0 || sinks != 0)) {
+      throw std::invalid_argument("blocks, windows and sinks need the int8 cache");
+    }
+    if (int8 && head_dim != 64 && head_dim != 128) {
+      throw std::invalid_argument("the int8 cache needs a head size of 64 or 128");
+    }
+    if (int8 && block != 32 && block != 64 && block != 128) {
+      throw std::invalid_argument("the int8 cache's block must be 32, 64 or 128 tokens");
+    }
+    Cuda(cudaStreamSynchronize(stream), "cache");
+    filled = 0;
+    logit_rows = 0;
+    cache_kind = kind;
+    cache_block = block;
+    attn_window = window;
+    attn_sinks = sinks;
+    k_cache.clear();
+    v_cache.clear();
+    k_scale.clear();
+    v_scale.clear();
+    slots = 0;
+    DropGraphs();
+    EnsureSlots(1);
+  }
+
   // src/llama_model.cc:150-166.
   void ForwardIds(const int32_t* ids, int32_t count, bool reset) {
     if (!Ready()) throw std::invalid_argument("llama weights are incomplete");
@@ -335,7 +369,9 @@ class Engine {
     if (reset) filled = 0;
     if (filled < 0 || count > cfg.context - filled) throw std::invalid_argument("forward exceeds context");
     CheckIds(ids, count);
+    EnsureSlots(1);
     EnsureRows(count, 1);
+    EnsureAttention(1, count);
     PinnedBuf& st = staging;
     st.Ensure(static_cast<size_t>(count) * 12 + 32);
     int32_t* h = st.as<int32_t>();
@@ -359,6 +395,7 @@ class Engine {
     Cuda(cudaMemcpyAsync(last_rows.p, h + 3 * count, 4, cudaMemcpyHostToDevice, stream), "rows");
     Forward(count, 1, false);
     Cuda(cudaStreamSynchronize(stream), "forward");
+    if (cache_kind == ACCEL_CACHE_INT8) CheckStatus();
     filled += count;
     logit_rows = 1;
   }
@@ -383,10 +420,11 @@ class Engine {
     EnsureSlots(batch);
     EnsureRows(std::max<int64_t>(rows, batch), batch);
     EnsureIds(batch, std::max(steps, 1));
+    EnsureAttention(batch, *std::max_element(counts, counts + batch));
     const bool sampled = temperature > 0.f;
 
     PinnedBuf& st = staging;
-    st.Ensure(static_cast<size_t>(rows) * 12 + static_cast<size_t>(batch) * 28 + 64);
+    st.Ensure(static_cast<size_t>(rows) * 12 + static_cast<size_t>(batch) * 32 + 64);
     int32_t* h = st.as<int32_t>();
     int32_t* h_tok = h;
     int32_t* h_seq = h + rows;
@@ -398,6 +436,7 @@ class Engine {
     int32_t* h_first = h_ident + batch;
     int32_t* h_count = h_first + batch;
     int32_t* h_pos0 = h_count + batch;
+    int32_t* h_ones = h_pos0 + batch;
     int64_t r = 0;
     prefill_max_rows = 0;
     for (int32_t b = 0; b < batch; ++b) {
@@ -415,6 +454,7 @@ class Engine {
       const uint32_t sd = seeds != nullptr ? seeds[b] : seed;
       h_rng[b] = sd == 0 ? 0x6d2b79f5u : sd;  // src/llama_model.cc:111
       h_ident[b] = b;
+      h_ones[b] = 1;
     }
     Cuda(cudaMemcpyAsync(tokens.p, h_tok, rows * 4, cudaMemcpyHostToDevice, stream), "prompt ids");
     NoteBytesToDevice(static_cast<size_t>(rows) * 4);
@@ -427,6 +467,9 @@ class Engine {
     Cuda(cudaMemcpyAsync(seq_first.p, h_first, batch * 4, cudaMemcpyHostToDevice, stream), "rows");
     Cuda(cudaMemcpyAsync(seq_count.p, h_count, batch * 4, cudaMemcpyHostToDevice, stream), "rows");
     Cuda(cudaMemcpyAsync(seq_pos0.p, h_pos0, batch * 4, cudaMemcpyHostToDevice, stream), "rows");
+    if (cache_kind == ACCEL_CACHE_INT8) {
+      Cuda(cudaMemcpyAsync(row_ones.p, h_ones, batch * 4, cudaMemcpyHostToDevice, stream), "rows");
+    }
     Cuda(cudaMemsetAsync(done.p, 0, batch * 4, stream), "state");
     Cuda(cudaMemsetAsync(count.p, 0, batch * 4, stream), "state");
     Cuda(cudaMemsetAsync(step.p, 0, 16, stream), "state");
@@ -453,10 +496,7 @@ class Engine {
     Cuda(cudaMemcpyAsync(fin.as<int32_t>() + batch, status.p, 4, cudaMemcpyDeviceToHost, stream), "status");
     Cuda(cudaStreamSynchronize(stream), "counts");
     std::memcpy(cnt.data(), fin.p, cnt.size() * 4);
-    if (fin.as<int32_t>()[batch] != 0) {
-      Cuda(cudaMemsetAsync(status.p, 0, 4, stream), "status");
-      throw std::runtime_error("a decode attention copy did not complete within its wait bound");
-    }
+    if (fin.as<int32_t>()[batch] != 0) FailStatus(fin.as<int32_t>()[batch]);
     if (single) {
       Cuda(cudaMemcpy(out_ids, ids.p, static_cast<size_t>(cnt[0]) * 4, cudaMemcpyDeviceToHost), "ids");
       NoteBytesToHost(static_cast<size_t>(cnt[0]) * 4);
@@ -503,6 +543,29 @@ class Engine {
     if (slot < 0 || slot >= slots || layer < 0 || layer >= cfg.layers || (which != 0 && which != 1) || nrows < 0 ||
         nrows > cfg.context || out == nullptr) {
       throw std::invalid_argument("invalid cache read");
+    }
+    if (cache_kind == ACCEL_CACHE_INT8) {
+      if (nrows == 0) return;
+      // The slot's own rows, read back as fp32 in the reference layout.
+      accel_b200_q8_cache one = Q8Of(layer);
+      one.k += slot * one.seq_stride;
+      one.v += slot * one.seq_stride;
+      one.k_scale += slot * one.scale_seq_stride;
+      one.v_scale += slot * one.scale_seq_stride;
+      one.slots = 1;
+      const int32_t run[3] = {0, nrows, 0};  // first, count, pos0
+      DevBuf args, rows_out;
+      args.Alloc(sizeof(run));
+      rows_out.Alloc(static_cast<size_t>(nrows) * kv_out * 4);
+      Cuda(cudaMemcpy(args.p, run, sizeof(run), cudaMemcpyHostToDevice), "cache");
+      const int32_t* at = args.as<int32_t>();
+      float* dst = rows_out.as<float>();
+      Abi(accel_b200_cache_rows_q8(&one, at, at + 1, at + 2, 1, nrows, which == 0 ? dst : nullptr,
+                                   which == 1 ? dst : nullptr, kv_out, nrows, nullptr, stream));
+      Cuda(cudaMemcpyAsync(out, dst, static_cast<size_t>(nrows) * kv_out * 4, cudaMemcpyDeviceToHost, stream),
+           "cache");
+      Cuda(cudaStreamSynchronize(stream), "cache");
+      return;
     }
     // Head-major in HBM; the reference layout [rows, kv_heads, head_dim] on the host.
     const DevBuf& c = which == 0 ? k_cache[static_cast<size_t>(layer)] : v_cache[static_cast<size_t>(layer)];
@@ -572,17 +635,82 @@ class Engine {
   void EnsureSlots(int32_t n) {
     if (n <= slots) return;
     cudaStreamSynchronize(stream);
-    const size_t per = static_cast<size_t>(n) * cfg.context * kv_out * sizeof(float);
+    const bool int8 = cache_kind == ACCEL_CACHE_INT8;
+    const size_t per = static_cast<size_t>(n) * cfg.context * kv_out * (int8 ? sizeof(int8_t) : sizeof(float));
+    slots = 0;  // until all of them are there
+    const size_t scales = int8 ? static_cast<size_t>(n) * cfg.kv_heads * Q8Blocks() * sizeof(float) : 0;
     k_cache.clear();
     v_cache.clear();
+    k_scale.clear();
+    v_scale.clear();
     k_cache.resize(static_cast<size_t>(cfg.layers));
     v_cache.resize(static_cast<size_t>(cfg.layers));
+    k_scale.resize(static_cast<size_t>(int8 ? cfg.layers : 0));
+    v_scale.resize(static_cast<size_t>(int8 ? cfg.layers : 0));
     for (int32_t l = 0; l < cfg.layers; ++l) {
       k_cache[static_cast<size_t>(l)].Alloc(per);
       v_cache[static_cast<size_t>(l)].Alloc(per);
+      if (int8) {
+        k_scale[static_cast<size_t>(l)].Alloc(scales);
+        v_scale[static_cast<size_t>(l)].Alloc(scales);
+      }
     }
     slots = n;
     DropGraphs();
+  }
+
+  int64_t Q8Blocks() const { return (cfg.context + cache_block - 1) / cache_block; }
+
+  // A layer's int8 cache.
+  accel_b200_q8_cache Q8Of(int32_t layer) {
+    const size_t l = static_cast<size_t>(layer);
+    accel_b200_q8_cache c{};
+    c.k = k_cache[l].as<int8_t>();
+    c.v = v_cache[l].as<int8_t>();
+    c.k_scale = k_scale[l].as<float>();
+    c.v_scale = v_scale[l].as<float>();
+    c.head_stride = static_cast<int64_t>(cfg.context) * head_dim;
+    c.seq_stride = c.head_stride * cfg.kv_heads;
+    c.scale_head_stride = Q8Blocks();
+    c.scale_seq_stride = c.scale_head_stride * cfg.kv_heads;
+    c.slots = slots;
+    c.kv_heads = cfg.kv_heads;
+    c.head_dim = head_dim;
+    c.context = cfg.context;
+    c.block = cache_block;
+    return c;
+  }
+
+  // The int8 cache's attention workspace and the decode rows' counts, for
+  // `seqs` sequences with at most `max_rows` prompt rows each. (Call it behind
+  // EnsureSlots.)
+  void EnsureAttention(int32_t seqs, int32_t max_rows) {
+    if (cache_kind != ACCEL_CACHE_INT8) return;
+    const accel_b200_q8_cache c = Q8Of(0);
+    const size_t need =
+        std::max(accel_b200_attention_decode_q8_workspace(&c, seqs, cfg.heads, attn_window, attn_sinks),
+                 accel_b200_attention_prefill_q8_workspace(&c, seqs, max_rows, cfg.heads, attn_window, attn_sinks));
+    bool moved = attn_ws.Ensure(need);
+    moved |= row_ones.Ensure(static_cast<size_t>(seqs) * 4);
+    if (moved) DropGraphs();
+  }
+
+  // Reads the status word of kernels that report through it.
+  void CheckStatus() {
+    int32_t bits = 0;
+    Cuda(cudaMemcpy(&bits, status.p, 4, cudaMemcpyDeviceToHost), "status");
+    if (bits != 0) FailStatus(bits);
+  }
+
+  [[noreturn]] void FailStatus(int32_t bits) {
+    Cuda(cudaMemsetAsync(status.p, 0, 4, stream), "status");
+    if ((bits & ACCEL_B200_STATUS_COPY_TIMEOUT) != 0) {
+      throw std::runtime_error("a decode attention copy did not complete within its wait bound");
+    }
+    if ((bits & ACCEL_B200_STATUS_NONFINITE) != 0) {
+      throw std::runtime_error("a key or value that is not finite was written to the int8 cache");
+    }
+    throw std::runtime_error("a kernel reported status " + std::to_string(bits));
   }
 
   void EnsureRows(int64_t rows, int32_t seqs) {
@@ -724,20 +852,43 @@ class Engine {
     Abi(accel_b200_embed(tok, 0, embed.as<float>(), hid, rows, H, cfg.vocab, nullptr, stream));
     for (int32_t li = 0; li < cfg.layers; ++li) {
       Layer& l = layers[static_cast<size_t>(li)];
-      float* kc = k_cache[static_cast<size_t>(li)].as<float>();
-      float* vc = v_cache[static_cast<size_t>(li)].as<float>();
+      const bool int8 = cache_kind == ACCEL_CACHE_INT8;
+      float* kc = int8 ? nullptr : k_cache[static_cast<size_t>(li)].as<float>();
+      float* vc = int8 ? nullptr : v_cache[static_cast<size_t>(li)].as<float>();
       // Decode: the q|k|v product lets the attention launch only after its
       // own wait, so the attention reads the cache (written by earlier
       // kernels, all completed by then) and starts its first copies before
       // it waits for the q|k|v rows.
-      const bool fused = decode && head_dim == 64;
+      const bool fused = decode && head_dim == 64 && !int8;
       accel_b200_epilogue qkv_ep{};
       qkv_ep.alpha = 1.f;
       qkv_ep.flags = ACCEL_B200_EP_TRIGGER_AFTER_WAIT;
       const bool early = fused && l.qkv.kind == WKind::Q8;
       NormGemm(hid, l.attn_norm, l.qkv, rows, qkv.as<float>(), qkv_ld, early ? &qkv_ep : nullptr, normed,
                li > 0 ? sq : nullptr);
-      if (fused) {
+      if (int8) {
+        // RoPE in place and quantising append of each sequence's rows, then
+        // attention over the int8 cache. A finished sequence's position is
+        // negative: both skip it.
+        const accel_b200_q8_cache cache = Q8Of(li);
+        float* rows_q = qkv.as<float>();
+        int32_t* st = status.as<int32_t>();
+        const int32_t* first = decode ? dec_seq.as<int32_t>() : seq_first.as<int32_t>();
+        const int32_t* cnt = decode ? row_ones.as<int32_t>() : seq_count.as<int32_t>();
+        const int32_t* pos0 = decode ? dec_pos.as<int32_t>() : seq_pos0.as<int32_t>();
+        const int32_t most = decode ? 1 : prefill_max_rows;
+        Abi(accel_b200_rope_append_q8(rows_q, qkv_ld, rows, &cache, first, cnt, pos0, seqs, most, cfg.heads,
+                                      rope_cos.as<float>(), rope_sin.as<float>(), rows_q, qkv_ld, st, stream));
+        if (decode) {
+          Abi(accel_b200_attention_decode_q8(rows_q, qkv_ld, &cache, nullptr, pos0, rows, cfg.heads, attn_window,
+                                             attn_sinks, mixed.as<float>(), q_out, attn_ws.p, attn_ws.bytes, st,
+                                             stream));
+        } else {
+          Abi(accel_b200_attention_prefill_q8(rows_q, qkv_ld, &cache, first, cnt, pos0, seqs, most, rows, cfg.heads,
+                                              attn_window, attn_sinks, mixed.as<float>(), q_out, attn_ws.p,
+                                              attn_ws.bytes, st, stream));
+        }
+      } else if (fused) {
         // Rope, AppendCache and attention of the new rows in one kernel.
         // While it runs, the int8 weights of the products that follow (this
         // layer's o, gate|up and down, then the next layer's q|k|v or, after
@@ -852,6 +1003,9 @@ class Engine {
   std::vector<Layer> layers;
   Group lm_head;
   std::vector<DevBuf> k_cache, v_cache;
+  std::vector<DevBuf> k_scale, v_scale;  // int8 cache: per layer
+  int32_t cache_kind = ACCEL_CACHE_F32, cache_block = 0, attn_window = 0, attn_sinks = 0;
+  DevBuf attn_ws, row_ones;  // int8 cache: attention workspace; one row per decoded sequence
   int32_t slots = 0;
   DevBuf hidden, normed, qkv, mixed, gu, act, gathered, normed_last, logits;
   DevBuf tokens, row_seq, row_pos, last_rows, lens, dec_seq, dec_pos, done, count, pre_ids, rng, step, finished;
@@ -942,6 +1096,15 @@ ACCEL_B200_API int accel_llama_weight_q8(AccelLlama* handle, int32_t kind, int32
     return 1;
   }
   return Guarded(e, [&] { e->WeightQ8(kind, layer, q, scale, rows, cols); });
+}
+
+ACCEL_B200_API int accel_llama_cache(AccelLlama* handle, int32_t kind, int32_t block, int32_t window, int32_t sinks) {
+  Engine* e = Cast(handle);
+  if (e == nullptr) {
+    Fail("invalid cache");
+    return 1;
+  }
+  return Guarded(e, [&] { e->SetCache(kind, block, window, sinks); });
 }
 
 ACCEL_B200_API int accel_llama_tokenizer(AccelLlama* handle, const char* path) {

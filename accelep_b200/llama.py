@@ -2,8 +2,8 @@
 
 Mirrors the reference binding (serve/llama.py:96-439): the same create /
 weight / generate / forward_ids / logit_max_abs / reset calls and counters,
-plus the backend's additions: int8 weights, batched generation, the logit
-row and cache rows as test hooks, and the model's CUDA stream. Weights come
+plus the backend's additions: int8 weights, an int8 key/value cache, batched
+generation, the logit row and cache rows as test hooks, and the model's CUDA stream. Weights come
 from numpy arrays in Hugging Face layout (the reference reads them from
 safetensors; no checkpoint is used here).
 """
@@ -83,6 +83,18 @@ class Llama:
                 self.weight(kind, layer, values)
         for (kind, layer), (q, s) in planes.items():
             self.weight_q8(kind, layer, q, s)
+
+    # ---------------------------------------------------------------- cache
+
+    def cache(self, kind="int8", block=64, window=0, sinks=0):
+        """Holds keys and values as "int8" (one scale per `block` tokens and kv
+        head; rows see the last `window` tokens, 0: all, and the first
+        `sinks`) or as "f32", the default of a new model. Ends the context."""
+        kinds = {"f32": 0, "int8": 1}
+        if kind not in kinds:
+            raise ValueError(f"cache kind must be one of {sorted(kinds)}")
+        block = block if kind == "int8" else 0
+        self._check(self._lib.accel_llama_cache(self._model, kinds[kind], block, window, sinks), "cache")
 
     # ----------------------------------------------------------- generation
 

@@ -13,6 +13,7 @@
  * Additions (no reference counterpart; they extend the same API):
  *   accel_llama_weight_q8        int8 weights with per-output-row scales
  *   accel_llama_generate_batch   many independent sequences in one decode loop
+ *   accel_llama_cache            int8 key/value cache, attention window and sinks
  *   accel_llama_stream           the CUDA stream the model runs on
  *
  * The tokenizer entry points (accel_llama_tokenizer / encode / decode /
@@ -96,6 +97,17 @@ ACCEL_B200_API int accel_llama_weight(AccelLlama* model, int32_t kind, int32_t l
    may mix fp32 and int8 linear weights. */
 ACCEL_B200_API int accel_llama_weight_q8(AccelLlama* model, int32_t kind, int32_t layer, const int8_t* q,
                                          const float* scale, int64_t rows, int64_t cols);
+/* Key/value cache kinds of accel_llama_cache. */
+enum { ACCEL_CACHE_F32 = 0, ACCEL_CACHE_INT8 = 1 };
+/* How the model holds keys and values, and what its rows see. ACCEL_CACHE_F32
+   (the default): the reference's fp32 cache; block, window and sinks are 0.
+   ACCEL_CACHE_INT8 (a quarter of the memory; head size 64 or 128): int8 with
+   one scale per `block` (32, 64 or 128) tokens and kv head, as
+   accel_b200_rope_append_q8 writes it, and attention over the last `window`
+   tokens (0: all) and the first `sinks` (accel_b200_attention_decode_q8).
+   Ends the present context (as accel_llama_reset) and frees the present
+   cache. A key or value that is not finite fails the call that wrote it. */
+ACCEL_B200_API int accel_llama_cache(AccelLlama* model, int32_t kind, int32_t block, int32_t window, int32_t sinks);
 ACCEL_B200_API int accel_llama_tokenizer(AccelLlama* model, const char* path);
 /* sim_api.h:78-83. */
 ACCEL_B200_API int accel_llama_generate(AccelLlama* model, const int32_t* prompt, int32_t prompt_count, int32_t max_new,
@@ -138,7 +150,7 @@ ACCEL_B200_API int accel_llama_logit_max_abs(AccelLlama* model, const float* ref
 ACCEL_B200_API int accel_llama_logits(AccelLlama* model, float* out, int32_t count);
 /* Copies rows [0, rows) of one layer's key (which 0) or value (which 1) cache
    of sequence slot `slot` to the host in the reference layout [rows,
-   kv_heads, head_dim]. Test hook; not counted. */
+   kv_heads, head_dim] (an int8 cache as the values it stands for). Test hook; not counted. */
 ACCEL_B200_API int accel_llama_cache_rows(AccelLlama* model, int32_t slot, int32_t layer, int32_t which, int32_t rows,
                                           float* out);
 ACCEL_B200_API void accel_llama_reset(AccelLlama* model);

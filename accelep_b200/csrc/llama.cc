@@ -473,6 +473,7 @@ class Engine {
     Cuda(cudaMemsetAsync(done.p, 0, batch * 4, stream), "state");
     Cuda(cudaMemsetAsync(count.p, 0, batch * 4, stream), "state");
     Cuda(cudaMemsetAsync(step.p, 0, 16, stream), "state");
+    Cuda(cudaMemsetAsync(finished.p, 0, 4, stream), "state");
     Forward(rows, batch, false);
     logit_rows = batch;
 

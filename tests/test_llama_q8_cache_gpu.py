@@ -136,6 +136,19 @@ def test_switching_caches_keeps_the_fp32_results(lib, cuda):
         assert np.array_equal(model.logits(), logits)
 
 
+@pytest.mark.parametrize("kind", ["f32", "int8"])
+def test_generating_again_after_sequences_ended(lib, cuda, kind):
+    """Sequences that ended (here by a full context) do not count towards the
+    next call's, whose loop looks every 32 steps whether all have."""
+    prompts = [syn.prompts(CFG, 1, n, n)[0] for n in (300, 310)]
+    with engine(CFG, syn.llama_weights(CFG, 9, std=0.08)) as model:
+        model.cache(kind)
+        short = syn.prompts(CFG, 1, 20, 6)[0]
+        want = model.generate(short, 100)
+        assert [len(x) for x in model.generate_batch(prompts, 50)] == [21, 11]
+        assert np.array_equal(model.generate(short, 100), want) and len(want) == 100
+
+
 def test_refusals(lib, cuda):
     with engine(CFG, syn.llama_weights(CFG, 1)) as model:
         with pytest.raises(ValueError):

@@ -83,9 +83,25 @@ struct alignas(16) State {
   float o[kVec][D];
 };
 
-// Grid (split, kv head x vector group, sequence or row). kRuns: a sequence's
-// rows (prefill), else single rows.
-template <int D, bool kRuns>
+// Units of 32 tokens of which some are seen: those of the sinks that lie before
+// the unit of `near`, then from that on to the unit of pos.
+struct Units {
+  int near, sinks, count;
+};
+__device__ __forceinline__ Units UnitsOf(int near, int pos, int sinks) {
+  Units u;
+  u.near = near / kUnit;
+  u.sinks = static_cast<int>(Min64((static_cast<int64_t>(sinks) + kUnit - 1) / kUnit, u.near));
+  u.count = u.sinks + pos / kUnit - u.near + 1;
+  return u;
+}
+
+// What a launch's rows are: single rows or runs of a sequence's rows, in grid
+// (split, kv head x vector group, row or sequence); or single rows, at most 32,
+// over a flat grid whose CTAs go to the rows by how much each row sees.
+enum class Rows { kSingle, kRuns, kBalanced };
+
+template <int D, Rows kRows>
 __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
     const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const AttnArgs a) {
   constexpr int kKw = D / 16;      // 32-bit words of a lane's share of a key row
@@ -102,10 +118,53 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   PdlWait();
   const accel_b200_q8_cache& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
-  const int S = static_cast<int>(gridDim.x), split = static_cast<int>(blockIdx.x);
+  constexpr bool kRuns = kRows == Rows::kRuns;
   const int G = a.heads / c.kv_heads;
-  const int g = static_cast<int>(blockIdx.y) % c.kv_heads, group = static_cast<int>(blockIdx.y) / c.kv_heads;
-  const bool reports = split == 0 && blockIdx.y == 0 && tid == 0;
+  int S = static_cast<int>(gridDim.x), split = static_cast<int>(blockIdx.x), pair = static_cast<int>(blockIdx.y);
+  int64_t z = blockIdx.z;
+  if constexpr (kRows == Rows::kBalanced) {
+    // Lane r counts row r's units (rows that are not attended: none). CTAs of
+    // q units each, q the least of 32 sizes, from an even share of all units to
+    // twice that, whose CTAs do not exceed the grid: rows get ceil(units / q).
+    const int pairs = c.kv_heads * ((G + kVec - 1) / kVec), T = static_cast<int>(gridDim.x);
+    int mine_units = 0;
+    if (lane < a.single_rows) {
+      const int pos = a.row_pos[lane];
+      const int64_t slot = a.row_seq != nullptr ? a.row_seq[lane] : lane;
+      if (pos >= 0 && (pos >= c.context || slot < 0 || slot >= c.slots)) {
+        if (blockIdx.x == 0 && warp == 0 && a.status != nullptr) atomicOr(a.status, ACCEL_B200_STATUS_BAD_POSITION);
+      } else if (pos >= 0) {
+        mine_units = UnitsOf(NearOf(pos, a.window), pos, a.sinks).count;
+      }
+    }
+    int64_t total = mine_units;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
+    const int even = static_cast<int>(Max64(kWarps * kWarpUnits, (total * pairs + T - 1) / T));
+    const int size = even + (even * lane + 31) / 32;
+    int64_t ctas = 0;
+    for (int r = 0; r < a.single_rows; ++r) ctas += (__shfl_sync(kFull, mine_units, r) + size - 1) / size;
+    // (Twice the even share always fits: it needs T / 2 CTAs and one more for
+    // each row and pair, of which there are fewer than T / 8.)
+    const int fits = __ffs(__ballot_sync(kFull, ctas * pairs <= T)) - 1;
+    const int q = __shfl_sync(kFull, size, fits < 0 ? 31 : fits);
+    const int share = (mine_units + q - 1) / q;  // CTAs per pair of row `lane`
+    int end = share * pairs;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(kFull, end, o);
+      if (lane >= o) end += before;
+    }
+    const int row = __ffs(__ballot_sync(kFull, end > static_cast<int>(blockIdx.x))) - 1;
+    if (row < 0) return;
+    S = __shfl_sync(kFull, share, row);
+    const int local = static_cast<int>(blockIdx.x) - (__shfl_sync(kFull, end, row) - S * pairs);
+    pair = local / S;
+    split = local % S;
+    z = row;
+  }
+  const int g = pair % c.kv_heads, group = pair / c.kv_heads;
+  const bool reports = split == 0 && pair == 0 && tid == 0;
 
   // The rows: `count` from `first` at positions pos0 + i of `slot`. A single
   // row's query does not wait for its position.
@@ -118,17 +177,17 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
                                               : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  if (!kRuns) load_query(blockIdx.z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
+  if (!kRuns) load_query(z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
   int64_t first, slot;
   int count, pos0;
   if (kRuns) {
-    slot = blockIdx.z;
+    slot = z;
     const Run run = RunOf(a.rows, static_cast<int>(slot), c.context, reports, a.status);
     first = run.first;
     count = run.count;
     pos0 = run.pos0;
   } else {
-    first = blockIdx.z;
+    first = z;
     pos0 = a.row_pos[first];
     slot = a.row_seq != nullptr ? a.row_seq[first] : first;
     count = pos0 >= 0 ? 1 : 0;
@@ -150,9 +209,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   const int near_lo = NearOf(pos_lo, a.window), near_hi = NearOf(pos_hi, a.window);
 
   // Units that some vector sees: sinks before the windows, then the windows.
-  const int unit0 = near_lo / kUnit;
-  const int sink_units = min((a.sinks + 0ll + kUnit - 1) / kUnit, static_cast<long long>(unit0));
-  const int units = sink_units + pos_hi / kUnit - unit0 + 1;
+  const Units seen = UnitsOf(near_lo, pos_hi, a.sinks);
+  const int unit0 = seen.near, sink_units = seen.sinks, units = seen.count;
   const int step = S * kWarps;
 
   const float* ksp = c.k_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
@@ -426,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   }
   if (S == 1) return;
 
-  if (S <= kMaxCluster) {
+  if (kRows != Rows::kBalanced && S <= kMaxCluster) {
     ClusterSync();  // every CTA's state is there
     // CTA `split` merges every S-th group of 4 elements, all peers' loads in flight.
     for (int e = 4 * (split + S * tid); e < kVec * D; e += 4 * S * kThreads) {
@@ -456,11 +514,15 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
     return;
   }
 
-  // Through the workspace: states [group][split], the last CTA merges them.
+  // Through the workspace: a state per CTA, those of a group side by side; the
+  // group's last CTA to arrive merges them.
   constexpr int kFloats = sizeof(State<D>) / 4;
-  const int64_t at = blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z;
+  const bool flat = kRows == Rows::kBalanced;
+  const int64_t at = flat ? static_cast<int64_t>(z) * c.kv_heads * ((G + kVec - 1) / kVec) + pair
+                          : blockIdx.y + static_cast<int64_t>(gridDim.y) * blockIdx.z;
+  const int64_t part0 = flat ? static_cast<int64_t>(blockIdx.x) - split : at * S;
   __syncthreads();
-  float* part = a.parts + (at * S + split) * kFloats;
+  float* part = a.parts + (part0 + split) * kFloats;
   for (int e = tid; e < kFloats / 4; e += kThreads) {
     reinterpret_cast<float4*>(part)[e] = reinterpret_cast<const float4*>(&cta_state)[e];
   }
@@ -471,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   if (!last) return;
   if (tid == 0) a.counters[at] = 0;
   __threadfence();
-  const float* parts = a.parts + at * S * kFloats;
+  const float* parts = a.parts + part0 * kFloats;
   // The factor and the sum of each (vector, CTA), then the weighted values with
   // eight CTAs' loads in flight.
   float* factors = reinterpret_cast<float*>(smem);  // [S][kVec], then the sums of the vectors
@@ -509,11 +571,12 @@ struct Split {
   int64_t groups;  // grid y * z
   int vec_groups;  // per (sequence or row, kv head)
   int s;
+  int balanced;    // CTAs of a balanced launch (0: none)
   size_t workspace;
 };
 
 Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run, int32_t heads, int32_t window,
-               int32_t sinks) {
+               int32_t sinks, bool single) {
   Split p{};
   p.vec_groups = static_cast<int>(CeilDiv(rows_per_run * (heads / c.kv_heads), kVec));
   p.groups = runs * c.kv_heads * p.vec_groups;
@@ -527,22 +590,28 @@ Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run,
   p.s = static_cast<int>(s);
   if (s > kMaxCluster) {
     const size_t state = static_cast<size_t>(2 * kVec + kVec * c.head_dim) * sizeof(float);
-    p.workspace = kCounterRegion + static_cast<size_t>(p.groups) * static_cast<size_t>(s) * state;
+    // Single rows of few long sequences take CTAs by their own lengths (88 ->
+    // XX us at 4 sequences of 40001 to 65536 tokens).
+    if (rows_per_run == 1 && runs <= 32 && single) p.balanced = static_cast<int>(resident);
+    p.workspace = kCounterRegion + static_cast<size_t>(resident) * state;
   }
   return p;
 }
 
-template <int D, bool kRuns>
+template <int D, Rows kRows>
 int LaunchVectors(AttnArgs a, const Split& p, int64_t runs, void* workspace, cudaStream_t stream, const char* what) {
   if (p.workspace > 0) {
     a.counters = static_cast<int32_t*>(workspace);
     a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterRegion);
   }
-  const dim3 grid(static_cast<unsigned>(p.s), static_cast<unsigned>(a.cache.kv_heads * p.vec_groups),
-                  static_cast<unsigned>(runs));
-  const unsigned cluster = p.s <= kMaxCluster ? static_cast<unsigned>(p.s) : 1u;
+  a.single_rows = static_cast<int32_t>(runs);
+  const dim3 grid = kRows == Rows::kBalanced
+                        ? dim3(static_cast<unsigned>(p.balanced))
+                        : dim3(static_cast<unsigned>(p.s), static_cast<unsigned>(a.cache.kv_heads * p.vec_groups),
+                               static_cast<unsigned>(runs));
+  const unsigned cluster = kRows != Rows::kBalanced && p.s <= kMaxCluster ? static_cast<unsigned>(p.s) : 1u;
   constexpr int kSmem = Queue<D>::kBytes + Queue<D>::kAlign;
-  const cudaError_t err = cudaFuncSetAttribute(AttnVectorsQ8Kernel<D, kRuns>,
+  const cudaError_t err = cudaFuncSetAttribute(AttnVectorsQ8Kernel<D, kRows>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (err != cudaSuccess) return CheckLaunchEx(err, what);
   const CUtensorMapSwizzle swizzle = D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
@@ -553,7 +622,7 @@ int LaunchVectors(AttnArgs a, const Split& p, int64_t runs, void* workspace, cud
     return SetError(ACCEL_B200_EINVAL, std::string(what) + ": cache tensor map rejected");
   }
   return CheckLaunchEx(
-      LaunchK(AttnVectorsQ8Kernel<D, kRuns>, grid, dim3(kThreads), kSmem, stream, cluster, 1u, tk, tv, a), what);
+      LaunchK(AttnVectorsQ8Kernel<D, kRows>, grid, dim3(kThreads), kSmem, stream, cluster, 1u, tk, tv, a), what);
 }
 
 int CheckWorkspace(const Split& p, const void* workspace, size_t bytes, const std::string& what) {
@@ -620,7 +689,7 @@ ACCEL_B200_API size_t accel_b200_attention_decode_q8_workspace(const accel_b200_
       heads % cache->kv_heads != 0 || window < 0 || sinks < 0) {
     return 0;
   }
-  return SplitFor(*cache, rows, 1, heads, window, sinks).workspace;
+  return SplitFor(*cache, rows, 1, heads, window, sinks, true).workspace;
 }
 
 ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
@@ -636,7 +705,7 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
   }
   if (rows == 0) return ClearError();
   if (rows > 65535) return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: more than 65535 rows");
-  const Split p = SplitFor(*cache, rows, 1, heads, window, sinks);
+  const Split p = SplitFor(*cache, rows, 1, heads, window, sinks, true);
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
     return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: grid too large");
   }
@@ -644,8 +713,13 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
   if (rc != ACCEL_B200_OK) return rc;
   const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{}, row_seq, row_pos, heads, window, sinks, out, out_ld, status);
   const char* what = "attention_decode_q8";
-  if (cache->head_dim == 64) return LaunchVectors<64, false>(a, p, rows, workspace, AsStream(stream), what);
-  return LaunchVectors<128, false>(a, p, rows, workspace, AsStream(stream), what);
+  cudaStream_t st = AsStream(stream);
+  if (p.balanced > 0) {
+    return cache->head_dim == 64 ? LaunchVectors<64, Rows::kBalanced>(a, p, rows, workspace, st, what)
+                                 : LaunchVectors<128, Rows::kBalanced>(a, p, rows, workspace, st, what);
+  }
+  return cache->head_dim == 64 ? LaunchVectors<64, Rows::kSingle>(a, p, rows, workspace, st, what)
+                               : LaunchVectors<128, Rows::kSingle>(a, p, rows, workspace, st, what);
 }
 
 ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200_q8_cache* cache, int32_t batch,
@@ -657,7 +731,7 @@ ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200
   }
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));
   if (TakesTiles(*cache, max_rows, heads)) return 0;
-  return SplitFor(*cache, batch, max_rows, heads, window, sinks).workspace;
+  return SplitFor(*cache, batch, max_rows, heads, window, sinks, false).workspace;
 }
 
 ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
@@ -678,15 +752,16 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
   const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads,
                             window, sinks, out, out_ld, status);
   if (TakesTiles(*cache, max_rows, heads)) return LaunchTilesQ8(a, batch, max_rows, AsStream(stream));
-  const Split p = SplitFor(*cache, batch, max_rows, heads, window, sinks);
+  const Split p = SplitFor(*cache, batch, max_rows, heads, window, sinks, false);
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: grid too large");
   }
   rc = CheckWorkspace(p, workspace, workspace_bytes, "attention_prefill_q8");
   if (rc != ACCEL_B200_OK) return rc;
   const char* what = "attention_prefill_q8";
-  if (cache->head_dim == 64) return LaunchVectors<64, true>(a, p, batch, workspace, AsStream(stream), what);
-  return LaunchVectors<128, true>(a, p, batch, workspace, AsStream(stream), what);
+  cudaStream_t st = AsStream(stream);
+  return cache->head_dim == 64 ? LaunchVectors<64, Rows::kRuns>(a, p, batch, workspace, st, what)
+                               : LaunchVectors<128, Rows::kRuns>(a, p, batch, workspace, st, what);
 }
 
 }  // extern "C"

@@ -24,6 +24,7 @@ struct AttnArgs {
   RaggedRows rows;         // prefill: rows by sequence
   const int32_t* row_seq;  // single rows: slot (null: the row's number) and position
   const int32_t* row_pos;
+  int32_t single_rows;     // how many of them
   int32_t heads;
   int32_t window;
   int32_t sinks;

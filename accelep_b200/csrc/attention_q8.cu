@@ -17,9 +17,9 @@
 // free to choose, and is chosen so that a lane's share of an MMA operand is a
 // run of bytes, the shared-memory reads have no bank conflicts under TMA's
 // swizzle, and the scores' register layout is the weights' operand layout.
-// (Measured at 4 sequences of 40001..65536 tokens, 8 kv heads of 128: 88 us,
-// 4.9 TB/s. With loads to registers 128 us and with per-lane cp.async 132 us:
-// an SM keeps too few of those in flight.) Units are dealt to all warps of the
+// (Measured at 4 sequences of 40001..65536 tokens, 8 kv heads of 128: 80 us,
+// 5.4 TB/s. Before the split by lengths it took 88 us, with loads to registers
+// 128 and with per-lane cp.async 132: an SM keeps too few of those in flight.) Units are dealt to all warps of the
 // S CTAs of a vector group in turn. Each unit's weighted values are summed on
 // their own and added, times the unit's value scale, to fp32 registers (the
 // tensor core's running sum rounds towards zero, which would drift over a long
@@ -50,6 +50,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnit = 32;      // tokens per step of a warp
 constexpr int kVec = 8;        // query vectors of a CTA
 constexpr int kMaxCluster = 8; // CTAs whose states merge through distributed shared memory
+constexpr int64_t kBalanceFrom = 16384;  // tokens from which single rows take CTAs by their lengths
 constexpr int kWarpUnits = 2;  // units a warp gets at least before the tokens are split further
 template <int D>
 constexpr int kResident = D == 64 ? 3 : 2;  // CTAs per SM
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
     int64_t ctas = 0;
     for (int r = 0; r < a.single_rows; ++r) ctas += (__shfl_sync(kFull, mine_units, r) + size - 1) / size;
     // (Twice the even share always fits: it needs T / 2 CTAs and one more for
-    // each row and pair, of which there are fewer than T / 8.)
+    // each row and pair, of which there are T / 2 at most.)
     const int fits = __ffs(__ballot_sync(kFull, ctas * pairs <= T)) - 1;
     const int q = __shfl_sync(kFull, size, fits < 0 ? 31 : fits);
     const int share = (mine_units + q - 1) / q;  // CTAs per pair of row `lane`
@@ -526,43 +527,49 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   for (int e = tid; e < kFloats / 4; e += kThreads) {
     reinterpret_cast<float4*>(part)[e] = reinterpret_cast<const float4*>(&cta_state)[e];
   }
-  __threadfence();
   __syncthreads();
-  if (tid == 0) last = atomicAdd(a.counters + at, 1) == S - 1;
-  __syncthreads();
-  if (!last) return;
-  if (tid == 0) a.counters[at] = 0;
-  __threadfence();
-  const float* parts = a.parts + part0 * kFloats;
-  // The factor and the sum of each (vector, CTA), then the weighted values with
-  // eight CTAs' loads in flight.
-  float* factors = reinterpret_cast<float*>(smem);  // [S][kVec], then the sums of the vectors
-  float* sums = factors + S * kVec;
-  for (int vec = warp; vec < kVec; vec += kWarps) {
-    float mx = -INFINITY, sum = 0.f;
-    for (int p = lane; p < S; p += 32) mx = fmaxf(mx, __ldcg(parts + static_cast<int64_t>(p) * kFloats + vec));
-    mx = WarpMax(mx);
-    for (int p = lane; p < S; p += 32) {
-      const float* q = parts + static_cast<int64_t>(p) * kFloats;
-      const float pm = __ldcg(q + vec);
-      const float f = factor_of(pm, mx);
-      factors[p * kVec + vec] = f;
-      sum = fmaf(__ldcg(q + kVec + vec), f, sum);
-    }
-    sum = WarpSum(sum);
-    if (lane == 0) sums[vec] = sum;
+  if (tid == 0) {
+    __threadfence();  // the barrier put the CTA's stores before it
+    last = atomicAdd(a.counters + at, 1) == S - 1;
+    if (last) a.counters[at] = 0;
+    __threadfence();
   }
   __syncthreads();
+  if (!last) return;
+  const float* parts = a.parts + part0 * kFloats;
 #pragma unroll
   for (int e = 4 * tid; e < kVec * D; e += 4 * kThreads) {
     const int vec = e / D;
+    float mx = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int p = 0; p < S; ++p) {
-      add4(&acc, factors[p * kVec + vec],
-           __ldcg(reinterpret_cast<const float4*>(parts + static_cast<int64_t>(p) * kFloats + 2 * kVec + e)));
+    for (int p0 = 0; p0 < S; p0 += 8) {
+      // Eight CTAs' loads in flight, then their states in order.
+      float pm[8], pl[8];
+      float4 po[8];
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        const float* part_p = parts + static_cast<int64_t>(min(p0 + p, S - 1)) * kFloats;
+        pm[p] = __ldcg(part_p + vec);
+        pl[p] = __ldcg(part_p + kVec + vec);
+        po[p] = __ldcg(reinterpret_cast<const float4*>(part_p + 2 * kVec + e));
+      }
+      float now = mx;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) now = fmaxf(now, pm[p]);
+      const float corr = factor_of(mx, now);
+      sum *= corr;
+      acc = make_float4(acc.x * corr, acc.y * corr, acc.z * corr, acc.w * corr);
+      mx = now;
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        if (p0 + p < S) {
+          const float f = factor_of(pm[p], mx);
+          sum = fmaf(pl[p], f, sum);
+          add4(&acc, f, po[p]);
+        }
+      }
     }
-    store(e, sums[vec], acc);
+    store(e, sum, acc);
   }
 }
 
@@ -588,11 +595,15 @@ Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run,
   int64_t s = Max64(1, Min64(resident / Max64(1, p.groups), most));
   if (p.groups > kMaxCounters) s = Min64(s, kMaxCluster);
   p.s = static_cast<int>(s);
-  if (s > kMaxCluster) {
+  // Single rows of few, long sequences take CTAs by their own lengths, where the
+  // grid has room for a CTA more per row and pair. (Measured with 8 kv heads
+  // of 128: 16 sequences of 2048..16384 tokens 91 -> 61 us, of 4096..32768 178
+  // -> 127; where all have the same length the states' way through the
+  // workspace instead of the cluster costs 3 us of 51 to 97.)
+  const bool few = single && runs <= 32 && p.groups <= resident / 2;
+  if (few && (s > kMaxCluster || seen >= kBalanceFrom)) p.balanced = static_cast<int>(resident);
+  if (s > kMaxCluster || p.balanced > 0) {
     const size_t state = static_cast<size_t>(2 * kVec + kVec * c.head_dim) * sizeof(float);
-    // Single rows of few long sequences take CTAs by their own lengths (88 ->
-    // XX us at 4 sequences of 40001 to 65536 tokens).
-    if (rows_per_run == 1 && runs <= 32 && single) p.balanced = static_cast<int>(resident);
     p.workspace = kCounterRegion + static_cast<size_t>(resident) * state;
   }
   return p;

@@ -115,6 +115,9 @@ SIGNATURES = {
     "accel_b200_attention_decode_q8_workspace": (c_sz, [P_q8c, c_i64, c_i32, c_i32, c_i32]),
     "accel_b200_attention_decode_q8": (c_int, [c_vp, c_i64, P_q8c, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_i64,
                                                c_vp, c_sz, c_vp, c_vp]),
+    "accel_b200_attention_decode_q8_prefetch": (c_int, [c_vp, c_i64, P_q8c, c_vp, c_vp, c_i64, c_i32, c_i32, c_i32,
+                                                        c_vp, c_i64, c_vp, c_sz, c_vp, ctypes.POINTER(L2Prefetch),
+                                                        c_vp]),
     "accel_b200_attention_prefill_q8_workspace": (c_sz, [P_q8c, c_i32, c_i32, c_i32, c_i32, c_i32]),
     "accel_b200_attention_prefill_q8": (c_int, [c_vp, c_i64, P_q8c, c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32,
                                                 c_i32, c_i32, c_vp, c_i64, c_vp, c_sz, c_vp, c_vp]),

@@ -39,6 +39,7 @@
 #include "attention_q8.cuh"
 #include "cluster.cuh"
 #include "common.cuh"
+#include "l2_prefetch.cuh"
 #include "q8_cache.cuh"
 #include "tensor_map.cuh"
 
@@ -116,7 +117,11 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   State<D>& cta_state = warp_state[kWarps];
   __shared__ bool last;
   PdlTrigger();
-  PdlWait();
+  // With CACHE_BEFORE_WAIT everything but the queries and the rows' own blocks
+  // is as the kernels before the previous one left it, and those have completed.
+  const bool early = kRows != Rows::kRuns && (a.prefetch.flags & ACCEL_B200_ATTN_CACHE_BEFORE_WAIT) != 0;
+  if (kRows != Rows::kRuns && threadIdx.x == 0 && a.prefetch.count > 0) PrefetchShare(a.prefetch);
+  if (!early) PdlWait();
   const accel_b200_q8_cache& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   constexpr bool kRuns = kRows == Rows::kRuns;
@@ -157,7 +162,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
       if (lane >= o) end += before;
     }
     const int row = __ffs(__ballot_sync(kFull, end > static_cast<int>(blockIdx.x))) - 1;
-    if (row < 0) return;
+    if (row < 0) {
+      if (early) PdlWait();  // no CTA leaves in front of the previous kernel's end
+      return;
+    }
     S = __shfl_sync(kFull, share, row);
     const int local = static_cast<int>(blockIdx.x) - (__shfl_sync(kFull, end, row) - S * pairs);
     pair = local / S;
@@ -178,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
                                               : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  if (!kRuns) load_query(z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
+  if (!kRuns && !early) load_query(z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
   int64_t first, slot;
   int count, pos0;
   if (kRuns) {
@@ -200,7 +208,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   // Vectors v0 .. v0 + 7 of the run's count * G (row v / G, head v % G). A
   // whole cluster leaves here or none of it.
   const int64_t v0 = static_cast<int64_t>(group) * kVec, vectors = static_cast<int64_t>(count) * G;
-  if (v0 >= vectors) return;
+  if (v0 >= vectors) {
+    if (early) PdlWait();
+    return;
+  }
   const int row_lo = static_cast<int>(v0 / G);
   const int row_hi = static_cast<int>(Min64(v0 + kVec - 1, vectors - 1) / G);
   const bool mine = v0 + gid < vectors;
@@ -238,8 +249,21 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
     FenceBarrierInit();
   }
   int u = split * kWarps + warp;
+  // Units in front of the row's own block do not wait for the previous kernel.
+  const int settled = early ? pos_lo / c.block * c.block : 0;
+  const auto settles = [&](int i) { return u + i * step < units && unit_of(u + i * step) * kUnit < settled; };
+  if (early) {
 #pragma unroll
-  for (int i = 0; i < Qu::kStages - 1; ++i) issue(u + i * step, i);
+    for (int i = 0; i < Qu::kStages - 1; ++i) {
+      if (settles(i)) issue(u + i * step, i);
+    }
+    PdlWait();
+    load_query(z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
+  }
+#pragma unroll
+  for (int i = 0; i < Qu::kStages - 1; ++i) {
+    if (!early || !settles(i)) issue(u + i * step, i);
+  }
 
   // Which token, and which dimensions, a lane's place in an MMA operand stands
   // for is free, as long as keys and queries, and weights and values, agree. It
@@ -703,11 +727,12 @@ ACCEL_B200_API size_t accel_b200_attention_decode_q8_workspace(const accel_b200_
   return SplitFor(*cache, rows, 1, heads, window, sinks, true).workspace;
 }
 
-ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
+ACCEL_B200_API int accel_b200_attention_decode_q8_prefetch(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
                                                   const int32_t* row_seq, const int32_t* row_pos, int64_t rows,
                                                   int32_t heads, int32_t window, int32_t sinks, float* out,
                                                   int64_t out_ld, void* workspace, size_t workspace_bytes,
-                                                  int32_t* status, void* stream) {
+                                                  int32_t* status, const accel_b200_l2_prefetch* prefetch,
+                                                  void* stream) {
   int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, "attention_decode_q8");
   if (rc != ACCEL_B200_OK) return rc;
   if (rows < 0 || row_pos == nullptr) return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: bad arguments");
@@ -716,13 +741,18 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
   }
   if (rows == 0) return ClearError();
   if (rows > 65535) return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: more than 65535 rows");
+  if (prefetch != nullptr) {
+    rc = CheckPrefetch(*prefetch, "attention_decode_q8");
+    if (rc != ACCEL_B200_OK) return rc;
+  }
   const Split p = SplitFor(*cache, rows, 1, heads, window, sinks, true);
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
     return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: grid too large");
   }
   rc = CheckWorkspace(p, workspace, workspace_bytes, "attention_decode_q8");
   if (rc != ACCEL_B200_OK) return rc;
-  const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{}, row_seq, row_pos, heads, window, sinks, out, out_ld, status);
+  AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{}, row_seq, row_pos, heads, window, sinks, out, out_ld, status);
+  if (prefetch != nullptr) a.prefetch = *prefetch;
   const char* what = "attention_decode_q8";
   cudaStream_t st = AsStream(stream);
   if (p.balanced > 0) {
@@ -731,6 +761,15 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
   }
   return cache->head_dim == 64 ? LaunchVectors<64, Rows::kSingle>(a, p, rows, workspace, st, what)
                                : LaunchVectors<128, Rows::kSingle>(a, p, rows, workspace, st, what);
+}
+
+ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
+                                                  const int32_t* row_seq, const int32_t* row_pos, int64_t rows,
+                                                  int32_t heads, int32_t window, int32_t sinks, float* out,
+                                                  int64_t out_ld, void* workspace, size_t workspace_bytes,
+                                                  int32_t* status, void* stream) {
+  return accel_b200_attention_decode_q8_prefetch(q, q_ld, cache, row_seq, row_pos, rows, heads, window, sinks, out,
+                                                 out_ld, workspace, workspace_bytes, status, nullptr, stream);
 }
 
 ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200_q8_cache* cache, int32_t batch,

@@ -34,6 +34,7 @@ struct AttnArgs {
   int32_t* status;
   int32_t* counters;  // splits through the workspace: arrivals by vector group, then the CTAs' states
   float* parts;
+  accel_b200_l2_prefetch prefetch;  // single rows: ranges for L2, and whether blocks are read before the wait
 };
 
 __device__ __forceinline__ float Exp2(float x) {

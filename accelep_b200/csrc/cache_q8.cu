@@ -81,8 +81,11 @@ __global__ void __launch_bounds__(kThreads) RopeAppendQ8Kernel(AppendArgs a) {
   constexpr int kHalf = D / 2;
   constexpr int kPerRow = D / 8;  // items of a row
   __shared__ uint32_t red[kThreads / 32];
-  PdlTrigger();
+  // The next kernel starts only behind this wait, so that every kernel before
+  // this one has completed by then (the decode attention reads the blocks that
+  // this one leaves alone meanwhile).
   PdlWait();
+  PdlTrigger();
   const accel_b200_q8_cache& c = a.cache;
   const int b = blockIdx.z, y = blockIdx.y;
   const Run run = RunOf(a.rows, b, c.context, blockIdx.x == 0 && y == 0 && threadIdx.x == 0, a.status);

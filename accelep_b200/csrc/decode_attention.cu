@@ -33,6 +33,7 @@
 #include "accel_b200.h"
 #include "cluster.cuh"
 #include "common.cuh"
+#include "l2_prefetch.cuh"
 #include "tma.cuh"
 
 namespace accel_b200 {
@@ -68,23 +69,6 @@ struct FusedArgs {
   int32_t* status;
   accel_b200_l2_prefetch prefetch;  // ranges brought into L2 before the wait (count 0: none)
 };
-
-constexpr int64_t kPrefetchChunk = 32 * 1024;  // bytes per L2 prefetch instruction
-
-// This CTA's share of the prefetch ranges: chunk c of the ranges' 32 KiB
-// chunks goes to CTA c mod (CTAs).
-__device__ __forceinline__ void PrefetchShare(const accel_b200_l2_prefetch& pf) {
-  const int64_t cta = blockIdx.x + static_cast<int64_t>(gridDim.x) * (blockIdx.y + static_cast<int64_t>(gridDim.y) *
-                                                                                       blockIdx.z);
-  const int64_t ctas = static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z;
-  for (int i = 0; i < pf.count && i < 4; ++i) {
-    const char* base = static_cast<const char*>(pf.ptr[i]);
-    for (int64_t off = cta * kPrefetchChunk; off < pf.bytes[i]; off += ctas * kPrefetchChunk) {
-      const uint32_t n = static_cast<uint32_t>(Min64(kPrefetchChunk, pf.bytes[i] - off)) & ~15u;
-      if (n > 0) PrefetchL2(base + off, n);
-    }
-  }
-}
 
 template <int G>
 __global__ void __launch_bounds__(kThreads, 3) AttnDecodeFusedKernel(FusedArgs a) {
@@ -462,15 +446,8 @@ ACCEL_B200_API int accel_b200_decode_attention_prefetch(
   if (group > kMaxG) return SetError(ACCEL_B200_EINVAL, "decode_attention: more than 8 query heads per kv head");
   accel_b200_l2_prefetch pf{};
   if (prefetch != nullptr) {
-    if (prefetch->count < 0 || prefetch->count > 4 || (prefetch->flags & ~ACCEL_B200_ATTN_CACHE_BEFORE_WAIT) != 0) {
-      return SetError(ACCEL_B200_EINVAL, "decode_attention: bad prefetch");
-    }
-    for (int i = 0; i < prefetch->count; ++i) {
-      if (prefetch->bytes[i] < 0 || (prefetch->bytes[i] > 0 && prefetch->ptr[i] == nullptr) ||
-          reinterpret_cast<uintptr_t>(prefetch->ptr[i]) % 16 != 0) {
-        return SetError(ACCEL_B200_EINVAL, "decode_attention: prefetch ranges must be 16-byte aligned");
-      }
-    }
+    const int rc = CheckPrefetch(*prefetch, "decode_attention");
+    if (rc != ACCEL_B200_OK) return rc;
     pf = *prefetch;
   }
   FusedArgs a{qkv,     qkv_ld,  row_seq,    row_pos,     cos_table, sin_table, k_cache,

@@ -823,6 +823,23 @@ class Engine {
     return true;
   }
 
+  // What a decode attention brings into L2 while it runs: the int8 weights of
+  // the products that follow (this layer's o, gate|up and down, then the next
+  // layer's q|k|v or, after the last layer, the LM head).
+  accel_b200_l2_prefetch NextWeights(int32_t li) {
+    Layer& l = layers[static_cast<size_t>(li)];
+    accel_b200_l2_prefetch pf{};
+    const Group* next[4] = {&l.o, &l.gu, &l.down,
+                            li + 1 < cfg.layers ? &layers[static_cast<size_t>(li) + 1].qkv : &lm_head};
+    for (const Group* g : next) {
+      if (g == nullptr || g->kind != WKind::Q8) continue;
+      pf.ptr[pf.count] = g->w.p;
+      pf.bytes[pf.count] = g->k * g->n;
+      ++pf.count;
+    }
+    return pf;
+  }
+
   // src/llama_model.cc:209-247 over `rows` rows of `seqs` sequences. The
   // last row of each sequence gives its logit row. decode: rows == seqs,
   // row b is sequence b's new token at dec_pos[b].
@@ -881,9 +898,13 @@ class Engine {
         Abi(accel_b200_rope_append_q8(rows_q, qkv_ld, rows, &cache, first, cnt, pos0, seqs, most, cfg.heads,
                                       rope_cos.as<float>(), rope_sin.as<float>(), rows_q, qkv_ld, st, stream));
         if (decode) {
-          Abi(accel_b200_attention_decode_q8(rows_q, qkv_ld, &cache, nullptr, pos0, rows, cfg.heads, attn_window,
-                                             attn_sinks, mixed.as<float>(), q_out, attn_ws.p, attn_ws.bytes, st,
-                                             stream));
+          // The blocks in front of the rows' own are read while the append
+          // runs, and the next products' int8 weights go to L2 meanwhile.
+          accel_b200_l2_prefetch pf = NextWeights(li);
+          pf.flags = ACCEL_B200_ATTN_CACHE_BEFORE_WAIT;
+          Abi(accel_b200_attention_decode_q8_prefetch(rows_q, qkv_ld, &cache, nullptr, pos0, rows, cfg.heads,
+                                                      attn_window, attn_sinks, mixed.as<float>(), q_out, attn_ws.p,
+                                                      attn_ws.bytes, st, &pf, stream));
         } else {
           Abi(accel_b200_attention_prefill_q8(rows_q, qkv_ld, &cache, first, cnt, pos0, seqs, most, rows, cfg.heads,
                                               attn_window, attn_sinks, mixed.as<float>(), q_out, attn_ws.p,
@@ -891,18 +912,7 @@ class Engine {
         }
       } else if (fused) {
         // Rope, AppendCache and attention of the new rows in one kernel.
-        // While it runs, the int8 weights of the products that follow (this
-        // layer's o, gate|up and down, then the next layer's q|k|v or, after
-        // the last layer, the LM head) go to L2.
-        accel_b200_l2_prefetch pf{};
-        const Group* next[4] = {&l.o, &l.gu, &l.down,
-                                li + 1 < cfg.layers ? &layers[static_cast<size_t>(li) + 1].qkv : &lm_head};
-        for (const Group* g : next) {
-          if (g == nullptr || g->kind != WKind::Q8) continue;
-          pf.ptr[pf.count] = g->w.p;
-          pf.bytes[pf.count] = g->k * g->n;
-          ++pf.count;
-        }
+        accel_b200_l2_prefetch pf = NextWeights(li);
         if (early) pf.flags = ACCEL_B200_ATTN_CACHE_BEFORE_WAIT;
         Abi(accel_b200_decode_attention_prefetch(qkv.as<float>(), qkv_ld, rseq, rpos, rows, cfg.heads, cfg.kv_heads,
                                                  head_dim, rope_cos.as<float>(), rope_sin.as<float>(), cfg.context,

@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from ._lib import P_i64, Epilogue, Q8CacheStruct, Q8Plane, check, load
+from ._lib import P_i64, Epilogue, L2Prefetch, Q8CacheStruct, Q8Plane, check, load
 
 ACT = {"none": 0, "relu": 1, "gelu": 2}
 
@@ -292,6 +292,16 @@ def rope_append(qkv, row_seq, row_pos, heads, kv_heads, head_dim, cos_t, sin_t, 
                                         kv_heads * ctx * head_dim, ctx * head_dim, head_dim, _s()))
 
 
+def _l2_prefetch(tensors, flags):
+    pf = L2Prefetch()
+    for i, t in enumerate(tensors):
+        pf.ptr[i] = t.data_ptr()
+        pf.bytes[i] = t.numel() * t.element_size()
+    pf.count = len(tensors)
+    pf.flags = flags
+    return pf
+
+
 def decode_attention(qkv, row_pos, heads, kv_heads, cos_t, sin_t, k_cache, v_cache, row_seq=None, out=None,
                      status=None, prefetch=None, flags=0):
     """Fused decode step (Rope, AppendCache, attention) over un-rotated q|k|v
@@ -306,13 +316,7 @@ def decode_attention(qkv, row_pos, heads, kv_heads, cos_t, sin_t, k_cache, v_cac
     if prefetch is None and flags == 0:
         check(load().accel_b200_decode_attention(*args, _s()))
     else:
-        from ._lib import L2Prefetch
-        pf = L2Prefetch()
-        for i, t in enumerate(prefetch or []):
-            pf.ptr[i] = t.data_ptr()
-            pf.bytes[i] = t.numel() * t.element_size()
-        pf.count = len(prefetch or [])
-        pf.flags = flags
+        pf = _l2_prefetch(prefetch or [], flags)
         check(load().accel_b200_decode_attention_prefetch(*args, ctypes.byref(pf), _s()))
     return out
 
@@ -479,19 +483,26 @@ def attention_decode_q8_workspace(cache, rows, heads, window=0, sinks=0):
 
 
 def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=0, out=None, workspace=None,
-                        status=None):
+                        status=None, prefetch=None, flags=0):
     """Attention of roped query rows q [rows, heads * head_dim], row r at
     position row_pos[r] of slot row_seq[r] (None: slot r), over an int8 cache.
     window: how many of the last tokens a row sees (0: all); sinks: first
-    tokens it sees besides. Rows with row_pos < 0 are left."""
+    tokens it sees besides. Rows with row_pos < 0 are left. prefetch: up to
+    four contiguous device tensors to bring into L2 meanwhile; flags: launch
+    options (ATTN_CACHE_BEFORE_WAIT)."""
     index = cache.index
     rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
     if workspace is None:
         workspace = attention_decode_q8_workspace(cache, rows, heads, window, sinks)
     ws, ws_bytes = _bytes(workspace, index)
-    _call(index, load().accel_b200_attention_decode_q8, q.data_ptr(), q_ld, cache._ref,
-          _i32("row_seq", row_seq, index, rows), _i32("row_pos", row_pos, index, rows), rows, heads, window, sinks,
-          out.data_ptr(), out_ld, ws, ws_bytes, _i32("status", status, index, 1))
+    args = (q.data_ptr(), q_ld, cache._ref, _i32("row_seq", row_seq, index, rows),
+            _i32("row_pos", row_pos, index, rows), rows, heads, window, sinks, out.data_ptr(), out_ld, ws, ws_bytes,
+            _i32("status", status, index, 1))
+    if prefetch is None and flags == 0:
+        _call(index, load().accel_b200_attention_decode_q8, *args)
+    else:
+        _call(index, load().accel_b200_attention_decode_q8_prefetch, *args,
+              ctypes.byref(_l2_prefetch(prefetch or [], flags)))
     return out
 
 

@@ -530,6 +530,20 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
                                                   int64_t out_ld, void* workspace, size_t workspace_bytes,
                                                   int32_t* status, void* stream);
 
+/* accel_b200_attention_decode_q8 that also brings `prefetch`'s ranges into L2
+   (as accel_b200_decode_attention_prefetch does). With
+   ACCEL_B200_ATTN_CACHE_BEFORE_WAIT in its flags the positions, the slots and
+   the cache in front of each row's own block are read before the kernel waits
+   for the previous kernel of the stream (the queries, the scales and the rows'
+   own blocks after it). The caller guarantees that no kernel still running when
+   this one starts writes those: the previous kernel is accel_b200_rope_append_q8
+   of rows in these blocks (it lets this one start only after its own wait), or
+   one that does not launch its dependents early. prefetch may be NULL. */
+ACCEL_B200_API int accel_b200_attention_decode_q8_prefetch(
+    const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, const int32_t* row_seq, const int32_t* row_pos,
+    int64_t rows, int32_t heads, int32_t window, int32_t sinks, float* out, int64_t out_ld, void* workspace,
+    size_t workspace_bytes, int32_t* status, const accel_b200_l2_prefetch* prefetch, void* stream);
+
 /* The same attention for many rows of each sequence: rows first[b] ..
    first[b] + count[b] - 1 of q and out (`rows` of them in all, max_rows >=
    every count) at positions pos0[b] + i of slot b; the cache already holds

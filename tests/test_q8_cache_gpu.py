@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from accelep_b200 import kernels as K
+from accelep_b200._lib import B200Error
 from tests import q8_cache_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -255,6 +256,66 @@ def test_decode_long_and_few(lib, cuda, rows, heads, kv, d, context, window):
     q = rng.standard_normal((rows, heads * d), dtype=np.float32)
     got = H(K.attention_decode_q8(T(q), device_cache(c), T(pos), heads, window=window, sinks=5))
     check_rows(c, q, got, [(r, r, int(p)) for r, p in enumerate(pos)], heads, window, 5)
+
+
+def test_decode_balanced_over_lengths(lib, cuda):
+    """Few rows of very different lengths in a long context, some finished or
+    misplaced, several of one slot: CTAs go to rows by what they see."""
+    rng = np.random.default_rng(31)
+    heads, kv, d, context = 12, 2, 64, 16500
+    c = filled(rng, 4, kv, context, d, 64)
+    slot = np.array([3, 0, 1, 2, 0, 4, 3, 1, 2, 2], np.int32)
+    pos = np.array([16499, 0, -1, 33, 9000, 5, 16500, 16383, 700, 31], np.int32)
+    q = rng.standard_normal((10, heads * d), dtype=np.float32)
+    dev = device_cache(c)
+    for window in (0, 5000):
+        ws = K.attention_decode_q8_workspace(dev, 10, heads, window, 2)
+        if window == 0:
+            assert ws is not None
+        for _ in range(2):  # the counters are left as they were found
+            out = torch.full((10, heads * d), 7.0, device="cuda")
+            status = torch.zeros(1, dtype=torch.int32, device="cuda")
+            K.attention_decode_q8(T(q), dev, T(pos), heads, row_seq=T(slot), window=window, sinks=2, out=out,
+                                  workspace=ws, status=status)
+            assert H(status)[0] == BAD_POSITION
+            assert (H(out)[[2, 5, 6]] == 7.0).all()
+            if ws is not None:
+                assert not H(ws)[:65536].any()
+            check_rows(c, q, H(out), [(r, int(slot[r]), int(pos[r])) for r in (0, 1, 3, 4, 7, 8, 9)], heads, window, 2)
+
+
+def test_decode_before_the_appends_end(lib, cuda):
+    """ACCEL_B200_ATTN_CACHE_BEFORE_WAIT behind rope_append_q8, as the engine runs
+    them: the same bits as without, over block edges and growing scales, and
+    the ranges brought into L2 stay as they are."""
+    rng = np.random.default_rng(41)
+    heads, kv, d, block, context, batch = 9, 3, 64, 64, 700, 6
+    cos, sin = (T(t) for t in O.tables(context, d))
+    c = filled(rng, batch, kv, context, d, block)
+    caches = [device_cache(c) for _ in range(2)]
+    other = T(rng.integers(0, 255, 1 << 20).astype(np.uint8))
+    keep = other.clone()
+    pos = np.array([63, 64, 65, 640, -1, 0], np.int32)
+    ident, ones = I(list(range(batch))), I([1] * batch)
+    for n in range(4):
+        x = T(rng.standard_normal((batch, (heads + 2 * kv) * d), dtype=np.float32) * (1 + 3 * n))
+        outs = []
+        for i, dev in enumerate(caches):
+            out = torch.full((batch, heads * d), 7.0, device="cuda")
+            q = torch.zeros(batch, heads * d, device="cuda")
+            at = T(pos)
+            torch.cuda.synchronize()
+            K.rope_append_q8(x, dev, ident, ones, at, heads, 1, cos, sin, q_out=q)
+            extra = dict(prefetch=[other], flags=K.ATTN_CACHE_BEFORE_WAIT) if i else {}
+            K.attention_decode_q8(q, dev, at, heads, out=out, **extra)
+            outs.append(H(out))
+        np.testing.assert_array_equal(outs[0], outs[1])
+        same(caches[1], type("C", (), {"q": {k: H(getattr(caches[0], k)) for k in "kv"},
+                                       "s": {k: H(getattr(caches[0], k + "_scale")) for k in "kv"}}))
+        pos[pos >= 0] += 1
+    assert torch.equal(other, keep)
+    with pytest.raises(B200Error, match="prefetch"):
+        K.attention_decode_q8(q, caches[0], T(pos), heads, flags=6)
 
 
 def test_decode_rows_that_share_slots(lib, cuda):

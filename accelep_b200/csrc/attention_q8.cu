@@ -669,10 +669,20 @@ int CheckWorkspace(const Split& p, const void* workspace, size_t bytes, const st
   return ACCEL_B200_OK;
 }
 
-// Sequences of more vectors than this per kv head take 256-vector tiles.
-constexpr int64_t kMostVectors = 64;
-bool TakesTiles(const accel_b200_q8_cache& c, int64_t max_rows, int32_t heads) {
-  return max_rows * (heads / c.kv_heads) > kMostVectors;
+// Whether a prefill takes the 256-vector tiles of attention_q8_tiles.cu. Both
+// kernels' times go by the tokens that rows see: a tile CTA walks 128 of them
+// in about 2.4 us (3.0 at 128 dimensions), one wave of 148 CTAs after another;
+// the groups of 8 vectors here share the whole GPU at about 1500 (1200) of
+// their units of 32 tokens per us. Tiles are faster from 900 groups per wave.
+// (Measured with 3 kv heads of 64, 12 heads, 16000 tokens: 32 sequences of 21
+// rows 336 us in tiles and 234 here, of 42 rows 328 and 385; one sequence of
+// 170 rows 268 and 56. With 8 kv heads of 128, 32 heads: 32 sequences of 8 rows
+// 686 and 480, of 16 rows 717 and 785; 4 of 64 rows 421 and 524.)
+constexpr int64_t kTileGroups = 900;
+bool TakesTiles(const accel_b200_q8_cache& c, int64_t batch, int64_t max_rows, int32_t heads) {
+  const int64_t vectors = max_rows * (heads / c.kv_heads), runs = batch * c.kv_heads;
+  const int64_t waves = CeilDiv(runs * CeilDiv(vectors, kTileVectors), kSms);
+  return runs * CeilDiv(vectors, kVec) > kTileGroups * waves;
 }
 
 AttnArgs ArgsOf(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, const RaggedRows& rows,
@@ -780,7 +790,7 @@ ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200
     return 0;
   }
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));
-  if (TakesTiles(*cache, max_rows, heads)) return 0;
+  if (TakesTiles(*cache, batch, max_rows, heads)) return 0;
   return SplitFor(*cache, batch, max_rows, heads, window, sinks, false).workspace;
 }
 
@@ -801,7 +811,7 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));  // a longer run does not fit
   const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads,
                             window, sinks, out, out_ld, status);
-  if (TakesTiles(*cache, max_rows, heads)) return LaunchTilesQ8(a, batch, max_rows, AsStream(stream));
+  if (TakesTiles(*cache, batch, max_rows, heads)) return LaunchTilesQ8(a, batch, max_rows, AsStream(stream));
   const Split p = SplitFor(*cache, batch, max_rows, heads, window, sinks, false);
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: grid too large");

@@ -65,8 +65,9 @@ __device__ __forceinline__ void SplitPair(float x, float y, uint32_t* hi, uint32
 // First position that a window ending at pos covers.
 __device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
-// Prefill attention on the tcgen05 tensor cores, 256 query vectors per CTA
-// (attention_q8_tiles.cu).
+// Prefill attention on the tcgen05 tensor cores, kTileVectors query vectors per
+// CTA (attention_q8_tiles.cu).
+constexpr int kTileVectors = 256;
 int LaunchTilesQ8(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stream);
 
 }  // namespace accel_b200

@@ -45,6 +45,7 @@ namespace accel_b200 {
 namespace {
 
 constexpr int kHalf = 128;         // vectors of a half: TMEM lanes
+static_assert(2 * kHalf == kTileVectors, "");
 constexpr int kTile = 128;         // tokens per tile
 constexpr int kConverters = 4;     // warps
 constexpr int kChunk = 32;         // tokens whose scores a thread holds at a time: one scale block at most

@@ -190,6 +190,20 @@ def test_misplaced_sequences_are_skipped(lib, cuda, first, count, pos0, max_rows
     assert H(status)[0] == BAD_POSITION and (H(out)[:3] == 7.0).all() and (H(out)[3:] != 7.0).all()
 
 
+@pytest.mark.parametrize("first,count,pos0", [([0, 3], [3, 3], [3998, 0]), ([-1, 3], [3, 3], [0, 0]),
+                                              ([4, 3], [3, 3], [0, 0]), ([0, 3], [4001, 3], [0, 0])])
+def test_misplaced_sequences_are_skipped_by_tiles(lib, cuda, first, count, pos0):
+    rng = np.random.default_rng(6)
+    d, context, rows = 64, 4000, 6
+    c = filled(rng, 2, 1, context, d, 64)
+    q = rng.standard_normal((rows, d), dtype=np.float32)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    out = torch.full((rows, d), 7.0, device="cuda")
+    K.attention_prefill_q8(T(q), device_cache(c), I(first), I(count), I(pos0), 1, context, out=out, status=status)
+    assert H(status)[0] == BAD_POSITION and (H(out)[:3] == 7.0).all()
+    check_rows(c, q, H(out), [(3, 1, 0), (4, 1, 1), (5, 1, 2)], 1, 0, 0)
+
+
 @pytest.mark.parametrize("kv,d,block,pos0,count", [
     (3, 64, 64, [0, 63, 100, 7], [200, 2, 1, 0]),
     (2, 128, 32, [199, 31, -1], [1, 65, 5]),
@@ -346,14 +360,15 @@ PREFILLS = [
 
 @pytest.mark.parametrize("heads,kv,d,block,pos0,count", PREFILLS)
 @pytest.mark.parametrize("window,sinks", [(0, 0), (1, 2), (50, 4), (64, 64), (130, 1), (1000, 7)])
-def test_prefill_matches(lib, cuda, heads, kv, d, block, pos0, count, window, sinks):
+@pytest.mark.parametrize("most", [300, 1200])  # max_rows: small calls go 8 vectors to a warp, large ones by tiles
+def test_prefill_matches(lib, cuda, heads, kv, d, block, pos0, count, window, sinks, most):
     rng = np.random.default_rng(heads * 1000 + d + window)
-    c = filled(rng, len(pos0), kv, 300, d, block)
+    c = filled(rng, len(pos0), kv, most, d, block)
     first, rows = ragged(count), int(np.sum(count)) + 3
     q = rng.standard_normal((rows, heads * d), dtype=np.float32)
     out = torch.full((rows, heads * d), 7.0, device="cuda")
     status = torch.zeros(1, dtype=torch.int32, device="cuda")
-    K.attention_prefill_q8(T(q), device_cache(c), I(first), I(count), I(pos0), heads, max(count), window=window,
+    K.attention_prefill_q8(T(q), device_cache(c), I(first), I(count), I(pos0), heads, most, window=window,
                            sinks=sinks, out=out, status=status)
     got = H(out)
     assert H(status)[0] == 0 and (got[-3:] == 7.0).all()
@@ -384,7 +399,7 @@ def test_what_a_row_does_not_see_does_not_matter(lib, cuda, bad):
     """Scales of blocks that hold nothing a row sees (behind it, or before its
     window) are any values; rows of a visible block behind the row any bytes."""
     rng = np.random.default_rng(2)
-    heads, kv, d, block, context = 6, 2, 64, 32, 400
+    heads, kv, d, block, context = 6, 2, 64, 32, 2400
     c = filled(rng, 1, kv, context, d, block)
     q = rng.standard_normal((40, heads * d), dtype=np.float32)
     window, sinks, pos = 60, 3, 210
@@ -393,9 +408,10 @@ def test_what_a_row_does_not_see_does_not_matter(lib, cuda, bad):
         c.s[name][:, :, (pos + 39) // block + 1:] = bad
     got = H(K.attention_decode_q8(T(q[:1]), device_cache(c), I([pos + 39]), heads, window=window, sinks=sinks))
     check_rows(c, q, got, [(0, 0, pos + 39)], heads, window, sinks)
-    got = H(K.attention_prefill_q8(T(q), device_cache(c), I([0]), I([40]), I([pos]), heads, 40, window=window,
-                                   sinks=sinks))
-    check_rows(c, q, got, [(r, 0, pos + r) for r in range(40)], heads, window, sinks)
+    for most in (40, context):
+        got = H(K.attention_prefill_q8(T(q), device_cache(c), I([0]), I([40]), I([pos]), heads, most, window=window,
+                                       sinks=sinks))
+        check_rows(c, q, got, [(r, 0, pos + r) for r in range(40)], heads, window, sinks)
 
 
 @pytest.mark.parametrize("size", [1e-30, 1e-3, 40.0, 1e4])
@@ -403,8 +419,8 @@ def test_queries_and_scales_of_any_size(lib, cuda, size):
     """Tiny queries (even weights), and ones whose softmax is a single position;
     scales far from one."""
     rng = np.random.default_rng(12)
-    heads, kv, d = 4, 2, 64
-    c = filled(rng, 2, kv, 200, d, 64)
+    heads, kv, d, context = 4, 2, 64, 2400
+    c = filled(rng, 2, kv, context, d, 64)
     for name in "kv":
         c.s[name][1] *= np.float32(1e-25 if name == "k" else 1e25)
     q = (rng.standard_normal((2, heads * d)) * size).astype(np.float32)
@@ -412,8 +428,9 @@ def test_queries_and_scales_of_any_size(lib, cuda, size):
     q[0, :d] = 0  # a head with no direction: even weights
     dev = device_cache(c)
     check_rows(c, q, H(K.attention_decode_q8(T(q), dev, I([199, 150]), heads)), [(0, 0, 199), (1, 1, 150)], heads, 0, 0)
-    got = H(K.attention_prefill_q8(T(q), dev, I([0, 1]), I([1, 1]), I([199, 150]), heads, 1))
-    check_rows(c, q, got, [(0, 0, 199), (1, 1, 150)], heads, 0, 0)
+    for most in (1, context):
+        got = H(K.attention_prefill_q8(T(q), dev, I([0, 1]), I([1, 1]), I([199, 150]), heads, most))
+        check_rows(c, q, got, [(0, 0, 199), (1, 1, 150)], heads, 0, 0)
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -422,7 +439,7 @@ def test_value_scales_far_apart(lib, cuda, d, apart):
     """Blocks of one tile whose value scales differ by 2^5 to 2^40, or are zero,
     where the small ones have all of the weight, half of it or none."""
     rng = np.random.default_rng(int(d + min(apart, 1e6)))
-    heads, kv, block, context, n = 4, 1, 32, 320, 60
+    heads, kv, block, context, n = 4, 1, 32, 2400, 60
     c = filled(rng, 1, kv, context, d, block)
     q = rng.standard_normal((n, heads * d), dtype=np.float32)
     q[:, :d] *= 30  # one head of large scores
@@ -433,8 +450,9 @@ def test_value_scales_far_apart(lib, cuda, d, apart):
         c.q["k"][0, 0, j * block:(j + 1) * block] = direction * rng.integers(60, 127, (block, 1))
     dev = device_cache(c)
     for first_pos in (4, 250):
-        got = H(K.attention_prefill_q8(T(q), dev, I([0]), I([n]), I([first_pos]), heads, n))
-        check_rows(c, q, got, [(r, 0, first_pos + r) for r in range(0, n, 3)], heads, 0, 0)
+        for most in (n, context):
+            got = H(K.attention_prefill_q8(T(q), dev, I([0]), I([n]), I([first_pos]), heads, most))
+            check_rows(c, q, got, [(r, 0, first_pos + r) for r in range(0, n, 3)], heads, 0, 0)
     rows = min(n, 3)
     got = H(K.attention_decode_q8(T(q[:rows]), dev, I([40, 200, 319]), heads, row_seq=I([0] * rows)))
     check_rows(c, q, got, [(0, 0, 40), (1, 0, 200), (2, 0, 319)], heads, 0, 0)
@@ -442,13 +460,14 @@ def test_value_scales_far_apart(lib, cuda, d, apart):
 
 def test_nan_queries_stay_in_their_head(lib, cuda):
     rng = np.random.default_rng(13)
-    heads, kv, d = 6, 2, 64
-    c = filled(rng, 2, kv, 200, d, 64)
+    heads, kv, d, context = 6, 2, 64, 2400
+    c = filled(rng, 2, kv, context, d, 64)
     q = rng.standard_normal((2, heads * d), dtype=np.float32)
     q[0, 2 * d + 5] = np.nan
     dev = device_cache(c)
     for got in (H(K.attention_decode_q8(T(q), dev, I([199, 150]), heads)),
-                H(K.attention_prefill_q8(T(q), dev, I([0, 1]), I([1, 1]), I([199, 150]), heads, 1))):
+                H(K.attention_prefill_q8(T(q), dev, I([0, 1]), I([1, 1]), I([199, 150]), heads, 1)),
+                H(K.attention_prefill_q8(T(q), dev, I([0, 1]), I([1, 1]), I([199, 150]), heads, context))):
         assert np.isnan(got[0, 2 * d:3 * d]).all()
         got[0, 2 * d:3 * d] = 0
         clean = q.copy()

@@ -706,7 +706,7 @@ AttnArgs ArgsOf(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, 
 }
 
 int CheckAttention(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, int32_t heads, int32_t window,
-                   int32_t sinks, const float* out, int64_t out_ld, const std::string& what) {
+                   int32_t sinks, const float* out, int64_t out_ld, int64_t rows, const std::string& what) {
   const int rc = CheckQ8Cache(cache, what.c_str());
   if (rc != ACCEL_B200_OK) return rc;
   if (heads <= 0 || heads % cache->kv_heads != 0 || window < 0 || sinks < 0 || q == nullptr || out == nullptr) {
@@ -716,6 +716,9 @@ int CheckAttention(const float* q, int64_t q_ld, const accel_b200_q8_cache* cach
   if (q_ld < width || out_ld < width) return SetError(ACCEL_B200_EINVAL, what + ": row strides too small");
   if (q_ld % 4 != 0 || out_ld % 4 != 0 || (reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) % 16 != 0) {
     return SetError(ACCEL_B200_EINVAL, what + ": rows must be 16-byte aligned");
+  }
+  if (!RowsApart(q, q_ld, width, out, out_ld, width, rows)) {
+    return SetError(ACCEL_B200_EINVAL, what + ": out overlaps q otherwise than in place");
   }
   if (heads > 65535) return SetError(ACCEL_B200_EINVAL, what + ": more than 65535 heads");
   return ACCEL_B200_OK;
@@ -743,7 +746,7 @@ ACCEL_B200_API int accel_b200_attention_decode_q8_prefetch(const float* q, int64
                                                   int64_t out_ld, void* workspace, size_t workspace_bytes,
                                                   int32_t* status, const accel_b200_l2_prefetch* prefetch,
                                                   void* stream) {
-  int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, "attention_decode_q8");
+  int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, rows, "attention_decode_q8");
   if (rc != ACCEL_B200_OK) return rc;
   if (rows < 0 || row_pos == nullptr) return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: bad arguments");
   if (row_seq == nullptr && rows > cache->slots) {
@@ -800,7 +803,7 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
                                                    int32_t window, int32_t sinks, float* out, int64_t out_ld,
                                                    void* workspace, size_t workspace_bytes, int32_t* status,
                                                    void* stream) {
-  int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, "attention_prefill_q8");
+  int rc = CheckAttention(q, q_ld, cache, heads, window, sinks, out, out_ld, rows, "attention_prefill_q8");
   if (rc != ACCEL_B200_OK) return rc;
   if (rows < 0 || batch < 0 || max_rows < 0 || first == nullptr || count == nullptr || pos0 == nullptr) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: bad arguments");

@@ -308,6 +308,9 @@ ACCEL_B200_API int accel_b200_rope_append_q8(const float* qkv, int64_t qkv_ld, i
        reinterpret_cast<uintptr_t>(sin_table)) % 16 != 0) {
     return SetError(ACCEL_B200_EINVAL, "rope_append_q8: rows must be 16-byte aligned");
   }
+  if (!RowsApart(qkv, qkv_ld, width * cache->head_dim, q_out, q_ld, static_cast<int64_t>(heads) * cache->head_dim, rows)) {
+    return SetError(ACCEL_B200_EINVAL, "rope_append_q8: q_out overlaps qkv otherwise than in place");
+  }
   if (batch == 0 || max_rows == 0 || rows == 0) return ClearError();
   if (batch > 65535 || width > 65535) return SetError(ACCEL_B200_EINVAL, "rope_append_q8: grid too large");
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));  // a longer run does not fit
@@ -332,6 +335,11 @@ ACCEL_B200_API int accel_b200_cache_rows_q8(const accel_b200_q8_cache* cache, co
   }
   if (out_ld % 4 != 0 || (reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 != 0) {
     return SetError(ACCEL_B200_EINVAL, "cache_rows_q8: rows must be 16-byte aligned");
+  }
+  if (k_out != nullptr && v_out != nullptr &&
+      (k_out == v_out || !RowsApart(k_out, out_ld, static_cast<int64_t>(cache->kv_heads) * cache->head_dim, v_out, out_ld,
+                                    static_cast<int64_t>(cache->kv_heads) * cache->head_dim, rows))) {
+    return SetError(ACCEL_B200_EINVAL, "cache_rows_q8: k_out overlaps v_out");
   }
   if (batch == 0 || max_rows == 0 || rows == 0 || (k_out == nullptr && v_out == nullptr)) return ClearError();
   if (batch > 65535 || cache->kv_heads > 32767) return SetError(ACCEL_B200_EINVAL, "cache_rows_q8: grid too large");

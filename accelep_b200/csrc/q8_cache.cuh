@@ -20,6 +20,20 @@ inline bool Disjoint(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t inn
   return (s1 >= inner && s0 / n1 >= s1) || (s0 >= inner && s1 / n0 >= s0);
 }
 
+// Whether row buffers a (`wa` floats of each row, stride lda) and b may both be
+// used when b is written: they do not touch, are the same rows, or are other
+// columns of rows of the same stride.
+inline bool RowsApart(const float* a, int64_t lda, int64_t wa, const float* b, int64_t ldb, int64_t wb, int64_t rows) {
+  if (rows <= 0) return true;
+  const intptr_t a0 = reinterpret_cast<intptr_t>(a), b0 = reinterpret_cast<intptr_t>(b);
+  const intptr_t a1 = a0 + ((rows - 1) * lda + wa) * 4, b1 = b0 + ((rows - 1) * ldb + wb) * 4;
+  if (a1 <= b0 || b1 <= a0) return true;
+  if (rows > 1 && lda != ldb) return false;
+  const int64_t delta = (b0 - a0) / 4;  // 16-byte aligned rows
+  if (delta == 0) return true;
+  return delta > 0 ? delta >= wa && (rows == 1 || delta + wb <= lda) : -delta >= wb && (rows == 1 || wa - delta <= lda);
+}
+
 // Rows of head_dim bytes from the first of a plane to behind its last run; row
 // t of (slot s, head g) is (s * seq_stride + g * head_stride) / head_dim + t.
 inline int64_t PlaneRows(const accel_b200_q8_cache& c) {
@@ -34,6 +48,7 @@ inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
   if (c == nullptr || c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) {
     return SetError(ACCEL_B200_EINVAL, w + ": the cache has a null plane");
   }
+  if (c->k == c->v || c->k_scale == c->v_scale) return SetError(ACCEL_B200_EINVAL, w + ": keys and values are one plane");
   if (c->head_dim != 64 && c->head_dim != 128) {
     return SetError(ACCEL_B200_EINVAL, w + ": head_dim must be 64 or 128");
   }

@@ -472,9 +472,10 @@ typedef struct accel_b200_q8_cache {
 /* RoPE and append with quantisation. Sequence b < batch owns fused projection
    rows first[b] .. first[b] + count[b] - 1 of qkv (device arrays; rows as in
    accel_b200_rope_append, `rows` of them in all, max_rows >= every count) at
-   positions pos0[b] + i of slot b. The roped queries go to q_out (row stride
-   q_ld; qkv itself with qkv_ld rotates in place, any other overlap is not
-   allowed), roped keys and values to the cache.
+   positions pos0[b] + i of slot b; no row belongs to two sequences. The
+   tables hold [context][head_dim]. The roped queries go to q_out (row stride
+   q_ld; qkv itself with qkv_ld rotates in place, any other overlap is
+   refused), roped keys and values to the cache.
 
    Block by block of a (slot, head) plane: amax is the largest finite |x| of
    the new rows, `need` the least power of two >= 2^-126 with amax <= 127 *
@@ -516,8 +517,9 @@ ACCEL_B200_API int accel_b200_cache_rows_q8(const accel_b200_q8_cache* cache, co
    softmax(q . k / sqrt(head_dim)) v. Several rows may name one slot. Rows with
    row_pos[r] < 0 are skipped (their output is not written); a position or
    slot outside the cache is skipped with ACCEL_B200_STATUS_BAD_POSITION.
-   heads is any multiple of kv_heads; rows are 16-byte aligned. The result
-   does not depend on how the work is split between calls of the same sizes.
+   heads is any multiple of kv_heads; rows are 16-byte aligned; out may be q
+   itself. Scales of blocks that a row sees are finite and not negative; other
+   blocks may hold anything. Equal calls give equal bits.
    The workspace holds accel_b200_attention_decode_q8_workspace(...) bytes (0:
    none) whose first 64 KiB are zero before the first call, as for the
    products; every call leaves them zero. Calls that share it must not overlap

@@ -16,7 +16,7 @@ P = 1 << 20  # an aligned address that is never read
 
 
 def cache(**change):
-    d = {"k": P, "v": P, "k_scale": P, "v_scale": P, "seq_stride": 2 * 100 * 64, "head_stride": 100 * 64,
+    d = {"k": P, "v": 2 * P, "k_scale": 3 * P, "v_scale": 4 * P, "seq_stride": 2 * 100 * 64, "head_stride": 100 * 64,
          "scale_seq_stride": 4, "scale_head_stride": 2, "slots": 3, "kv_heads": 2, "head_dim": 64, "context": 100,
          "block": 64}
     d.update(change)
@@ -24,14 +24,14 @@ def cache(**change):
 
 
 BAD_CACHES = [{"k": None}, {"v_scale": None}, {"head_dim": 96}, {"head_dim": 32}, {"block": 16}, {"block": 0},
-              {"block": 48}, {"slots": 0}, {"kv_heads": 0}, {"context": 0}, {"k": P + 8}, {"v_scale": P + 2},
+              {"block": 48}, {"slots": 0}, {"kv_heads": 0}, {"context": 0}, {"k": P + 8}, {"v_scale": P + 2}, {"v": P}, {"v_scale": 3 * P},
               {"head_stride": 99 * 64}, {"seq_stride": 100 * 64}, {"seq_stride": 2 * 100 * 64 + 8},
               {"scale_head_stride": 1}, {"scale_seq_stride": 3}, {"head_stride": -100 * 64}]
 
 
 def append(lib, c, **change):
     d = {"qkv": P, "ld": 8 * 64, "rows": 5, "first": P, "count": P, "pos0": P, "batch": 3, "max_rows": 4, "heads": 4,
-         "cos": P, "sin": P, "q": P, "q_ld": 4 * 64}
+         "cos": P, "sin": P, "q": 5 * P, "q_ld": 4 * 64}
     d.update(change)
     return lib.accel_b200_rope_append_q8(d["qkv"], d["ld"], d["rows"], c, d["first"], d["count"], d["pos0"],
                                          d["batch"], d["max_rows"], d["heads"], d["cos"], d["sin"], d["q"], d["q_ld"],
@@ -39,14 +39,14 @@ def append(lib, c, **change):
 
 
 def read(lib, c, **change):
-    d = {"first": P, "count": P, "pos0": P, "batch": 3, "max_rows": 4, "k": P, "v": P, "ld": 128, "rows": 5}
+    d = {"first": P, "count": P, "pos0": P, "batch": 3, "max_rows": 4, "k": P, "v": 2 * P, "ld": 128, "rows": 5}
     d.update(change)
     return lib.accel_b200_cache_rows_q8(c, d["first"], d["count"], d["pos0"], d["batch"], d["max_rows"], d["k"],
                                         d["v"], d["ld"], d["rows"], None, None)
 
 
 def decode(lib, c, **change):
-    d = {"q": P, "ld": 256, "seq": None, "pos": P, "rows": 3, "heads": 4, "window": 0, "sinks": 0, "out": P,
+    d = {"q": P, "ld": 256, "seq": None, "pos": P, "rows": 3, "heads": 4, "window": 0, "sinks": 0, "out": 2 * P,
          "out_ld": 256}
     d.update(change)
     return lib.accel_b200_attention_decode_q8(d["q"], d["ld"], c, d["seq"], d["pos"], d["rows"], d["heads"],
@@ -55,7 +55,7 @@ def decode(lib, c, **change):
 
 def prefill(lib, c, **change):
     d = {"q": P, "ld": 256, "first": P, "count": P, "pos0": P, "batch": 3, "max_rows": 4, "rows": 5, "heads": 4,
-         "window": 0, "sinks": 0, "out": P, "out_ld": 256}
+         "window": 0, "sinks": 0, "out": 2 * P, "out_ld": 256}
     d.update(change)
     return lib.accel_b200_attention_prefill_q8(d["q"], d["ld"], c, d["first"], d["count"], d["pos0"], d["batch"],
                                                d["max_rows"], d["rows"], d["heads"], d["window"], d["sinks"],
@@ -75,6 +75,9 @@ def test_bad_caches_are_refused(lib, call, change):
     (append, {"rows": -1}), (append, {"batch": -1}), (append, {"batch": 4}), (append, {"heads": 3}),
     (append, {"heads": 0}), (append, {"ld": 7 * 64}), (append, {"q_ld": 4 * 64 - 4}), (append, {"ld": 8 * 64 + 2}),
     (append, {"qkv": P + 4}), (append, {"q": P + 8}), (append, {"max_rows": -1}),
+    (append, {"q": P}), (append, {"q": P + 16, "q_ld": 8 * 64}), (append, {"q": P + 4 * 512, "q_ld": 512}),
+    (append, {"q": P - 4 * 128, "q_ld": 512}), (read, {"v": P}), (read, {"v": P + 64}), (read, {"v": P + 4 * 128}),
+    (decode, {"out": P + 64}), (decode, {"out": P, "out_ld": 512}), (prefill, {"out": P + 4 * 256}),
     (read, {"first": None}), (read, {"batch": 4}), (read, {"ld": 124}), (read, {"ld": 130}), (read, {"k": P + 4}),
     (read, {"rows": -2}),
     (decode, {"q": None}), (decode, {"pos": None}), (decode, {"rows": 4}), (decode, {"rows": -1}),
@@ -86,6 +89,15 @@ def test_bad_caches_are_refused(lib, call, change):
 def test_bad_arguments_are_refused(lib, call, change):
     assert call(lib, cache(), **change) == 1
     assert lib.accel_b200_last_error()
+
+
+def test_overlaps_that_are_taken(lib):
+    """In place, and other columns of the same rows (no rows: nothing runs)."""
+    assert append(lib, cache(), q=P, q_ld=512, max_rows=0) == 0
+    assert append(lib, cache(), ld=1024, q=P + 4 * 512, q_ld=1024, max_rows=0) == 0
+    assert append(lib, cache(), qkv=P + 4 * 256, ld=1024, q=P, q_ld=1024, max_rows=0) == 0
+    assert read(lib, cache(), ld=256, v=P + 4 * 128, max_rows=0) == 0
+    assert prefill(lib, cache(), out=P, max_rows=0) == 0
 
 
 def test_empty_calls_queue_nothing(lib):

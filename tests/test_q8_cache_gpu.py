@@ -458,6 +458,25 @@ def test_value_scales_far_apart(lib, cuda, d, apart):
     check_rows(c, q, got, [(0, 0, 40), (1, 0, 200), (2, 0, 319)], heads, 0, 0)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_in_place(lib, cuda, d):
+    """out may be q: every split of a row has read it before it is written."""
+    rng = np.random.default_rng(d)
+    heads, kv, context = 6, 2, 9000
+    c = filled(rng, 2, kv, context, d, 64)
+    dev = device_cache(c)
+    for rows, pos in ((1, [8999]), (2, [700, 8000])):
+        q = rng.standard_normal((rows, heads * d), dtype=np.float32)
+        x = T(q)
+        K.attention_decode_q8(x, dev, I(pos), heads, out=x)
+        check_rows(c, q, H(x), [(r, r, p) for r, p in enumerate(pos)], heads, 0, 0)
+    q = rng.standard_normal((300, heads * d), dtype=np.float32)
+    for most in (300, context):
+        x = T(q)
+        K.attention_prefill_q8(x, dev, I([0, 290]), I([290, 10]), I([500, 8000]), heads, most, out=x)
+        check_rows(c, q, H(x), [(0, 0, 500), (289, 0, 789), (150, 0, 650), (290, 1, 8000), (299, 1, 8009)], heads, 0, 0)
+
+
 def test_nan_queries_stay_in_their_head(lib, cuda):
     rng = np.random.default_rng(13)
     heads, kv, d, context = 6, 2, 64, 2400

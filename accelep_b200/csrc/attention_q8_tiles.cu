@@ -1,14 +1,14 @@
 // Attention of many query rows over the int8 key/value cache on the 5th-
 // generation tensor cores (include/accel_b200.h, accel_b200_attention_prefill_q8).
 //
-// One CTA takes 256 consecutive query vectors (row x head, the heads of one kv
-// head) of one sequence and walks the 128-token tiles that any of them sees.
-// Keys and values become fp16 exactly; queries and weights are sums of two fp16
-// numbers (22 bits), the second parts' products summed first, so results are
-// fp32 results. Per tile and half (128 vectors):
+// One CTA takes consecutive query vectors (row x head, the heads of one kv head)
+// of one sequence, one or two halves of 128, and walks the 128-token tiles that
+// any of them sees. Keys and values become fp16 exactly; queries and weights
+// are sums of two fp16 numbers (22 bits), the second parts' products summed
+// first, so results are fp32 results. Per tile and half:
 //
 //   S = Qlo K^T + Qhi K^T      128 x 128 x D, operands in shared memory
-//   online softmax             one thread per vector, S read from TMEM
+//   online softmax             one or two threads per vector, S read from TMEM
 //   P, lo and hi parts         written over S in TMEM
 //   O = Plo V + Phi V          128 x D x 128, A operand from TMEM
 //   registers += vscale * O    fp32, rounded to nearest
@@ -18,12 +18,22 @@
 // the value scale and the softmax reference change from tile to tile. Scales
 // of the tile's blocks are folded into the weights relative to the largest.
 //
-// Roles: the first warps are the softmax of the two halves (while one half
-// computes, the tensor core works for the other); four turn the int8 tiles that
+// Roles: the first warps are the softmax (while one half, or the SM's other CTA,
+// computes, the tensor core works for this one); four turn the int8 tiles that
 // TMA brings into fp16 operands with the 128-byte swizzle; one thread of the
-// next issues every MMA. Bound by the tensor core at 128
-// dimensions (two fp16 products in place of one) and by the softmax's issue
-// slots at 64.
+// next issues every MMA.
+//
+// Measured: 2 sequences of 2047 and fewer rows behind 14000 tokens, 32 heads over
+// 8 kv heads of 128, window 4096: 560 us, 427 TFLOP/s of scores and values (twice
+// that in fp16 products). A half's chain (weights 2600 cycles, its four products
+// 2800, maximum 900, read-out 500) and the other's overlap to 7000 cycles a tile,
+// of which the tensor core works 5600: an M = 128, N = 128, K = 16 product takes
+// 102 cycles with A in shared memory, 72 from TMEM. 32 sequences of 512 rows, 9
+// heads over 3 of 64: 76 us, by issue slots (55% of them used) and the first and
+// last steps of short walks. What brought it there, on the first of these: one
+// elected thread instead of lane 0 issuing (1617 -> 1250 us), values freed in
+// front of the next scores and four converter warps (-> 806), chunk loops kept
+// rolled so that their code stays in the instruction cache (-> 632).
 //
 // Every wait is bounded; one that runs out sets a flag that ends every role,
 // gives NaN and ORs ACCEL_B200_STATUS_COPY_TIMEOUT.
@@ -45,12 +55,10 @@ namespace accel_b200 {
 namespace {
 
 constexpr int kHalf = 128;         // vectors of a half: TMEM lanes
-static_assert(2 * kHalf == kTileVectors, "");
 constexpr int kTile = 128;         // tokens per tile
 constexpr int kConverters = 4;     // warps
 constexpr int kChunk = 32;         // tokens whose scores a thread holds at a time: one scale block at most
 constexpr int kChunks = kTile / kChunk;
-constexpr uint32_t kTmemCols = 512;
 constexpr float kMostLift = 6.f;    // scales of a tile further apart than 2^6 are applied one by one
 constexpr int kPanel = 128 * 128;  // bytes of 128 rows x 64 fp16, the swizzle's row length
 
@@ -60,30 +68,34 @@ struct Tiles {
   // the dimensions: two where the sums of 64 dimensions leave the registers
   // for it (one is left waiting for its own instructions most of the time).
   static constexpr int kParts = D == 64 ? 2 : 1;
-  static constexpr int kSoftWarps = 8 * kParts, kMmaWarp = kSoftWarps + kConverters;
+  // Halves of a CTA and CTAs of an SM: 256 vectors in all. Two CTAs, where shared
+  // memory and TMEM allow, hide each other's first and last steps; two halves
+  // share one conversion of the keys and values.
+  static constexpr int kHalves = D == 64 ? 1 : 2, kCtas = 2 / kHalves;
+  static_assert(kHalves * kCtas * kHalf == kTileVectors, "");
+  static constexpr int kSoftWarps = 4 * kParts * kHalves, kMmaWarp = kSoftWarps + kConverters;
   static constexpr int kThreads = (kSoftWarps + 8) * 32;  // whole warpgroups
   // Registers of the softmax threads and of the others from their start on:
-  // in all no more than the launch gives out, 65536 / kThreads each (down to a
-  // multiple of 8).
-  static constexpr int kLaunch = 65536 / kThreads / 8 * 8;
-  static constexpr int kLess = 48, kMore = kLaunch + (kLaunch - kLess) * 256 / (kSoftWarps * 32);
+  // in all no more than the launch gives out (a multiple of 8 each).
+  static constexpr int kLaunch = 65536 / (kThreads * kCtas) / 8 * 8;
+  static constexpr int kLess = D == 64 ? 32 : 48, kMore = kLaunch + (kLaunch - kLess) * 256 / (kSoftWarps * 32);
   static_assert(kMore % 8 == 0 && kSoftWarps * 32 * kMore + 256 * kLess <= kThreads * kLaunch, "");
   static constexpr int kPanels = D / 64;
   static constexpr int kOperand = kPanels * kPanel;     // a 128 x D fp16 operand
-  static constexpr int kStages = D == 64 ? 2 : 1;       // fp16 key and value tiles
+  static constexpr int kStages = 1;                     // fp16 key and value tiles
   static constexpr int kQ = 0;                          // [half][hi, lo]
-  static constexpr int kK = kQ + 4 * kOperand;
+  static constexpr int kK = kQ + 2 * kHalves * kOperand;
   static constexpr int kV = kK + kStages * kOperand;
   static constexpr int kRaw = kV + kStages * kOperand;  // int8 tiles as they come: keys, values
   static constexpr int kRawBytes = kTile * D;
   static constexpr int kBars = kRaw + 2 * kRawBytes;
   static constexpr int kShared = kBars + 256;           // float [half][vector] and [2][half][part][vector]
-  static constexpr int kBytes = kShared + (kParts > 1 ? (2 + 4 * kParts) * 128 * 4 : 0);
+  static constexpr int kBytes = kShared + (kParts > 1 ? (1 + 2 * kParts) * kHalves * 128 * 4 : 0);
   static constexpr int kAlign = 1024;
-  static_assert(kBytes + kAlign <= 227 * 1024, "shared memory of a CTA");
+  static_assert((kBytes + kAlign + 1024) * kCtas <= 228 * 1024, "shared memory of an SM");
   // TMEM columns: scores (then weights) and weighted values of the halves.
-  static constexpr uint32_t kScores = 0, kOut = 2 * kTile;
-  static_assert(kOut + 2 * D <= kTmemCols, "TMEM of an SM");
+  static constexpr uint32_t kScores = 0, kOut = kHalves * kTile, kTmemCols = 512 / kCtas;
+  static_assert(kOut + kHalves * D <= kTmemCols, "TMEM of an SM");
 };
 
 struct Bars {
@@ -183,9 +195,9 @@ __device__ __forceinline__ bool MeetAny(int id, int threads, bool any) {
   return r != 0;
 }
 
-// Grid (256-vector tile, kv head, sequence).
+// Grid (tile of kHalves * 128 vectors, kv head, sequence).
 template <int D>
-__global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
+__global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     AttnTilesQ8Kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const AttnArgs a) {
   using L = Tiles<D>;
   extern __shared__ char smem_raw[];
@@ -198,8 +210,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
   const Run run = RunOf(a.rows, b, c.context, blockIdx.x == 0 && g == 0 && tid == 0, a.status);
   const int64_t vectors = static_cast<int64_t>(run.count) * G;
   // Latest rows (the longest walks) first.
-  const int64_t tiles = (vectors + 2 * kHalf - 1) / (2 * kHalf);
-  const int64_t v0 = (tiles - 1 - static_cast<int64_t>(blockIdx.x)) * (2 * kHalf);
+  constexpr int kVectors = L::kHalves * kHalf;
+  const int64_t tiles = (vectors + kVectors - 1) / kVectors;
+  const int64_t v0 = (tiles - 1 - static_cast<int64_t>(blockIdx.x)) * kVectors;
   if (v0 < 0) {
     PdlTrigger();
     return;
@@ -222,7 +235,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
   }
   // TMEM is taken behind the wait for the previous kernel, and the next kernel
   // is let in behind that: neither can hold the columns the other waits for.
-  if (warp == L::kMmaWarp) TmemAlloc(&bars.tmem, kTmemCols);
+  if (warp == L::kMmaWarp) TmemAlloc(&bars.tmem, L::kTmemCols);
   // Every role passes here once, the softmax with its queries' loads in flight.
   const auto set_up = [&] {
     TcFenceBeforeSync();
@@ -235,13 +248,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
   // The tiles: those of the sinks before the windows, then the windows.
   const int64_t row_of_v0 = v0 / G;
   const uint32_t head_of_v0 = static_cast<uint32_t>(v0 - row_of_v0 * G);
-  const int64_t v_last = Min64(v0 + 2 * kHalf, vectors) - 1;
+  const int64_t v_last = Min64(v0 + kVectors, vectors) - 1;
   const Range all = RangeOf(v0, v_last, G, run.pos0, a.window);
   const int tile0 = all.near_lo / kTile;
   const int sink_tiles = static_cast<int>(Min64((static_cast<int64_t>(a.sinks) + kTile - 1) / kTile, tile0));
   const int n = sink_tiles + all.pos_hi / kTile - tile0 + 1;
   const auto token_of = [&](int j) { return (j < sink_tiles ? j : tile0 + (j - sink_tiles)) * kTile; };
-  const bool second = v0 + kHalf < vectors;
+  const bool second = L::kHalves > 1 && v0 + kHalf < vectors;
   // Half w's vectors, and whether they see any of tile j.
   const auto half_range = [&](int w) {
     const int64_t lo = Min64(v0 + w * kHalf, v_last);
@@ -276,7 +289,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
     constexpr int kOwn = kTile / kParts, kOwnChunks = kChunks / kParts, kDims = D / kParts;
     // What the threads of a vector tell each other, over a barrier of their two warps.
     float* factors = reinterpret_cast<float*>(smem + L::kShared) + w * kHalf;
-    float* tops = reinterpret_cast<float*>(smem + L::kShared) + 2 * kHalf + w * kParts * kHalf;
+    float* tops = reinterpret_cast<float*>(smem + L::kShared) + (L::kHalves + w * kParts) * kHalf;
     const auto meet = [&](bool bad) { return MeetAny(2 + w * 4 + quad, kParts * 32, bad); };
     // The queries as two fp16 parts of q * 2^e, their largest element at 2^13.
     // Four lanes load a vector, a warp 8 at a time.
@@ -505,7 +518,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
       }
       if (kParts > 1) {
         // Every other tile's exchange has its own place: the last one may still be read.
-        float* t = tops + (taken & 1) * 2 * kParts * kHalf;
+        float* t = tops + (taken & 1) * L::kHalves * kParts * kHalf;
         t[part * kHalf + r] = top;
         ok = !meet(!ok);
         top = fmaxf(top, t[(part ^ 1) * kHalf + r]);
@@ -562,7 +575,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
     if (!ok) l = __int_as_float(0x7fc00000);
     if (kParts > 1) {
       // The sum of all of the tokens' weights.
-      float* t = tops + (taken & 1) * 2 * kParts * kHalf;
+      float* t = tops + (taken & 1) * L::kHalves * kParts * kHalf;
       t[part * kHalf + r] = l;
       meet(false);
       l += t[(part ^ 1) * kHalf + r];
@@ -702,11 +715,11 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
         scores(w, j % L::kStages);
       };
       next_scores(0, 0);
-      next_scores(1, 0);
+      if (L::kHalves > 1) next_scores(1, 0);
       if (ok) MmaCommit(&bars.empty[0][0]);
       for (int j = 0; j < n && ok; ++j) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
+        for (int w = 0; w < L::kHalves; ++w) {
           if (ok && needed(w == 0 ? range0 : range1, w, j)) {
             ok = wait(&bars.weights[w], done[w] & 1) && wait(&bars.full[1][j % L::kStages], (j / L::kStages) & 1);
             if (!ok) continue;
@@ -727,7 +740,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
             }
           }
           // The values are free before the next scores are.
-          if (ok && w == 1) MmaCommit(&bars.empty[1][j % L::kStages]);
+          if (ok && w == L::kHalves - 1) MmaCommit(&bars.empty[1][j % L::kStages]);
           if (j + 1 < n) next_scores(w, j + 1);
         }
         if (!ok) break;
@@ -746,7 +759,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, 1)
   if (*failed != 0 && tid == 0) {
     if (a.status != nullptr) atomicOr(a.status, ACCEL_B200_STATUS_COPY_TIMEOUT);
   }
-  if (warp == L::kMmaWarp) TmemDealloc(bars.tmem, kTmemCols);
+  if (warp == L::kMmaWarp) TmemDealloc(bars.tmem, L::kTmemCols);
 }
 
 template <int D>
@@ -762,7 +775,7 @@ int Launch(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stre
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: cache tensor map rejected");
   }
   const int64_t vectors = static_cast<int64_t>(max_rows) * (a.heads / a.cache.kv_heads);
-  const dim3 grid(static_cast<unsigned>(CeilDiv(vectors, 2 * kHalf)), static_cast<unsigned>(a.cache.kv_heads),
+  const dim3 grid(static_cast<unsigned>(CeilDiv(vectors, Tiles<D>::kHalves * kHalf)), static_cast<unsigned>(a.cache.kv_heads),
                   static_cast<unsigned>(batch));
   return CheckLaunchEx(LaunchK(AttnTilesQ8Kernel<D>, grid, dim3(Tiles<D>::kThreads), kSmem, stream, 1u, 1u, tk, tv, a),
                        "attention_prefill_q8");

@@ -2,6 +2,8 @@
 
     python -m accelep_b200.profile_cases gemm [--path auto|tc|gemv|simt] [--shapes decode|prefill|c5|all]
     python -m accelep_b200.profile_cases attention [--batch 32] [--len 1280] [--kind fused|split|prefill]
+    python -m accelep_b200.profile_cases cache [--kind append|read|decode|prefill] [--batch 32] [--len 1280]
+                                               [--heads 9 --kv-heads 3 --head-dim 64] [--past 0] [--window 0]
     python -m accelep_b200.profile_cases step [--reps 3]
     python -m accelep_b200.profile_cases mlp [--reps 20]
     python -m accelep_b200.profile_cases list
@@ -213,15 +215,75 @@ def attention_case(batch, length, reps, kind="fused", context=2048, heads=9, kv_
     return {"case": f"attention_{kind}_b{batch}_len{length}", "us": round(us, 3), "gbs": round(nbytes / us / 1e3, 1)}
 
 
+def cache_case(kind, batch, length, reps, past=0, window=0, heads=9, kv_heads=3, head_dim=64, block=64):
+    """The int8 key/value cache: append or read back of `length` rows behind
+    `past` for each of `batch` sequences, decode attention of one row at
+    position past + length - 1, or prefill attention of the rows. Bytes and
+    operations counted: what the call cannot do without."""
+    context, rows = past + length, batch * length
+    copies = max(1, min(4, int(3e8 / (batch * kv_heads * context * head_dim * 2))))
+    caches = []
+    for _ in range(copies):
+        cache = K.Q8Cache.zeros(batch, kv_heads, context, head_dim, block)
+        for t in (cache.k, cache.v):
+            t.random_(-127, 128)
+        for t in (cache.k_scale, cache.v_scale):
+            t.fill_(2.0 ** -6)
+        caches.append(cache)
+
+    def ints(values):
+        return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+    first, count, pos0 = ints([b * length for b in range(batch)]), ints([length] * batch), ints([past] * batch)
+    seen = min(context, window) if window else context
+    kv = 2 * kv_heads * head_dim
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        if kind == "append":
+            x = torch.randn(rows, (heads + 2 * kv_heads) * head_dim, device="cuda")
+            q = torch.empty(rows, heads * head_dim, device="cuda")
+            cos_t, sin_t = torch.ones(context, head_dim, device="cuda"), torch.zeros(context, head_dim, device="cuda")
+            us = _time_graph(lambda i: K.rope_append_q8(x, caches[i % copies], first, count, pos0, heads, length, cos_t,
+                                                        sin_t, q_out=q), reps, stream)
+            nbytes, flops = rows * (8 * heads * head_dim + 5 * kv) + 8 * context * head_dim, 0
+        elif kind == "read":
+            outs = [torch.empty(rows, kv_heads * head_dim, device="cuda") for _ in range(2)]
+            us = _time_graph(lambda i: K.cache_rows_q8(caches[i % copies], first, count, pos0, length, *outs), reps,
+                             stream)
+            nbytes, flops = 5 * rows * kv, 0
+        elif kind == "decode":
+            q = torch.randn(batch, heads * head_dim, device="cuda")
+            out, pos = torch.empty_like(q), ints([context - 1] * batch)
+            ws = K.attention_decode_q8_workspace(caches[0], batch, heads, window)
+            us = _time_graph(lambda i: K.attention_decode_q8(q, caches[i % copies], pos, heads, window=window, out=out,
+                                                             workspace=ws), reps, stream)
+            nbytes, flops = batch * seen * kv, 4.0 * batch * heads * head_dim * seen
+        else:
+            q = torch.randn(rows, heads * head_dim, device="cuda")
+            out = torch.empty_like(q)
+            ws = K.attention_prefill_q8_workspace(caches[0], batch, length, heads, window)
+            us = _time_graph(lambda i: K.attention_prefill_q8(q, caches[i % copies], first, count, pos0, heads, length,
+                                                              window=window, out=out, workspace=ws), reps, stream)
+            each = sum(min(past + i + 1, window) if window else past + i + 1 for i in range(length))
+            nbytes, flops = batch * context * kv + 8 * rows * heads * head_dim, 4.0 * batch * heads * head_dim * each
+    return {"case": f"cache_{kind}_b{batch}_len{length}_past{past}_w{window}_{heads}x{kv_heads}x{head_dim}",
+            "us": round(us, 3), "gbs": round(nbytes / us / 1e3, 1), "tflops": round(flops / us / 1e6, 2)}
+
+
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("what", choices=["gemm", "attention", "step", "mlp", "list"])
+    ap.add_argument("what", choices=["gemm", "attention", "cache", "step", "mlp", "list"])
     ap.add_argument("--path", default="auto", choices=["auto", "tc", "gemv", "simt"])
     ap.add_argument("--shapes", default="decode", choices=["decode", "prefill", "c5", "all"])
     ap.add_argument("--batch", type=int, default=32)
     ap.add_argument("--len", type=int, default=1280)
     ap.add_argument("--reps", type=int, default=50)
-    ap.add_argument("--kind", default="fused", choices=["fused", "split", "prefill"])
+    ap.add_argument("--kind", default="", choices=["", "fused", "split", "prefill", "append", "read", "decode"])
+    ap.add_argument("--heads", type=int, default=9)
+    ap.add_argument("--kv-heads", type=int, default=3)
+    ap.add_argument("--head-dim", type=int, default=64)
+    ap.add_argument("--past", type=int, default=0)
+    ap.add_argument("--window", type=int, default=0)
     ap.add_argument("--only", default="", help="run one named gemm case")
     args = ap.parse_args()
     if args.what == "list":
@@ -242,8 +304,15 @@ def main():
         print(json.dumps(mlp_case(args.reps)), flush=True)
     elif args.what == "step":
         print(json.dumps(step_case(args.reps)), flush=True)
+    elif args.what == "cache":
+        if args.kind not in ("", "append", "read", "decode", "prefill"):
+            ap.error("cache kinds are append, read, decode and prefill")
+        print(json.dumps(cache_case(args.kind or "decode", args.batch, args.len, args.reps, args.past, args.window,
+                                    args.heads, args.kv_heads, args.head_dim)), flush=True)
     else:
-        print(json.dumps(attention_case(args.batch, args.len, args.reps, args.kind)), flush=True)
+        if args.kind not in ("", "fused", "split", "prefill"):
+            ap.error("attention kinds are fused, split and prefill")
+        print(json.dumps(attention_case(args.batch, args.len, args.reps, args.kind or "fused")), flush=True)
 
 
 if __name__ == "__main__":

@@ -377,22 +377,26 @@ class Q8Cache:
         return cls(*planes, *scales, block)
 
 
+_FLOAT32, _INT32 = torch.float32, torch.int32
+
+
 def _rows(name, t, index, width):
     """(rows, row stride) of a 2-D fp32 tensor of `width` columns on device `index`."""
     shape, stride = t.shape, t.stride()
-    if t.dtype is not torch.float32 or t.get_device() != index or len(shape) != 2 or shape[1] != width or stride[1] != 1:
+    if t.dtype is not _FLOAT32 or t.get_device() != index or len(shape) != 2 or shape[1] != width or stride[1] != 1:
         raise ValueError(f"{name} must be fp32 [rows, {width}] with contiguous rows on cuda:{index}")
+    rows = shape[0]
     # One row has no stride that matters (torch may report any).
-    return shape[0], stride[0] if shape[0] > 1 else max(stride[0], width)
+    return rows, stride[0] if rows > 1 else max(stride[0], width)
 
 
 def _i32(name, t, index, n):
-    """The address of a contiguous int32 vector of n on device `index` (None: 0)."""
+    """The address of n contiguous int32 on device `index` (None: 0)."""
     if t is None:
         return 0
-    if t.dtype is not torch.int32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 vector of {n} on cuda:{index}")
-    return t.data_ptr()
+    if t.numel() == n and t.dtype is _INT32 and t.get_device() == index and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name} must be {n} contiguous int32 on cuda:{index}")
 
 
 def _table(name, t, cache):
@@ -431,7 +435,7 @@ def rope_append_q8(qkv, cache, first, count, pos0, heads, max_rows, cos_t, sin_t
     queries [rows, heads * head_dim] (q_out; rows of no sequence are left)."""
     index, d = cache.index, cache.head_dim
     rows, ld = _rows("qkv", qkv, index, (heads + 2 * cache.kv_heads) * d)
-    batch = first.shape[0]
+    batch = first.numel()
     if q_out is None:
         q_out = torch.zeros(rows, heads * d, dtype=torch.float32, device=cache.device)
     q_rows, q_ld = _rows("q_out", q_out, index, heads * d)
@@ -447,7 +451,7 @@ def rope_append_q8(qkv, cache, first, count, pos0, heads, max_rows, cos_t, sin_t
 def cache_rows_q8(cache, first, count, pos0, max_rows, k_out=None, v_out=None, status=None):
     """Cache positions pos0[b] + i of slot b as fp32 into rows first[b] + i of
     k_out and v_out [rows, kv_heads * head_dim] (either may be None)."""
-    index, width, batch = cache.index, cache.kv_heads * cache.head_dim, first.shape[0]
+    index, width, batch = cache.index, cache.kv_heads * cache.head_dim, first.numel()
     k = v = None
     if k_out is not None:
         k = _rows("k_out", k_out, index, width)
@@ -518,7 +522,7 @@ def attention_prefill_q8(q, cache, first, count, pos0, heads, max_rows, window=0
     """Causal attention of sequence b's rows first[b] .. + count[b] - 1 of q
     (roped) at positions pos0[b] + i over slot b of an int8 cache that holds
     their keys and values. window and sinks as in attention_decode_q8."""
-    index, batch = cache.index, first.shape[0]
+    index, batch = cache.index, first.numel()
     rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
     if workspace is None:
         workspace = attention_prefill_q8_workspace(cache, batch, max_rows, heads, window, sinks)

@@ -626,3 +626,44 @@ def test_run_together_on_a_stream_and_replayed(lib, cuda):
         check_rows(c, H(step_q), H(step_out), [(b, b, int(at[b])) for b in live], heads, 0, 0)
         at[at >= 0] += 1
     assert H(status)[0] == 0
+
+
+def test_python_calls_refuse_other_tensors(lib, cuda):
+    dev = K.Q8Cache.zeros(2, 2, 100, 64, 32)
+    cos = torch.zeros(100, 64, device="cuda")
+    q, x, pos = torch.zeros(2, 256, device="cuda"), torch.zeros(2, 512, device="cuda"), I([0, 1])
+    out = torch.zeros(2, 128, device="cuda")
+    good = dict(cache=dev, first=pos, count=pos, pos0=pos, max_rows=1)
+    for change in ({"first": pos.long()}, {"count": I([1])}, {"pos0": pos.cpu()}, {"count": I([1, 0, 1, 0])[::2]}):
+        with pytest.raises(ValueError):
+            K.rope_append_q8(x, heads=4, cos_t=cos, sin_t=cos, **{**good, **change})
+        with pytest.raises(ValueError):
+            K.attention_prefill_q8(q, heads=4, **{**good, **change})
+        with pytest.raises(ValueError):
+            K.cache_rows_q8(k_out=out, **{**good, **change})
+    for bad in (x[:, :448], x.half(), x.cpu(), x.t().contiguous().t(), x.view(2, 2, 256)):
+        with pytest.raises((ValueError, TypeError, IndexError)):
+            K.rope_append_q8(bad, heads=4, cos_t=cos, sin_t=cos, **good)
+    for bad in (cos[:99], cos.double(), cos.cpu(), torch.zeros(100, 128, device="cuda")[:, ::2]):
+        with pytest.raises(ValueError):
+            K.rope_append_q8(x, heads=4, cos_t=bad, sin_t=cos, **good)
+    for bad in (q[:, :192], q.double(), q.cpu()):
+        with pytest.raises(ValueError):
+            K.attention_decode_q8(bad, dev, pos, 4)
+        with pytest.raises(ValueError):
+            K.attention_decode_q8(q, dev, pos, 4, out=bad)
+    for extra in ({"row_seq": pos.long()}, {"status": I([0, 0])}, {"out": torch.zeros(3, 256, device="cuda")},
+                  {"workspace": torch.zeros(8, device="cuda")}):
+        with pytest.raises(ValueError):
+            K.attention_decode_q8(q, dev, pos, 4, **extra)
+    with pytest.raises(ValueError):
+        K.cache_rows_q8(**good)
+    with pytest.raises(ValueError):
+        K.cache_rows_q8(k_out=out, v_out=torch.zeros(3, 128, device="cuda"), **good)
+    with pytest.raises(B200Error):
+        K.attention_decode_q8(torch.zeros(3, 256, device="cuda"), dev, I([0, 1, 2]), 4)  # more rows than slots
+    for bad in (dict(k=dev.k.float()), dict(v=dev.v[:, :, :50]), dict(k_scale=dev.k_scale[:, :, :3]),
+                dict(v_scale=dev.v_scale.double()), dict(k=dev.k.transpose(2, 3).contiguous().transpose(2, 3))):
+        planes = dict(k=dev.k, v=dev.v, k_scale=dev.k_scale, v_scale=dev.v_scale)
+        with pytest.raises(ValueError):
+            K.Q8Cache(**{**planes, **bad}, block=32)

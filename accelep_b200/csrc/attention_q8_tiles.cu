@@ -479,7 +479,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       // Weights carry their chunk's value scale relative to the tile's largest,
       // as a shift of the exponent, and the sum of weights takes it out again.
       // Where scales are so far apart that the smaller ones' weights would lose
-      // bits, each chunk is summed on its own.
+      // bits, each chunk is summed on its own; and where the largest is 0 or below
+      // 2^-128, whose reciprocal is infinite.
       float ks[kChunks], lift[kChunks], v_now = 0.f;
       bool apart = false;
 #pragma unroll
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
         lift[k] = lift[k] == -1.f ? 0.f : __log2f(lift[k] * v_inv);
-        apart = apart || !(lift[k] >= -kMostLift);
+        apart = apart || !(fabsf(lift[k]) <= kMostLift);
       }
       if (apart) {
 #pragma unroll

@@ -459,6 +459,36 @@ def test_value_scales_far_apart(lib, cuda, d, apart):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [2.0 ** -149, 2.0 ** -135, 2.0 ** -127])
+def test_subnormal_value_scales(lib, cuda, d, scale):
+    """Scales below 2^-128 have no finite reciprocal. Sums of values this small
+    are multiples of 2^-149, so besides its share of the magnitudes a result may
+    be off by half of that for its own rounding, and each rounding before it by
+    half of it in a unit of which the sum of weights is at least 2^10. There are
+    three per 32 tokens at most: a partial sum, a moved reference, and a merge of
+    states (4 warps' and those of a CTA per 256 tokens)."""
+    rng = np.random.default_rng(d)
+    heads, kv, context, n = 4, 2, 2400, 60
+    c = filled(rng, 1, kv, context, d, 64)
+    c.s["v"][:] = scale
+    q = rng.standard_normal((n, heads * d), dtype=np.float32)
+    dev = device_cache(c)
+
+    def near(got, row, pos):
+        want, tol = O.attend(c, q[row].reshape(heads, d), 0, pos)
+        limit = tol - 1e-30 + (0.5 + 3 * (pos / 32 + 6) / 2 ** 11) * 2.0 ** -149
+        assert (np.abs(got[row].reshape(heads, d) - want) <= limit).all(), (row, pos)
+
+    for most in (n, context):
+        got = H(K.attention_prefill_q8(T(q), dev, I([0]), I([n]), I([1000]), heads, most))
+        for r in (0, 31, n - 1):
+            near(got, r, 1000 + r)
+    got = H(K.attention_decode_q8(T(q[:2]), dev, I([5, 2399]), heads, row_seq=I([0, 0])))
+    near(got, 0, 5)
+    near(got, 1, 2399)
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_attention_in_place(lib, cuda, d):
     """out may be q: every split of a row has read it before it is written."""
     rng = np.random.default_rng(d)

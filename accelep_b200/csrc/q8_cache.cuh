@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <utility>
 
 #include "accel_b200.h"
 #include "common.cuh"
@@ -34,12 +35,40 @@ inline bool RowsApart(const float* a, int64_t lda, int64_t wa, const float* b, i
   return delta > 0 ? delta >= wa && (rows == 1 || delta + wb <= lda) : -delta >= wb && (rows == 1 || wa - delta <= lda);
 }
 
+// Whether runs of one layout touch runs of another like it (Disjoint in itself)
+// that lies `delta` elements behind. A run of the other reaches a run of the
+// first only next to where the strides put it: two candidates per level.
+inline bool Touch(int64_t delta, int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t inner) {
+  if (n0 <= 1 || (n1 > 1 && s1 > s0)) {  // the wider stride first; a stride of one run counts for nothing
+    std::swap(n0, n1);
+    std::swap(s0, s1);
+  }
+  const auto steps = [](int64_t d, int64_t n, int64_t s) { return n <= 1 ? 0 : d / s - (d % s < 0 ? 1 : 0); };
+  for (int i = 0; i < 2; ++i) {
+    const int64_t i0 = steps(delta, n0, s0) + i;
+    if (i0 <= -n0 || i0 >= n0) continue;
+    const int64_t rest = delta - (i0 != 0 ? i0 * s0 : 0);
+    for (int j = 0; j < 2; ++j) {
+      const int64_t i1 = steps(rest, n1, s1) + j;
+      if (i1 <= -n1 || i1 >= n1) continue;
+      const int64_t off = rest - (i1 != 0 ? i1 * s1 : 0);
+      if (off > -inner && off < inner) return true;
+    }
+  }
+  return false;
+}
+
+constexpr int64_t kMostRows = (int64_t{1} << 31) - 256;  // of a plane: row numbers are 32-bit in its tensor map
+
 // Rows of head_dim bytes from the first of a plane to behind its last run; row
 // t of (slot s, head g) is (s * seq_stride + g * head_stride) / head_dim + t.
+// Above kMostRows: some number above it.
 inline int64_t PlaneRows(const accel_b200_q8_cache& c) {
-  const int64_t last = (c.slots > 1 ? (c.slots - 1) * c.seq_stride : 0) +
-                       (c.kv_heads > 1 ? (c.kv_heads - 1) * c.head_stride : 0);
-  return last / c.head_dim + c.context;
+  const auto span = [&](int64_t n, int64_t stride) {
+    if (n <= 1) return int64_t{0};
+    return stride / c.head_dim > kMostRows / (n - 1) ? kMostRows : (n - 1) * (stride / c.head_dim);
+  };
+  return span(c.slots, c.seq_stride) + span(c.kv_heads, c.head_stride) + c.context;
 }
 
 // ACCEL_B200_OK, or EINVAL with a message that begins with `what`.
@@ -48,7 +77,6 @@ inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
   if (c == nullptr || c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) {
     return SetError(ACCEL_B200_EINVAL, w + ": the cache has a null plane");
   }
-  if (c->k == c->v || c->k_scale == c->v_scale) return SetError(ACCEL_B200_EINVAL, w + ": keys and values are one plane");
   if (c->head_dim != 64 && c->head_dim != 128) {
     return SetError(ACCEL_B200_EINVAL, w + ": head_dim must be 64 or 128");
   }
@@ -72,7 +100,12 @@ inline int CheckQ8Cache(const accel_b200_q8_cache* c, const char* what) {
       !Disjoint(c->slots, c->scale_seq_stride, c->kv_heads, c->scale_head_stride, blocks)) {
     return SetError(ACCEL_B200_EINVAL, w + ": cache strides do not hold the context");
   }
-  if (PlaneRows(*c) > (int64_t{1} << 31) - 256) return SetError(ACCEL_B200_EINVAL, w + ": more than 2^31 cache rows");
+  const int64_t scales = reinterpret_cast<intptr_t>(c->v_scale) / 4 - reinterpret_cast<intptr_t>(c->k_scale) / 4;
+  if (Touch(c->v - c->k, c->slots, c->seq_stride, c->kv_heads, c->head_stride, run) ||
+      Touch(scales, c->slots, c->scale_seq_stride, c->kv_heads, c->scale_head_stride, blocks)) {
+    return SetError(ACCEL_B200_EINVAL, w + ": keys and values overlap");
+  }
+  if (PlaneRows(*c) > kMostRows) return SetError(ACCEL_B200_EINVAL, w + ": more than 2^31 cache rows");
   return ACCEL_B200_OK;
 }
 

@@ -450,9 +450,10 @@ ACCEL_B200_API int accel_b200_decode_attention_prefetch(
    head_stride + t * head_dim + d] and stands for that integer times
    k_scale[s * scale_seq_stride + g * scale_head_stride + t / block]; v the
    same. The planes are 16-byte aligned with strides that are multiples of
-   head_dim, the scales 4-byte aligned; no two (slot, head) runs overlap, in
-   either order of slots and heads, and a plane spans less than 2^31 rows. head_dim is 64 or 128, block 32, 64 or 128 tokens.
-   Device memory of the current device throughout. */
+   head_dim, the scales 4-byte aligned; no two (slot, head) runs overlap, of one
+   plane (in either order of slots and heads) or of keys and values, and a
+   plane spans less than 2^31 rows. head_dim is 64 or 128, block 32, 64 or 128
+   tokens. Device memory of the current device throughout. */
 typedef struct accel_b200_q8_cache {
   int8_t* k;
   int8_t* v;
@@ -518,8 +519,9 @@ ACCEL_B200_API int accel_b200_cache_rows_q8(const accel_b200_q8_cache* cache, co
    row_pos[r] < 0 are skipped (their output is not written); a position or
    slot outside the cache is skipped with ACCEL_B200_STATUS_BAD_POSITION.
    heads is any multiple of kv_heads; rows are 16-byte aligned; out may be q
-   itself. Scales of blocks that a row sees are finite and not negative; other
-   blocks may hold anything. Equal calls give equal bits.
+   itself. Scales of blocks that a row sees are not negative and at most 2^64
+   (sums of weights up to 2^44 times values stay finite); other blocks may hold
+   anything. Equal calls give equal bits.
    The workspace holds accel_b200_attention_decode_q8_workspace(...) bytes (0:
    none) whose first 64 KiB are zero before the first call, as for the
    products; every call leaves them zero. Calls that share it must not overlap
@@ -548,8 +550,8 @@ ACCEL_B200_API int accel_b200_attention_decode_q8_prefetch(
 
 /* The same attention for many rows of each sequence: rows first[b] ..
    first[b] + count[b] - 1 of q and out (`rows` of them in all, max_rows >=
-   every count) at positions pos0[b] + i of slot b; the cache already holds
-   their keys and values. Sequences are skipped as by
+   every count) at positions pos0[b] + i of slot b, no row of two sequences; the
+   cache already holds their keys and values. Sequences are skipped as by
    accel_b200_rope_append_q8 (a skipped sequence's output is not written).
    Workspace as above. */
 ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200_q8_cache* cache, int32_t batch,

@@ -26,7 +26,11 @@ def cache(**change):
 BAD_CACHES = [{"k": None}, {"v_scale": None}, {"head_dim": 96}, {"head_dim": 32}, {"block": 16}, {"block": 0},
               {"block": 48}, {"slots": 0}, {"kv_heads": 0}, {"context": 0}, {"k": P + 8}, {"v_scale": P + 2}, {"v": P}, {"v_scale": 3 * P},
               {"head_stride": 99 * 64}, {"seq_stride": 100 * 64}, {"seq_stride": 2 * 100 * 64 + 8},
-              {"scale_head_stride": 1}, {"scale_seq_stride": 3}, {"head_stride": -100 * 64}]
+              {"scale_head_stride": 1}, {"scale_seq_stride": 3}, {"head_stride": -100 * 64},
+              {"seq_stride": 64 << 56}, {"head_stride": 64 << 56, "seq_stride": 64 << 57},
+              {"seq_stride": 64 << 30}, {"seq_stride": 64 << 55, "slots": 1 << 10},
+              {"v": P + 99 * 64}, {"v": P - 64}, {"v": P + 5 * 100 * 64}, {"v": P + 2 * 2 * 100 * 64 + 16},
+              {"v_scale": 3 * P + 4}, {"v_scale": 3 * P - 4 * 11}]
 
 
 def append(lib, c, **change):
@@ -115,6 +119,12 @@ def test_empty_calls_queue_nothing(lib):
     {"seq_stride": 100 * 64, "head_stride": 3 * 100 * 64, "scale_seq_stride": 2, "scale_head_stride": 6},  # heads outside
     {"slots": 1, "seq_stride": 0, "scale_seq_stride": 0},       # one slot: its stride is never used
     {"kv_heads": 1, "head_stride": 0, "scale_head_stride": 0},  # one head: the same
+    # Keys and values by turns: of each (slot, head), of each slot, of all.
+    {"v": P + 100 * 64, "head_stride": 2 * 100 * 64, "seq_stride": 4 * 100 * 64, "v_scale": 3 * P + 8,
+     "scale_head_stride": 4, "scale_seq_stride": 8},
+    {"v": P - 2 * 100 * 64, "seq_stride": 4 * 100 * 64, "v_scale": 3 * P + 16, "scale_seq_stride": 8},
+    {"v": P + 6 * 100 * 64, "v_scale": 3 * P - 48},
+    {"v": P + 64 * 100, "seq_stride": 64 << 29, "slots": 4, "head_stride": 64 << 27},
 ])
 def test_other_orders_of_the_cache_are_taken(lib, order):
     batch = {"batch": min(3, order.get("slots", 3)), "max_rows": 0}

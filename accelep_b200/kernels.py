@@ -352,6 +352,8 @@ class Q8Cache:
 
     def __init__(self, k, v, k_scale, v_scale, block=64):
         slots, kv_heads, context, head_dim = k.shape
+        if block not in (32, 64, 128):
+            raise ValueError("block must be 32, 64 or 128 tokens")
         blocks = -(-context // block)
         for name, t, dtype, shape in (("k", k, torch.int8, k.shape), ("v", v, torch.int8, k.shape),
                                       ("k_scale", k_scale, torch.float32, (slots, kv_heads, blocks)),
@@ -372,6 +374,8 @@ class Q8Cache:
 
     @classmethod
     def zeros(cls, slots, kv_heads, context, head_dim, block=64, device="cuda"):
+        if block not in (32, 64, 128):
+            raise ValueError("block must be 32, 64 or 128 tokens")
         planes = [torch.zeros(slots, kv_heads, context, head_dim, dtype=torch.int8, device=device) for _ in range(2)]
         scales = [torch.zeros(slots, kv_heads, -(-context // block), device=device) for _ in range(2)]
         return cls(*planes, *scales, block)
@@ -397,6 +401,13 @@ def _i32(name, t, index, n):
     if t.numel() == n and t.dtype is _INT32 and t.get_device() == index and t.is_contiguous():
         return t.data_ptr()
     raise ValueError(f"{name} must be {n} contiguous int32 on cuda:{index}")
+
+
+def _counts(*numbers):
+    """Refuses what a C int would hold as another number."""
+    for n in numbers:
+        if not 0 <= n <= 0x7fffffff:
+            raise ValueError(f"{n} is not a count of 31 bits")
 
 
 def _table(name, t, cache):
@@ -441,6 +452,9 @@ def rope_append_q8(qkv, cache, first, count, pos0, heads, max_rows, cos_t, sin_t
     q_rows, q_ld = _rows("q_out", q_out, index, heads * d)
     if q_rows != rows:
         raise ValueError("q_out must have a row for each row of qkv")
+    _counts(max_rows)
+    if rows == 0 or batch == 0:
+        return q_out
     _call(index, load().accel_b200_rope_append_q8, qkv.data_ptr(), ld, rows, cache._ref,
           _i32("first", first, index, batch), _i32("count", count, index, batch), _i32("pos0", pos0, index, batch),
           batch, max_rows, heads, _table("cos_t", cos_t, cache), _table("sin_t", sin_t, cache), q_out.data_ptr(), q_ld,
@@ -460,6 +474,9 @@ def cache_rows_q8(cache, first, count, pos0, max_rows, k_out=None, v_out=None, s
     if (k or v) is None or (k is not None and v is not None and k != v):
         raise ValueError("k_out and v_out must have the same rows and strides, and one must be given")
     rows, ld = k or v
+    _counts(max_rows)
+    if rows == 0 or batch == 0:
+        return k_out, v_out
     _call(index, load().accel_b200_cache_rows_q8, cache._ref, _i32("first", first, index, batch),
           _i32("count", count, index, batch), _i32("pos0", pos0, index, batch), batch, max_rows,
           0 if k is None else k_out.data_ptr(), 0 if v is None else v_out.data_ptr(), ld, rows,
@@ -482,6 +499,7 @@ def _attention_io(q, cache, heads, out):
 def attention_decode_q8_workspace(cache, rows, heads, window=0, sinks=0):
     """A zeroed workspace for attention_decode_q8 calls of these sizes (None:
     none needed)."""
+    _counts(rows, window, sinks)
     need = load().accel_b200_attention_decode_q8_workspace(cache._ref, rows, heads, window, sinks)
     return torch.zeros(need, dtype=torch.uint8, device=cache.device) if need else None
 
@@ -496,6 +514,9 @@ def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=
     options (ATTN_CACHE_BEFORE_WAIT)."""
     index = cache.index
     rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
+    _counts(window, sinks)
+    if rows == 0:
+        return out
     if workspace is None:
         workspace = attention_decode_q8_workspace(cache, rows, heads, window, sinks)
     ws, ws_bytes = _bytes(workspace, index)
@@ -505,6 +526,9 @@ def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=
     if prefetch is None and flags == 0:
         _call(index, load().accel_b200_attention_decode_q8, *args)
     else:
+        for t in prefetch or []:
+            if t.get_device() != index or not t.is_contiguous():
+                raise ValueError(f"prefetch takes contiguous tensors on cuda:{index}")
         _call(index, load().accel_b200_attention_decode_q8_prefetch, *args,
               ctypes.byref(_l2_prefetch(prefetch or [], flags)))
     return out
@@ -513,6 +537,7 @@ def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=
 def attention_prefill_q8_workspace(cache, batch, max_rows, heads, window=0, sinks=0):
     """A zeroed workspace for attention_prefill_q8 calls of these sizes (None:
     none needed)."""
+    _counts(batch, max_rows, window, sinks)
     need = load().accel_b200_attention_prefill_q8_workspace(cache._ref, batch, max_rows, heads, window, sinks)
     return torch.zeros(need, dtype=torch.uint8, device=cache.device) if need else None
 
@@ -524,6 +549,9 @@ def attention_prefill_q8(q, cache, first, count, pos0, heads, max_rows, window=0
     their keys and values. window and sinks as in attention_decode_q8."""
     index, batch = cache.index, first.numel()
     rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
+    _counts(max_rows, window, sinks)
+    if rows == 0 or batch == 0:
+        return out
     if workspace is None:
         workspace = attention_prefill_q8_workspace(cache, batch, max_rows, heads, window, sinks)
     ws, ws_bytes = _bytes(workspace, index)

@@ -151,3 +151,12 @@ def test_python_cache_refuses_host_tensors():
     s = torch.zeros(1, 1, 1)
     with pytest.raises(ValueError):
         K.Q8Cache(k, k.clone(), s, s.clone())
+
+
+@pytest.mark.parametrize("block", [0, -64, 16, 65])
+def test_python_cache_refuses_other_blocks(block):
+    k, s = torch.zeros(1, 1, 8, 64, dtype=torch.int8), torch.zeros(1, 1, 1)
+    with pytest.raises(ValueError, match="block"):
+        K.Q8Cache(k, k.clone(), s, s.clone(), block)
+    with pytest.raises(ValueError, match="block"):
+        K.Q8Cache.zeros(1, 1, 8, 64, block, device="cpu")

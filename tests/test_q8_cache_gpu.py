@@ -697,3 +697,31 @@ def test_python_calls_refuse_other_tensors(lib, cuda):
         planes = dict(k=dev.k, v=dev.v, k_scale=dev.k_scale, v_scale=dev.v_scale)
         with pytest.raises(ValueError):
             K.Q8Cache(**{**planes, **bad}, block=32)
+    for number in (-1, 1 << 31, (1 << 32) + 5):
+        for name in ("window", "sinks"):
+            with pytest.raises(ValueError):
+                K.attention_decode_q8(q, dev, pos, 4, **{name: number})
+            with pytest.raises(ValueError):
+                K.attention_prefill_q8(q, heads=4, **{**good, name: number})
+        for call, kind in ((K.rope_append_q8, dict(qkv=x, heads=4, cos_t=cos, sin_t=cos)), (K.cache_rows_q8, dict(k_out=out)),
+                           (K.attention_prefill_q8, dict(q=q, heads=4))):
+            with pytest.raises(ValueError):
+                call(**{**good, **kind, "max_rows": number})
+    for bad in (x[:, ::2], x.cpu(), torch.zeros(1, device="cuda").expand(1 << 20)):
+        with pytest.raises(ValueError):
+            K.attention_decode_q8(q, dev, pos, 4, prefetch=[bad])
+
+
+def test_python_calls_of_nothing(lib, cuda):
+    """No rows, or no sequences, of any call: nothing runs and nothing is refused."""
+    dev = K.Q8Cache.zeros(2, 2, 100, 64, 32)
+    cos, one, none = torch.zeros(100, 64, device="cuda"), I([0, 1]), I([])
+    before = lib.accel_b200_launch_count()
+    for rows, seqs in ((0, one), (3, none), (0, none)):
+        x, q, kv = (torch.ones(rows, n, device="cuda") for n in (512, 256, 128))
+        run = dict(cache=dev, first=seqs, count=seqs, pos0=seqs, max_rows=1)
+        assert K.rope_append_q8(x, heads=4, cos_t=cos, sin_t=cos, **run).shape == q.shape
+        assert K.attention_prefill_q8(q, heads=4, **run).shape == q.shape
+        assert K.cache_rows_q8(k_out=kv, **run)[0] is kv
+    assert K.attention_decode_q8(torch.ones(0, 256, device="cuda"), dev, none, 4).shape == (0, 256)
+    assert lib.accel_b200_launch_count() == before

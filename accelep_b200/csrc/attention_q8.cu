@@ -7,8 +7,9 @@
 // an exact fp16 number, and a query or a weight is the sum of two fp16 numbers
 // (22 bits), whose products with it are exact in fp32. The two parts of 8
 // vectors (query rows x heads that share a kv head) are the 16 rows of one
-// MMA operand, so the pair costs no more than 16 single-precision-less vectors
-// would. Queries are scaled by a power of two to 2^13 and weights to about
+// MMA operand. (The 128-row tiles of attention_q8_tiles.cu would stand almost
+// empty here: a decoded row brings heads / kv_heads vectors, 3 to 8 in common
+// models.) Queries are scaled by a power of two to 2^13 and weights to about
 // 2^10, so their second parts stay far above fp16's smallest step.
 //
 // Work split. A warp owns 8 vectors and walks units of 32 tokens, which TMA
@@ -17,13 +18,13 @@
 // free to choose, and is chosen so that a lane's share of an MMA operand is a
 // run of bytes, the shared-memory reads have no bank conflicts under TMA's
 // swizzle, and the scores' register layout is the weights' operand layout.
-// (Measured at 4 sequences of 40001..65536 tokens, 8 kv heads of 128: 80 us,
-// 5.4 TB/s. Before the split by lengths it took 88 us, with loads to registers
-// 128 and with per-lane cp.async 132: an SM keeps too few of those in flight.) Units are dealt to all warps of the
-// S CTAs of a vector group in turn. Each unit's weighted values are summed on
-// their own and added, times the unit's value scale, to fp32 registers (the
-// tensor core's running sum rounds towards zero, which would drift over a long
-// context).
+// Units are dealt to all warps of the S CTAs of a vector group in turn. Each
+// unit's weighted values are summed on their own and added, times the unit's
+// value scale, to fp32 registers (the tensor core's running sum rounds towards
+// zero, which would drift over a long context). Measured at 4 sequences of 40001
+// to 65536 tokens, 8 kv heads of 128: 80 us, 5.4 TB/s. Before the split by lengths
+// it took 88 us, with loads to registers 128 and with per-lane cp.async 132: an SM
+// keeps too few of those in flight.
 //
 // Online softmax in base 2 against a reference that moves only when a score
 // passes it by more than kSlack (a vote; no weight above 2^(kBias + kSlack)).

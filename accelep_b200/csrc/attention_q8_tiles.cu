@@ -766,6 +766,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
 template <int D>
 int Launch(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stream) {
   constexpr int kSmem = Tiles<D>::kBytes + Tiles<D>::kAlign;
+  // The roles trade the registers that the launch gives out; were they fewer
+  // than the split adds up to, the role that takes more would wait for good.
+  static const int regs = [] {
+    cudaFuncAttributes f{};
+    return cudaFuncGetAttributes(&f, AttnTilesQ8Kernel<D>) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (regs != Tiles<D>::kLaunch) return SetError(ACCEL_B200_ECUDA, "attention_prefill_q8: the kernel's registers do not fit its split");
   const cudaError_t err =
       cudaFuncSetAttribute(AttnTilesQ8Kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (err != cudaSuccess) return CheckLaunchEx(err, "attention_prefill_q8");

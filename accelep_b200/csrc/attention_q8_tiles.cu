@@ -75,8 +75,9 @@ struct Tiles {
   static_assert(kHalves * kCtas * kHalf == kTileVectors, "");
   static constexpr int kSoftWarps = 4 * kParts * kHalves, kMmaWarp = kSoftWarps + kConverters;
   static constexpr int kThreads = (kSoftWarps + 8) * 32;  // whole warpgroups
-  // Registers of the softmax threads and of the others from their start on:
-  // in all no more than the launch gives out (a multiple of 8 each).
+  // Registers of the softmax threads and of the others from their start on: in
+  // all no more than the launch gives out (a multiple of 8 each). With 8 more or
+  // fewer for the others calls take 1 to 4% longer.
   static constexpr int kLaunch = 65536 / (kThreads * kCtas) / 8 * 8;
   static constexpr int kLess = D == 64 ? 32 : 48, kMore = kLaunch + (kLaunch - kLess) * 256 / (kSoftWarps * 32);
   static_assert(kMore % 8 == 0 && kSoftWarps * 32 * kMore + 256 * kLess <= kThreads * kLaunch, "");
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     const int my_pos = mine ? run.pos0 + static_cast<int>(row_of_v0 + my_down) : range.pos_hi;
     const int my_near = NearOf(my_pos, a.window);
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    constexpr int kOwn = kTile / kParts, kOwnChunks = kChunks / kParts, kDims = D / kParts;
+    constexpr int kOwnChunks = kChunks / kParts, kDims = D / kParts;
     // What the threads of a vector tell each other, over a barrier of their two warps.
     float* factors = reinterpret_cast<float*>(smem + L::kShared) + w * kHalf;
     float* tops = reinterpret_cast<float*>(smem + L::kShared) + (L::kHalves + w * kParts) * kHalf;
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       }
     }
 
-    const uint32_t my_scores = tmem + lanes + L::kScores + w * kTile + part * kOwn;
+    const uint32_t my_scores = tmem + lanes + L::kScores + w * kTile;
     const uint32_t my_out = tmem + lanes + L::kOut + w * D + part * kDims;
     float m = -INFINITY, l = 0.f, v_ref = 0.f;
     Pair o[kDims / 2];  // weighted values of dimensions 2 d and 2 d + 1 of this part
@@ -400,9 +401,10 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       float top = -INFINITY;
 #pragma unroll 1
       for (int i0 = 0; i0 < kOwnChunks; ++i0) {
-        const int k = part * kOwnChunks + i0;
+        const int k = i0 * kParts + part;
+        if (!kWhole && !SeesSome(range, t0 + k * kChunk, kChunk, a.sinks)) continue;
         uint32_t x[32];
-        TmemLoad32Raw(my_scores + i0 * kChunk, x);
+        TmemLoad32Raw(my_scores + k * kChunk, x);
         const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
         TmemWaitLoads(x);
         float mx = -INFINITY;
@@ -421,7 +423,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       constexpr bool kWhole = decltype(whole)::value;
 #pragma unroll 1
       for (int i0 = 0; i0 < kOwnChunks; ++i0) {
-        const int k = part * kOwnChunks + i0;
+        const int k = i0 * kParts + part;
+        if (!kWhole && !SeesSome(range, t0 + k * kChunk, kChunk, a.sinks)) {
+          const uint32_t none[16] = {};
+          TmemStore16Raw(my_scores + k * kChunk, none);
+          TmemStore16Raw(my_scores + k * kChunk + 16, none);
+          continue;
+        }
         const float f = factor * pick(ks, k), up = pick(lift, k), shift = ref - up;
         const uint32_t mask = kWhole ? ~0u : mask_of(t0 + k * kChunk);
         const Pair f2 = MakePair(f, f), shift2 = MakePair(-shift, -shift), minus2 = MakePair(-1.f, -1.f);
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t x[16], y[16];
-          TmemLoad16Raw(my_scores + i0 * kChunk + 16 * h, x);
+          TmemLoad16Raw(my_scores + k * kChunk + 16 * h, x);
           TmemWaitLoads(x);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
@@ -450,7 +458,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
             y[i / 2] = *reinterpret_cast<const uint32_t*>(&hi);
             y[8 + i / 2] = *reinterpret_cast<const uint32_t*>(&lo);
           }
-          TmemStore16Raw(my_scores + i0 * kChunk + 16 * h, y);
+          TmemStore16Raw(my_scores + k * kChunk + 16 * h, y);
         }
         const float2 sums = Split2(sum2);
         const float sum = sums.x + sums.y;

@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   const accel_b200_q8_cache& c = a.cache;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
   constexpr bool kRuns = kRows == Rows::kRuns;
-  const int G = a.heads / c.kv_heads;
+  const int G = a.group;
   int S = static_cast<int>(gridDim.x), split = static_cast<int>(blockIdx.x), pair = static_cast<int>(blockIdx.y);
   int64_t z = blockIdx.z;
   if constexpr (kRows == Rows::kBalanced) {
@@ -179,15 +179,15 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   // The rows: `count` from `first` at positions pos0 + i of `slot`. A single
   // row's query does not wait for its position.
   float x[kKw][4];
-  const auto load_query = [&](int64_t row, int64_t vec, bool some) {
-    const float* q = a.q + row * a.q_ld + static_cast<int64_t>(g * G + vec % G) * D + tig * 16;
+  const auto load_query = [&](int64_t row, int head, bool some) {
+    const float* q = a.q + row * a.q_ld + static_cast<int64_t>(g * G + head) * D + tig * 16;
 #pragma unroll
     for (int j = 0; j < kKw; ++j) {
       *reinterpret_cast<float4*>(x[j]) = some ? *reinterpret_cast<const float4*>(q + (j / 4) * 64 + (j % 4) * 4)
                                               : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  if (!kRuns && !early) load_query(z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
+  if (!kRuns && !early) load_query(z, group * kVec + gid, group * kVec + gid < G);
   int64_t first, slot;
   int count, pos0;
   if (kRuns) {
@@ -213,10 +213,14 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
     if (early) PdlWait();
     return;
   }
-  const int row_lo = static_cast<int>(v0 / G);
-  const int row_hi = static_cast<int>(Min64(v0 + kVec - 1, vectors - 1) / G);
-  const bool mine = v0 + gid < vectors;
-  const int my_row = mine ? static_cast<int>((v0 + gid) / G) : row_hi;
+  // (A single row's vectors are its heads.)
+  const Vectors place(kRuns ? v0 : 0, G);
+  const int top_vec = static_cast<int>(Min64(kVec, vectors - v0)) - 1;
+  const int row_lo = kRuns ? static_cast<int>(place.row0) : 0;
+  const int row_hi = kRuns ? row_lo + static_cast<int>(place.Down(top_vec)) : 0;
+  const bool mine = gid <= top_vec;
+  const uint32_t my_down = kRuns ? place.Down(gid) : 0;
+  const int my_row = mine && kRuns ? row_lo + static_cast<int>(my_down) : row_hi;
   const int my_pos = pos0 + my_row, my_near = NearOf(my_pos, a.window);
   const int pos_lo = pos0 + row_lo, pos_hi = pos0 + row_hi;
   const int near_lo = NearOf(pos_lo, a.window), near_hi = NearOf(pos_hi, a.window);
@@ -228,7 +232,8 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
 
   const float* ksp = c.k_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
   const float* vsp = c.v_scale + slot * c.scale_seq_stride + g * c.scale_head_stride;
-  const int per_block = c.block / kUnit;
+  const int unit_shift = a.block_shift - 5;  // units per scale block
+  static_assert(kUnit == 32, "");
   const int plane_row = static_cast<int>((slot * c.seq_stride + g * c.head_stride) / D);
 
   // One lane of the warp copies its units; rows behind the context are of the
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   }
   int u = split * kWarps + warp;
   // Units in front of the row's own block do not wait for the previous kernel.
-  const int settled = early ? pos_lo / c.block * c.block : 0;
+  const int settled = early ? pos_lo >> a.block_shift << a.block_shift : 0;
   const auto settles = [&](int i) { return u + i * step < units && unit_of(u + i * step) * kUnit < settled; };
   if (early) {
 #pragma unroll
@@ -259,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
       if (settles(i)) issue(u + i * step, i);
     }
     PdlWait();
-    load_query(z, static_cast<int64_t>(group) * kVec + gid, group * kVec + gid < G);
+    load_query(z, group * kVec + gid, group * kVec + gid < G);
   }
 #pragma unroll
   for (int i = 0; i < Qu::kStages - 1; ++i) {
@@ -289,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   float factor;  // raw sums to scores in base 2 (without the key scale)
   {
     uint32_t amax = 0;
-    if (kRuns) load_query(first + my_row, v0 + gid, mine);
+    if (kRuns) load_query(first + my_row, static_cast<int>(place.Head(gid, my_down)), mine);
 #pragma unroll
     for (int j = 0; j < kKw; ++j) {
 #pragma unroll
@@ -316,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   bool ok = true;
   for (; u < units; u += step) {
     const int t0 = unit_of(u) * kUnit;
-    const float ks = ksp[unit_of(u) / per_block], vs = vsp[unit_of(u) / per_block];
+    const float ks = ksp[unit_of(u) >> unit_shift], vs = vsp[unit_of(u) >> unit_shift];
     // The stage behind the last one read is free: every lane has read it.
     __syncwarp();
     issue(u + (Qu::kStages - 1) * step, stage == 0 ? Qu::kStages - 1 : stage - 1);
@@ -466,9 +471,10 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
   __syncthreads();
   // Element e of the CTA's vectors, four at a time.
   const auto store = [&](int e, float sum, float4 acc) {
-    const int64_t v = v0 + e / D;
-    if (v < vectors) {
-      *reinterpret_cast<float4*>(a.out + (first + v / G) * a.out_ld + (g * G + v % G) * D + e % D) =
+    const int v = e / D;
+    if (v <= top_vec) {
+      const uint32_t down = kRuns ? place.Down(v) : 0, head = kRuns ? place.Head(v, down) : group * kVec + v;
+      *reinterpret_cast<float4*>(a.out + (first + row_lo + down) * a.out_ld + static_cast<int64_t>(g * G + head) * D + e % D) =
           make_float4(acc.x / sum, acc.y / sum, acc.z / sum, acc.w / sum);
     }
   };
@@ -697,6 +703,8 @@ AttnArgs ArgsOf(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, 
   a.row_seq = row_seq;
   a.row_pos = row_pos;
   a.heads = heads;
+  a.group = heads / cache->kv_heads;
+  a.block_shift = cache->block == 32 ? 5 : cache->block == 64 ? 6 : 7;
   a.window = window;
   a.sinks = sinks;
   a.scale = 1.f / sqrtf(static_cast<float>(cache->head_dim));

@@ -26,6 +26,8 @@ struct AttnArgs {
   const int32_t* row_pos;
   int32_t single_rows;     // how many of them
   int32_t heads;
+  int32_t group;        // heads per kv head
+  int32_t block_shift;  // tokens per scale block, as a power of two
   int32_t window;
   int32_t sinks;
   float scale;
@@ -61,6 +63,23 @@ __device__ __forceinline__ void SplitPair(float x, float y, uint32_t* hi, uint32
   *hi = *reinterpret_cast<const uint32_t*>(&h);
   *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
+
+// Rows and heads of query vectors v0, v0 + 1, ... (row x head, `group` heads a
+// row). 64-bit divisions cost a hundred instructions each, so there is one, and
+// none where v0 fits 32 bits.
+struct Vectors {
+  int64_t row0;
+  uint32_t head0, group;
+  __device__ __forceinline__ Vectors(int64_t v0, int32_t heads_per_row) : group(static_cast<uint32_t>(heads_per_row)) {
+    row0 = v0 <= 0xffffffffll ? static_cast<int64_t>(static_cast<uint32_t>(v0) / group) : v0 / group;
+    head0 = static_cast<uint32_t>(v0 - row0 * group);
+  }
+  // Row behind row0 of vector v0 + i.
+  __device__ __forceinline__ uint32_t Down(int i) const { return (head0 + static_cast<uint32_t>(i)) / group; }
+  __device__ __forceinline__ uint32_t Head(int i, uint32_t down) const {
+    return head0 + static_cast<uint32_t>(i) - down * group;
+  }
+};
 
 // First position that a window ending at pos covers.
 __device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }

@@ -119,10 +119,11 @@ struct Range {
   int pos_lo, pos_hi, near_lo, near_hi;
 };
 
-__device__ __forceinline__ Range RangeOf(int64_t v_lo, int64_t v_hi, int G, int pos0, int window) {
+// Vectors lo .. hi behind those that `v` begins with, whose first is at pos0.
+__device__ __forceinline__ Range RangeOf(const Vectors& v, int lo, int hi, int pos0, int window) {
   Range r;
-  r.pos_lo = pos0 + static_cast<int>(v_lo / G);
-  r.pos_hi = pos0 + static_cast<int>(v_hi / G);
+  r.pos_lo = pos0 + static_cast<int>(v.Down(lo));
+  r.pos_hi = pos0 + static_cast<int>(v.Down(hi));
   r.near_lo = NearOf(r.pos_lo, window);
   r.near_hi = NearOf(r.pos_hi, window);
   return r;
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   Bars& bars = *reinterpret_cast<Bars*>(smem + L::kBars);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kFull, tid >> 5, 0);
   const accel_b200_q8_cache& c = a.cache;
-  const int G = a.heads / c.kv_heads, g = blockIdx.y, b = blockIdx.z;
+  const int G = a.group, g = blockIdx.y, b = blockIdx.z;
   PdlWait();
   const Run run = RunOf(a.rows, b, c.context, blockIdx.x == 0 && g == 0 && tid == 0, a.status);
   const int64_t vectors = static_cast<int64_t>(run.count) * G;
@@ -247,19 +248,19 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   };
 
   // The tiles: those of the sinks before the windows, then the windows.
-  const int64_t row_of_v0 = v0 / G;
-  const uint32_t head_of_v0 = static_cast<uint32_t>(v0 - row_of_v0 * G);
-  const int64_t v_last = Min64(v0 + kVectors, vectors) - 1;
-  const Range all = RangeOf(v0, v_last, G, run.pos0, a.window);
+  const Vectors place(v0, G);
+  const int last = static_cast<int>(Min64(kVectors, vectors - v0)) - 1;
+  const int pos_of_v0 = run.pos0 + static_cast<int>(place.row0);
+  const Range all = RangeOf(place, 0, last, pos_of_v0, a.window);
   const int tile0 = all.near_lo / kTile;
   const int sink_tiles = static_cast<int>(Min64((static_cast<int64_t>(a.sinks) + kTile - 1) / kTile, tile0));
   const int n = sink_tiles + all.pos_hi / kTile - tile0 + 1;
   const auto token_of = [&](int j) { return (j < sink_tiles ? j : tile0 + (j - sink_tiles)) * kTile; };
-  const bool second = L::kHalves > 1 && v0 + kHalf < vectors;
+  const bool second = L::kHalves > 1 && kHalf <= last;
   // Half w's vectors, and whether they see any of tile j.
   const auto half_range = [&](int w) {
-    const int64_t lo = Min64(v0 + w * kHalf, v_last);
-    return RangeOf(lo, Min64(lo + kHalf - 1, v_last), G, run.pos0, a.window);
+    const int lo = min(w * kHalf, last);
+    return RangeOf(place, lo, min(lo + kHalf - 1, last), pos_of_v0, a.window);
   };
   const auto needed = [&](const Range& range, int w, int j) {
     return (w == 0 || second) && SeesSome(range, token_of(j), kTile, a.sinks);
@@ -279,12 +280,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     const int w = warp / (4 * kParts), part = (warp >> 2) % kParts;  // half, and which tokens and dimensions of it
     const int quad = warp & 3, r = quad * 32 + lane;                  // vector of the half: its TMEM lane
     const Range range = half_range(w);
-    const bool mine = v0 + w * kHalf + r < vectors;
-    // Row (from row_of_v0) and head of this lane's vector, for itself and, by
-    // shuffle, for lanes that move its row.
-    const uint32_t my_down = (head_of_v0 + w * kHalf + r) / static_cast<uint32_t>(G);
-    const uint32_t my_place = my_down << 16 | (head_of_v0 + w * kHalf + r - my_down * G);
-    const int my_pos = mine ? run.pos0 + static_cast<int>(row_of_v0 + my_down) : range.pos_hi;
+    const int my_vector = w * kHalf + r;
+    const bool mine = my_vector <= last;
+    // Row (behind the first vector's) and head of this lane's vector, for itself
+    // and, by shuffle, for lanes that move its row.
+    const uint32_t my_down = place.Down(my_vector);
+    const uint32_t my_place = my_down << 16 | place.Head(my_vector, my_down);
+    const int my_pos = mine ? pos_of_v0 + static_cast<int>(my_down) : range.pos_hi;
     const int my_near = NearOf(my_pos, a.window);
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     constexpr int kOwnChunks = kChunks / kParts, kDims = D / kParts;
@@ -292,6 +294,22 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     float* factors = reinterpret_cast<float*>(smem + L::kShared) + w * kHalf;
     float* tops = reinterpret_cast<float*>(smem + L::kShared) + (L::kHalves + w * kParts) * kHalf;
     const auto meet = [&](bool bad) { return MeetAny(2 + w * 4 + quad, kParts * 32, bad); };
+    const float* ksp = c.k_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
+    const float* vsp = c.v_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
+    // Scales of a tile's chunks, one per lane: keys' in lanes 0 .. 3, values' in
+    // 4 .. 7; of chunks that nobody sees 0 and -1. They load a tile ahead.
+    const auto next_needed = [&](int j) {
+      while (j < n && !needed(range, w, j)) ++j;
+      return j;
+    };
+    const auto load_scales = [&](int j) {
+      const int t = (j < n ? token_of(j) : 0) + (lane & 3) * kChunk;
+      const bool value = (lane & 4) != 0;
+      if (j >= n || lane >= 2 * kChunks || !SeesSome(range, t, kChunk, a.sinks)) return value ? -1.f : 0.f;
+      return (value ? vsp : ksp)[t >> a.block_shift];
+    };
+    int j = next_needed(0);
+    float scales = load_scales(j);
     // The queries as two fp16 parts of q * 2^e, their largest element at 2^13.
     // Four lanes load a vector, a warp 8 at a time.
     float factor = 0.f;
@@ -306,10 +324,10 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
 #pragma unroll
         for (int i = 0; i < kTogether; ++i) {
           const int row = (part * kBatches + b0 + i) * 8 + (lane >> 2);  // of the quad
-          const uint32_t place = __shfl_sync(kFull, my_place, row);
-          const float* q = a.q + (run.first + row_of_v0 + (place >> 16)) * a.q_ld +
-                           static_cast<int64_t>(g * G + (place & 0xffffu)) * D + (lane & 3) * 4;
-          const bool some = v0 + w * kHalf + quad * 32 + row < vectors;
+          const uint32_t at = __shfl_sync(kFull, my_place, row);
+          const float* q = a.q + (run.first + place.row0 + (at >> 16)) * a.q_ld +
+                           static_cast<int64_t>(g * G + (at & 0xffffu)) * D + (lane & 3) * 4;
+          const bool some = w * kHalf + quad * 32 + row <= last;
 #pragma unroll
           for (int k = 0; k < kLoads; ++k) {
             x[i][k] = some ? *reinterpret_cast<const float4*>(q + 16 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -369,8 +387,6 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     Pair o[kDims / 2];  // weighted values of dimensions 2 d and 2 d + 1 of this part
 #pragma unroll
     for (int d = 0; d < kDims / 2; ++d) o[d] = 0;
-    const float* ksp = c.k_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
-    const float* vsp = c.v_scale + b * c.scale_seq_stride + g * c.scale_head_stride;
     // registers += v_ref * the last tile's weighted values.
     const auto take_out = [&] {
       const Pair ref2 = MakePair(v_ref, v_ref);
@@ -468,20 +484,6 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     int taken = 0, outs = 0;  // tiles whose scores, and MMA groups whose values, were taken
     bool pending = false;     // weighted values of the last tile are still to be taken
     bool ok = true;
-    // Scales of a tile's chunks, one per lane: keys' in lanes 0 .. 3, values' in
-    // 4 .. 7; of chunks that nobody sees 0 and -1. They load a tile ahead.
-    const auto next_needed = [&](int j) {
-      while (j < n && !needed(range, w, j)) ++j;
-      return j;
-    };
-    const auto load_scales = [&](int j) {
-      const int t = (j < n ? token_of(j) : 0) + (lane & 3) * kChunk;
-      const bool value = (lane & 4) != 0;
-      if (j >= n || lane >= 2 * kChunks || !SeesSome(range, t, kChunk, a.sinks)) return value ? -1.f : 0.f;
-      return (value ? vsp : ksp)[t / c.block];
-    };
-    int j = next_needed(0);
-    float scales = load_scales(j);
     while (j < n && ok) {
       const int t0 = token_of(j), next = next_needed(j + 1);
       // Weights carry their chunk's value scale relative to the tile's largest,
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
 #pragma unroll 1
         for (int k = 0; k < kChunks && ok; ++k) {
           const bool seen = SeesSome(range, t0 + k * kChunk, kChunk, a.sinks);
-          v_ref = seen ? vsp[(t0 + k * kChunk) / c.block] : 0.f;
+          v_ref = seen ? vsp[(t0 + k * kChunk) >> a.block_shift] : 0.f;
           ok = __all_sync(kFull, wait(&bars.out[w], outs & 1));
           if (!ok) break;
           TcFenceAfterSync();
@@ -604,13 +606,13 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       }
       __syncwarp();
       constexpr int kRows = 32 / kPieces;  // rows that the warp's lanes cover
-      float* out = a.out + (run.first + row_of_v0) * a.out_ld + static_cast<int64_t>(g) * G * D + part * kDims;
+      float* out = a.out + (run.first + place.row0) * a.out_ld + static_cast<int64_t>(g) * G * D + part * kDims;
 #pragma unroll 8
       for (int i0 = 0; i0 < 32; i0 += kRows) {
         const int i = i0 + lane / kPieces, piece = lane % kPieces;
-        const uint32_t place = __shfl_sync(kFull, my_place, i);
-        if (v0 + w * kHalf + quad * 32 + i < vectors) {
-          *reinterpret_cast<float4*>(out + static_cast<int64_t>(place >> 16) * a.out_ld + (place & 0xffffu) * D + piece * 4) =
+        const uint32_t at = __shfl_sync(kFull, my_place, i);
+        if (w * kHalf + quad * 32 + i <= last) {
+          *reinterpret_cast<float4*>(out + static_cast<int64_t>(at >> 16) * a.out_ld + (at & 0xffffu) * D + piece * 4) =
               *reinterpret_cast<const float4*>(mine_rows + i * kRowBytes + ((piece ^ (i & 7)) << 4));
         }
       }

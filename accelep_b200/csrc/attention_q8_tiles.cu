@@ -219,25 +219,6 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     PdlTrigger();
     return;
   }
-  if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
-      MbarInit(&bars.raw_full[i], 1);
-      for (int s = 0; s < 2; ++s) {
-        MbarInit(&bars.full[i][s], kConverters);
-        MbarInit(&bars.empty[i][s], 1);
-      }
-      MbarInit(&bars.queries[i], 4 * L::kParts);
-      MbarInit(&bars.scores[i], 1);
-      MbarInit(&bars.weights[i], 4 * L::kParts);
-      MbarInit(&bars.out[i], 1);
-    }
-    MbarInit(&bars.drain, 1);
-    bars.failed = 0;
-    FenceBarrierInit();
-  }
-  // TMEM is taken behind the wait for the previous kernel, and the next kernel
-  // is let in behind that: neither can hold the columns the other waits for.
-  if (warp == L::kMmaWarp) TmemAlloc(&bars.tmem, L::kTmemCols);
   // Every role passes here once, the softmax with its queries' loads in flight.
   const auto set_up = [&] {
     TcFenceBeforeSync();
@@ -491,25 +472,21 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       // Where scales are so far apart that the smaller ones' weights would lose
       // bits, each chunk is summed on its own; and where the largest is 0 or below
       // 2^-128, whose reciprocal is infinite.
-      float ks[kChunks], lift[kChunks], v_now = 0.f;
-      bool apart = false;
+      const bool value = (lane & 4) != 0;
+      float v_now = value ? fmaxf(scales, 0.f) : 0.f;
+      v_now = fmaxf(v_now, __shfl_xor_sync(kFull, v_now, 1));
+      v_now = fmaxf(v_now, __shfl_xor_sync(kFull, v_now, 2));
+      const float up = value && scales != -1.f ? __log2f(scales * (1.f / v_now)) : 0.f;
+      const bool apart = (__ballot_sync(kFull, !(fabsf(up) <= kMostLift)) & 0xf0u) != 0;  // lanes 4 .. 7
+      const float mine_up = value ? (apart ? 0.f : up) : scales;
+      v_now = __shfl_sync(kFull, v_now, kChunks);
+      float ks[kChunks], lift[kChunks];
 #pragma unroll
       for (int k = 0; k < kChunks; ++k) {
-        ks[k] = __shfl_sync(kFull, scales, k);
-        lift[k] = __shfl_sync(kFull, scales, kChunks + k);
-        v_now = fmaxf(v_now, lift[k]);
+        ks[k] = __shfl_sync(kFull, mine_up, k);
+        lift[k] = __shfl_sync(kFull, mine_up, kChunks + k);
       }
       scales = load_scales(next);
-      const float v_inv = 1.f / v_now;
-#pragma unroll
-      for (int k = 0; k < kChunks; ++k) {
-        lift[k] = lift[k] == -1.f ? 0.f : __log2f(lift[k] * v_inv);
-        apart = apart || !(fabsf(lift[k]) <= kMostLift);
-      }
-      if (apart) {
-#pragma unroll
-        for (int k = 0; k < kChunks; ++k) lift[k] = 0.f;
-      }
       if (pending) {
         // The last tile's weighted values, while the tensor core sums this one's scores.
         ok = __all_sync(kFull, wait(&bars.out[w], outs & 1));
@@ -620,7 +597,6 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   } else if (warp < L::kMmaWarp) {
     // ---------------------------------------------------------- int8 -> fp16
     RegsDown<L::kLess>();
-    set_up();
     const int ct = tid - L::kSoftWarps * 32;
     const int plane_row = static_cast<int>((b * c.seq_stride + g * c.head_stride) / D);
     const auto fetch = [&](int plane, int j) {
@@ -628,10 +604,26 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       TmaLoad2D(smem + L::kRaw + plane * L::kRawBytes, plane == 0 ? &tk : &tv, 0, plane_row + token_of(j),
                 &bars.raw_full[plane]);
     };
+    // The first tiles come while the other roles set up.
     if (ct == 0) {
+      for (int i = 0; i < 2; ++i) {
+        MbarInit(&bars.raw_full[i], 1);
+        for (int s = 0; s < 2; ++s) {
+          MbarInit(&bars.full[i][s], kConverters);
+          MbarInit(&bars.empty[i][s], 1);
+        }
+        MbarInit(&bars.queries[i], 4 * L::kParts);
+        MbarInit(&bars.scores[i], 1);
+        MbarInit(&bars.weights[i], 4 * L::kParts);
+        MbarInit(&bars.out[i], 1);
+      }
+      MbarInit(&bars.drain, 1);
+      bars.failed = 0;
+      FenceBarrierInit();
       fetch(0, 0);
       fetch(1, 0);
     }
+    set_up();
     bool ok = true;
     int fetched[2] = {0, 0};  // tiles read of each plane; the next is in flight
     for (int j = 0; j < n && ok; ++j) {
@@ -680,6 +672,10 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   } else {
     // ------------------------------------------------------------------ MMA
     RegsDown<L::kLess>();
+    // TMEM is taken behind the wait for the previous kernel, and the next kernel
+    // is let in behind that: neither can hold the columns the other waits for.
+    // (The softmax's registers wait for this warpgroup's, so those went first.)
+    if (warp == L::kMmaWarp) TmemAlloc(&bars.tmem, L::kTmemCols);
     const uint32_t tmem = set_up();
     if (warp == L::kMmaWarp && ElectOne()) {
       constexpr uint32_t kQkDesc = InstrDescF16(kTile, false), kPvDesc = InstrDescF16(D, true);

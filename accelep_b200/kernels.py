@@ -403,11 +403,10 @@ def _i32(name, t, index, n):
     raise ValueError(f"{name} must be {n} contiguous int32 on cuda:{index}")
 
 
-def _counts(*numbers):
-    """Refuses what a C int would hold as another number."""
-    for n in numbers:
-        if not 0 <= n <= 0x7fffffff:
-            raise ValueError(f"{n} is not a count of 31 bits")
+def _counts(bits):
+    """Refuses numbers (or-ed together) that a C int would hold as others."""
+    if bits >> 31:
+        raise ValueError("rows, windows and sinks are counts of 31 bits")
 
 
 def _table(name, t, cache):
@@ -499,7 +498,7 @@ def _attention_io(q, cache, heads, out):
 def attention_decode_q8_workspace(cache, rows, heads, window=0, sinks=0):
     """A zeroed workspace for attention_decode_q8 calls of these sizes (None:
     none needed)."""
-    _counts(rows, window, sinks)
+    _counts(rows | window | sinks)
     need = load().accel_b200_attention_decode_q8_workspace(cache._ref, rows, heads, window, sinks)
     return torch.zeros(need, dtype=torch.uint8, device=cache.device) if need else None
 
@@ -514,7 +513,7 @@ def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=
     options (ATTN_CACHE_BEFORE_WAIT)."""
     index = cache.index
     rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
-    _counts(window, sinks)
+    _counts(window | sinks)
     if rows == 0:
         return out
     if workspace is None:
@@ -537,7 +536,7 @@ def attention_decode_q8(q, cache, row_pos, heads, row_seq=None, window=0, sinks=
 def attention_prefill_q8_workspace(cache, batch, max_rows, heads, window=0, sinks=0):
     """A zeroed workspace for attention_prefill_q8 calls of these sizes (None:
     none needed)."""
-    _counts(batch, max_rows, window, sinks)
+    _counts(batch | max_rows | window | sinks)
     need = load().accel_b200_attention_prefill_q8_workspace(cache._ref, batch, max_rows, heads, window, sinks)
     return torch.zeros(need, dtype=torch.uint8, device=cache.device) if need else None
 
@@ -549,7 +548,7 @@ def attention_prefill_q8(q, cache, first, count, pos0, heads, max_rows, window=0
     their keys and values. window and sinks as in attention_decode_q8."""
     index, batch = cache.index, first.numel()
     rows, q_ld, out, out_ld = _attention_io(q, cache, heads, out)
-    _counts(max_rows, window, sinks)
+    _counts(max_rows | window | sinks)
     if rows == 0 or batch == 0:
         return out
     if workspace is None:

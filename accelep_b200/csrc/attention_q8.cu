@@ -21,10 +21,11 @@
 // Units are dealt to all warps of the S CTAs of a vector group in turn. Each
 // unit's weighted values are summed on their own and added, times the unit's
 // value scale, to fp32 registers (the tensor core's running sum rounds towards
-// zero, which would drift over a long context). Measured at 4 sequences of 40001
-// to 65536 tokens, 8 kv heads of 128: 80 us, 5.4 TB/s. Before the split by lengths
-// it took 88 us, with loads to registers 128 and with per-lane cp.async 132: an SM
-// keeps too few of those in flight.
+// zero, which would drift over a long context). Bound by HBM on long sequences:
+// 4 of 40001 to 65536 tokens, 8 kv heads of 128, take 77 us, 5.6 TB/s with inputs
+// that no cache holds. Before the split by lengths it took 88 us, with loads to
+// registers 128 and with per-lane cp.async 132: an SM keeps too few of those in
+// flight. Short calls are a chain of latencies, so what needs no division has none.
 //
 // Online softmax in base 2 against a reference that moves only when a score
 // passes it by more than kSlack (a vote; no weight above 2^(kBias + kSlack)).
@@ -679,12 +680,12 @@ int CheckWorkspace(const Split& p, const void* workspace, size_t bytes, const st
 // Whether a prefill takes the 256-vector tiles of attention_q8_tiles.cu. Both
 // kernels' times go by the tokens that rows see: a tile CTA walks 128 of them
 // in about 2.4 us (3.0 at 128 dimensions), one wave of 148 CTAs after another;
-// the groups of 8 vectors here share the whole GPU at about 1500 (1200) of
+// the groups of 8 vectors here share the whole GPU at about 1700 (1100) of
 // their units of 32 tokens per us. Tiles are faster from 900 groups per wave.
-// (Measured with 3 kv heads of 64, 12 heads, 16000 tokens: 32 sequences of 21
-// rows 336 us in tiles and 234 here, of 42 rows 328 and 385; one sequence of
-// 170 rows 268 and 56. With 8 kv heads of 128, 32 heads: 32 sequences of 8 rows
-// 686 and 480, of 16 rows 717 and 785; 4 of 64 rows 421 and 524.)
+// (Measured behind 16000 tokens, with 3 kv heads of 64, 12 heads: 32 sequences of
+// 16 rows 311 us in tiles and 216 here, of 32 rows 304 and 357; one sequence of
+// 128 rows 209 and 52. With 8 kv heads of 128, 32 heads: 32 sequences of 8 rows
+// 695 and 450, of 16 rows 727 and 734; 4 of 64 rows 425 and 489.)
 constexpr int64_t kTileGroups = 900;
 bool TakesTiles(const accel_b200_q8_cache& c, int64_t batch, int64_t max_rows, int32_t heads) {
   const int64_t vectors = max_rows * (heads / c.kv_heads), runs = batch * c.kv_heads;

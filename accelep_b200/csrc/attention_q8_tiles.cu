@@ -24,16 +24,18 @@
 // next issues every MMA.
 //
 // Measured: 2 sequences of 2047 and fewer rows behind 14000 tokens, 32 heads over
-// 8 kv heads of 128, window 4096: 560 us, 427 TFLOP/s of scores and values (twice
+// 8 kv heads of 128, window 4096: 562 us, 425 TFLOP/s of scores and values (twice
 // that in fp16 products). A half's chain (weights 2600 cycles, its four products
 // 2800, maximum 900, read-out 500) and the other's overlap to 7000 cycles a tile,
 // of which the tensor core works 5600: an M = 128, N = 128, K = 16 product takes
 // 102 cycles with A in shared memory, 72 from TMEM. 32 sequences of 512 rows, 9
-// heads over 3 of 64: 76 us, by issue slots (55% of them used) and the first and
-// last steps of short walks. What brought it there, on the first of these: one
-// elected thread instead of lane 0 issuing (1617 -> 1250 us), values freed in
-// front of the next scores and four converter warps (-> 806), chunk loops kept
-// rolled so that their code stays in the instruction cache (-> 632).
+// heads over 3 of 64: 69 us, by issue slots (55% of them used) and the first and
+// last steps of short walks (13000 of a four-tile CTA's 39000 cycles). What brought
+// it there, on the first of these: one elected thread instead of lane 0 issuing
+// (1617 -> 1250 us), values freed in front of the next scores and four converter
+// warps (-> 806), chunk loops kept rolled so that their code stays in the
+// instruction cache (-> 632); on the second: one half per CTA (80 -> 76), no 64-bit
+// divisions in any role and the first loads ahead of the set-up (-> 69).
 //
 // Every wait is bounded; one that runs out sets a flag that ends every role,
 // gives NaN and ORs ACCEL_B200_STATUS_COPY_TIMEOUT.

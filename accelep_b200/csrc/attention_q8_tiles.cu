@@ -124,7 +124,7 @@ struct Range {
 // Vectors lo .. hi behind those that `v` begins with, whose first is at pos0.
 __device__ __forceinline__ Range RangeOf(const Vectors& v, int lo, int hi, int pos0, int window) {
   Range r;
-  r.pos_lo = pos0 + static_cast<int>(v.Down(lo));
+  r.pos_lo = lo == 0 ? pos0 : pos0 + static_cast<int>(v.Down(lo));
   r.pos_hi = pos0 + static_cast<int>(v.Down(hi));
   r.near_lo = NearOf(r.pos_lo, window);
   r.near_hi = NearOf(r.pos_hi, window);
@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   const bool second = L::kHalves > 1 && kHalf <= last;
   // Half w's vectors, and whether they see any of tile j.
   const auto half_range = [&](int w) {
+    if (L::kHalves == 1) return all;
     const int lo = min(w * kHalf, last);
     return RangeOf(place, lo, min(lo + kHalf - 1, last), pos_of_v0, a.window);
   };

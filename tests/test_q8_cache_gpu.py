@@ -596,6 +596,19 @@ def test_offsets_past_32_bits(lib, cuda):
     assert H(status)[0] == 0
 
 
+def test_prefill_of_more_tiles_than_a_grid_is_high(lib, cuda):
+    """8.4 million query vectors of one kv head (65600 tiles of 128). Each row sees
+    itself only, so its output is its value: one weight, divided by itself."""
+    rows, heads, d = 32800, 256, 64
+    c = filled(np.random.default_rng(5), 1, 1, rows, d, 64)
+    x = torch.rand(rows, heads * d, device="cuda")
+    K.attention_prefill_q8(x, device_cache(c), I([0]), I([rows]), I([0]), heads, rows, window=1, out=x)
+    want = T(c.value("v", 0, 0, np.arange(rows)).astype(np.float32))
+    for r in range(0, rows, 4100):
+        off = (x[r:r + 4100].view(-1, heads, d) - want[r:r + 4100, None]).abs()
+        assert (off <= 2.0 ** -20 * want[r:r + 4100, None].abs()).all(), r
+
+
 def test_run_together_on_a_stream_and_replayed(lib, cuda):
     """A prompt and then single tokens, as a serving loop runs them: the step
     captured once on a side stream and replayed with new rows and positions."""

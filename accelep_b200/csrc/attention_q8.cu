@@ -641,12 +641,15 @@ Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run,
   return p;
 }
 
+// Arrivals, then the CTAs' states.
+void SetWorkspace(AttnArgs* a, void* workspace) {
+  a->counters = static_cast<int32_t*>(workspace);
+  a->parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterRegion);
+}
+
 template <int D, Rows kRows>
 int LaunchVectors(AttnArgs a, const Split& p, int64_t runs, void* workspace, cudaStream_t stream, const char* what) {
-  if (p.workspace > 0) {
-    a.counters = static_cast<int32_t*>(workspace);
-    a.parts = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterRegion);
-  }
+  if (p.workspace > 0) SetWorkspace(&a, workspace);
   a.single_rows = static_cast<int32_t>(runs);
   const dim3 grid = kRows == Rows::kBalanced
                         ? dim3(static_cast<unsigned>(p.balanced))
@@ -668,9 +671,9 @@ int LaunchVectors(AttnArgs a, const Split& p, int64_t runs, void* workspace, cud
       LaunchK(AttnVectorsQ8Kernel<D, kRows>, grid, dim3(kThreads), kSmem, stream, cluster, 1u, tk, tv, a), what);
 }
 
-int CheckWorkspace(const Split& p, const void* workspace, size_t bytes, const std::string& what) {
-  if (p.workspace == 0) return ACCEL_B200_OK;
-  if (workspace == nullptr || bytes < p.workspace) return SetError(ACCEL_B200_EINVAL, what + ": workspace too small");
+int CheckWorkspace(size_t need, const void* workspace, size_t bytes, const std::string& what) {
+  if (need == 0) return ACCEL_B200_OK;
+  if (workspace == nullptr || bytes < need) return SetError(ACCEL_B200_EINVAL, what + ": workspace too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
     return SetError(ACCEL_B200_EINVAL, what + ": the workspace must be 16-byte aligned");
   }
@@ -772,7 +775,7 @@ ACCEL_B200_API int accel_b200_attention_decode_q8_prefetch(const float* q, int64
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
     return SetError(ACCEL_B200_EINVAL, "attention_decode_q8: grid too large");
   }
-  rc = CheckWorkspace(p, workspace, workspace_bytes, "attention_decode_q8");
+  rc = CheckWorkspace(p.workspace, workspace, workspace_bytes, "attention_decode_q8");
   if (rc != ACCEL_B200_OK) return rc;
   AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{}, row_seq, row_pos, heads, window, sinks, out, out_ld, status);
   if (prefetch != nullptr) a.prefetch = *prefetch;
@@ -803,7 +806,7 @@ ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200
     return 0;
   }
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));
-  if (TakesTiles(*cache, batch, max_rows, heads)) return 0;
+  if (TakesTiles(*cache, batch, max_rows, heads)) return TilesWorkspaceQ8(*cache, batch, max_rows, heads, window, sinks);
   return SplitFor(*cache, batch, max_rows, heads, window, sinks, false).workspace;
 }
 
@@ -822,14 +825,21 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
   if (rows == 0 || batch == 0 || max_rows == 0) return ClearError();
   if (batch > 65535) return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: more than 65535 sequences");
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));  // a longer run does not fit
-  const AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads,
-                            window, sinks, out, out_ld, status);
-  if (TakesTiles(*cache, batch, max_rows, heads)) return LaunchTilesQ8(a, batch, max_rows, AsStream(stream));
+  AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads, window,
+                      sinks, out, out_ld, status);
+  a.sequences = batch;
+  if (TakesTiles(*cache, batch, max_rows, heads)) {
+    const size_t need = TilesWorkspaceQ8(*cache, batch, max_rows, heads, window, sinks);
+    rc = CheckWorkspace(need, workspace, workspace_bytes, "attention_prefill_q8");
+    if (rc != ACCEL_B200_OK) return rc;
+    if (need > 0) SetWorkspace(&a, workspace);
+    return LaunchTilesQ8(a, max_rows, AsStream(stream));
+  }
   const Split p = SplitFor(*cache, batch, max_rows, heads, window, sinks, false);
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: grid too large");
   }
-  rc = CheckWorkspace(p, workspace, workspace_bytes, "attention_prefill_q8");
+  rc = CheckWorkspace(p.workspace, workspace, workspace_bytes, "attention_prefill_q8");
   if (rc != ACCEL_B200_OK) return rc;
   const char* what = "attention_prefill_q8";
   cudaStream_t st = AsStream(stream);

@@ -25,6 +25,7 @@ struct AttnArgs {
   const int32_t* row_seq;  // single rows: slot (null: the row's number) and position
   const int32_t* row_pos;
   int32_t single_rows;     // how many of them
+  int32_t sequences;       // prefill: sequences of `rows`
   int32_t heads;
   int32_t group;        // heads per kv head
   int32_t block_shift;  // tokens per scale block, as a power of two
@@ -85,8 +86,10 @@ struct Vectors {
 __device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
 // Prefill attention on the tcgen05 tensor cores, kTileVectors query vectors per
-// CTA (attention_q8_tiles.cu).
+// SM (attention_q8_tiles.cu), and the bytes of workspace that it takes.
 constexpr int kTileVectors = 256;
-int LaunchTilesQ8(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stream);
+size_t TilesWorkspaceQ8(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
+                        int32_t sinks);
+int LaunchTilesQ8(const AttnArgs& a, int32_t max_rows, cudaStream_t stream);
 
 }  // namespace accel_b200

@@ -24,7 +24,7 @@
 // next issues every MMA.
 //
 // Measured: 2 sequences of 2047 and fewer rows behind 14000 tokens, 32 heads over
-// 8 kv heads of 128, window 4096: 562 us, 425 TFLOP/s of scores and values (twice
+// 8 kv heads of 128, window 4096: 489 us, 489 TFLOP/s of scores and values (twice
 // that in fp16 products). A half's chain (weights 2600 cycles, its four products
 // 2800, maximum 900, read-out 500) and the other's overlap to 7000 cycles a tile,
 // of which the tensor core works 5600: an M = 128, N = 128, K = 16 product takes
@@ -61,6 +61,9 @@ constexpr int kTile = 128;         // tokens per tile
 constexpr int kConverters = 4;     // warps
 constexpr int kChunk = 32;         // tokens whose scores a thread holds at a time: one scale block at most
 constexpr int kChunks = kTile / kChunk;
+constexpr int kMostShares = 8;      // CTAs that a walk is split over at most
+constexpr int kLeastShare = 4;      // tiles that each of them gets at least (it costs about two to begin and end)
+constexpr int64_t kSplitFrom = 4096;  // tokens from which walks are split
 constexpr float kMostLift = 6.f;    // scales of a tile further apart than 2^6 are applied one by one
 constexpr int kPanel = 128 * 128;  // bytes of 128 rows x 64 fp16, the swizzle's row length
 
@@ -96,6 +99,8 @@ struct Tiles {
   static constexpr int kBytes = kShared + (kParts > 1 ? (1 + 2 * kParts) * kHalves * 128 * 4 : 0);
   static constexpr int kAlign = 1024;
   static_assert((kBytes + kAlign + 1024) * kCtas <= 228 * 1024, "shared memory of an SM");
+  static constexpr int kSlots = kSms * kCtas;                          // CTAs of a wave
+  static constexpr int kStateFloats = kHalves * kHalf * (D + 2);       // a split walk's: sums, references, weights
   // TMEM columns: scores (then weights) and weighted values of the halves.
   static constexpr uint32_t kScores = 0, kOut = kHalves * kTile, kTmemCols = 512 / kCtas;
   static_assert(kOut + kHalves * D <= kTmemCols, "TMEM of an SM");
@@ -204,7 +209,14 @@ __device__ __forceinline__ bool MeetAny(int id, int threads, bool any) {
 // (70 -> 62 us at 32 x 512 rows, against sequence after sequence). Tiles past the
 // grid's 65535 go with x.
 constexpr int64_t kGridTiles = 65535;
-template <int D>
+//
+// kSplit: a flat grid over the tiles of at most 32 sequences. Those that fill whole
+// waves of the SMs go a CTA each; the walks of the rest are dealt to several CTAs,
+// so that the last wave is as short as it has room to be, and the last CTA of a
+// tile to arrive merges their states in order. (480 tiles, 3.2 waves, of walks of
+// 33: 559 -> 489 us. In front of every CTA's first step it is 2000 cycles of counting,
+// so calls of short walks go without.)
+template <int D, bool kSplit>
 __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     AttnTilesQ8Kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const AttnArgs a) {
   using L = Tiles<D>;
@@ -213,17 +225,50 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   Bars& bars = *reinterpret_cast<Bars*>(smem + L::kBars);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(kFull, tid >> 5, 0);
   const accel_b200_q8_cache& c = a.cache;
-  const int G = a.group, b = blockIdx.y;
-  int g = blockIdx.x;
-  int64_t from_end = blockIdx.z;
-  if (gridDim.x > c.kv_heads) {
-    from_end += g / c.kv_heads * kGridTiles;
-    g %= c.kv_heads;
-  }
-  PdlWait();
-  const Run run = RunOf(a.rows, b, c.context, blockIdx.x == 0 && blockIdx.z == 0 && tid == 0, a.status);
-  const int64_t vectors = static_cast<int64_t>(run.count) * G;
+  const int G = a.group;
   constexpr int kVectors = L::kHalves * kHalf;
+  int g = blockIdx.x, b = blockIdx.y;
+  int64_t from_end = blockIdx.z;
+  int share = 0, shares = 1;  // this CTA's part of the tile's walk
+  int split_tile = 0, state0 = 0;  // the tile's counter and first state
+  PdlWait();
+  Run run;
+  if constexpr (kSplit) {
+    // Lane r counts the tiles of sequence r.
+    run = lane < a.sequences ? RunOf(a.rows, lane, c.context, blockIdx.x == 0 && warp == 0, a.status) : Run{0, 0, 0};
+    const int own = static_cast<int>((static_cast<int64_t>(run.count) * G + kVectors - 1) / kVectors) * c.kv_heads;
+    int end = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int before = __shfl_up_sync(kFull, end, o);
+      if (lane >= o) end += before;
+    }
+    const int items = __shfl_sync(kFull, end, 31), whole = items / L::kSlots * L::kSlots;
+    int item = blockIdx.x;
+    if (item >= whole && items > whole) {
+      shares = min(kMostShares, L::kSlots / (items - whole));
+      split_tile = (item - whole) / shares;
+      share = item - whole - split_tile * shares;
+      state0 = split_tile * shares;
+      item = whole + split_tile;
+    }
+    if (item >= items) {
+      PdlTrigger();
+      return;
+    }
+    b = __ffs(__ballot_sync(kFull, end > item)) - 1;
+    item -= __shfl_sync(kFull, end - own, b);
+    from_end = item / c.kv_heads;
+    g = item % c.kv_heads;
+    run = Run{__shfl_sync(kFull, run.first, b), __shfl_sync(kFull, run.count, b), __shfl_sync(kFull, run.pos0, b)};
+  } else {
+    if (gridDim.x > c.kv_heads) {
+      from_end += g / c.kv_heads * kGridTiles;
+      g %= c.kv_heads;
+    }
+    run = RunOf(a.rows, b, c.context, blockIdx.x == 0 && blockIdx.z == 0 && tid == 0, a.status);
+  }
+  const int64_t vectors = static_cast<int64_t>(run.count) * G;
   const int64_t tiles = (vectors + kVectors - 1) / kVectors;
   const int64_t v0 = (tiles - 1 - from_end) * kVectors;
   if (v0 < 0) {
@@ -246,8 +291,20 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   const Range all = RangeOf(place, 0, last, pos_of_v0, a.window);
   const int tile0 = all.near_lo / kTile;
   const int sink_tiles = static_cast<int>(Min64((static_cast<int64_t>(a.sinks) + kTile - 1) / kTile, tile0));
-  const int n = sink_tiles + all.pos_hi / kTile - tile0 + 1;
-  const auto token_of = [&](int j) { return (j < sink_tiles ? j : tile0 + (j - sink_tiles)) * kTile; };
+  int n = sink_tiles + all.pos_hi / kTile - tile0 + 1, j0 = 0;
+  if (kSplit && shares > 1) {
+    shares = min(shares, max(1, n / kLeastShare));  // the same for all CTAs of the tile
+    if (share >= shares) {
+      PdlTrigger();
+      return;
+    }
+    j0 = n * share / shares;
+    n = n * (share + 1) / shares - j0;
+  }
+  const auto token_of = [&](int j) {
+    j += j0;
+    return (j < sink_tiles ? j : tile0 + (j - sink_tiles)) * kTile;
+  };
   const bool second = L::kHalves > 1 && kHalf <= last;
   // Half w's vectors, and whether they see any of tile j.
   const auto half_range = [&](int w) {
@@ -586,7 +643,9 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       constexpr int kRowBytes = kDims * 4, kPieces = kRowBytes / 16;
       static_assert(32 * kRowBytes * 4 * kParts == 2 * L::kOperand, "");
       char* mine_rows = smem + L::kQ + w * 2 * L::kOperand + (part * 4 + quad) * 32 * kRowBytes;
-      const Pair inv2 = MakePair(1.f / l, 1.f / l);
+      const bool partial = kSplit && shares > 1;
+      const float inv = partial ? 1.f : 1.f / l;
+      const Pair inv2 = MakePair(inv, inv);
 #pragma unroll
       for (int k = 0; k < kPieces; ++k) {
         const float2 x = Split2(Mul2(o[2 * k], inv2)), y = Split2(Mul2(o[2 * k + 1], inv2));
@@ -596,13 +655,66 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       __syncwarp();
       constexpr int kRows = 32 / kPieces;  // rows that the warp's lanes cover
       float* out = a.out + (run.first + place.row0) * a.out_ld + static_cast<int64_t>(g) * G * D + part * kDims;
+      float* state = a.parts + static_cast<int64_t>(state0 + share) * L::kStateFloats;
 #pragma unroll 8
       for (int i0 = 0; i0 < 32; i0 += kRows) {
         const int i = i0 + lane / kPieces, piece = lane % kPieces;
         const uint32_t at = __shfl_sync(kFull, my_place, i);
         if (w * kHalf + quad * 32 + i <= last) {
-          *reinterpret_cast<float4*>(out + static_cast<int64_t>(at >> 16) * a.out_ld + (at & 0xffffu) * D + piece * 4) =
+          float* to = partial ? state + (w * kHalf + quad * 32 + i) * D + part * kDims
+                              : out + static_cast<int64_t>(at >> 16) * a.out_ld + (at & 0xffffu) * D;
+          *reinterpret_cast<float4*>(to + piece * 4) =
               *reinterpret_cast<const float4*>(mine_rows + i * kRowBytes + ((piece ^ (i & 7)) << 4));
+        }
+      }
+      if (partial) {
+        if (part == 0) {
+          state[kVectors * D + my_vector] = m;
+          state[kVectors * (D + 1) + my_vector] = l;
+        }
+        constexpr int kThreads = L::kSoftWarps * 32, kMergeBarrier = 10;
+        MeetAny(kMergeBarrier, kThreads, false);
+        bool merges = false;
+        if (tid == 0) {
+          __threadfence();  // the barrier put the CTA's stores before it
+          merges = atomicAdd(a.counters + split_tile, 1) == shares - 1;
+          if (merges) a.counters[split_tile] = 0;
+          __threadfence();
+        }
+        if (MeetAny(kMergeBarrier, kThreads, merges)) {
+          const float* states = a.parts + static_cast<int64_t>(state0) * L::kStateFloats;
+          for (int e = tid; e < (last + 1) * (D / 4); e += kThreads) {
+            const int v = e / (D / 4), d = e % (D / 4) * 4;
+            float pm[kMostShares], pl[kMostShares], mx = -INFINITY, sum = 0.f;
+            float4 po[kMostShares], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int p = 0; p < kMostShares; ++p) {
+              if (p < shares) {
+                const float* s = states + static_cast<int64_t>(p) * L::kStateFloats;
+                pm[p] = __ldcg(s + kVectors * D + v);
+                pl[p] = __ldcg(s + kVectors * (D + 1) + v);
+                po[p] = __ldcg(reinterpret_cast<const float4*>(s + v * D + d));
+                mx = fmaxf(mx, pm[p]);
+              }
+            }
+#pragma unroll
+            for (int p = 0; p < kMostShares; ++p) {
+              if (p < shares) {
+                // A share that saw nothing of a vector has reference -inf and sums of
+                // 0; one of NaN scores has that reference too, and sums that stay.
+                const float f = pm[p] == -INFINITY ? 1.f : Exp2(pm[p] - mx);
+                sum = fmaf(pl[p], f, sum);
+                acc.x = fmaf(po[p].x, f, acc.x);
+                acc.y = fmaf(po[p].y, f, acc.y);
+                acc.z = fmaf(po[p].z, f, acc.z);
+                acc.w = fmaf(po[p].w, f, acc.w);
+              }
+            }
+            const uint32_t down = place.Down(v), head = place.Head(v, down);
+            *reinterpret_cast<float4*>(a.out + (run.first + place.row0 + down) * a.out_ld +
+                                       static_cast<int64_t>(g * G + head) * D + d) =
+                make_float4(acc.x / sum, acc.y / sum, acc.z / sum, acc.w / sum);
+          }
         }
       }
     }
@@ -781,18 +893,34 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   if (warp == L::kMmaWarp) TmemDealloc(bars.tmem, L::kTmemCols);
 }
 
+// Tiles that a call has at most, by its largest number of rows.
 template <int D>
-int Launch(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stream) {
+int64_t MostTiles(const accel_b200_q8_cache& c, int64_t max_rows, int32_t heads) {
+  return CeilDiv(max_rows * (heads / c.kv_heads), Tiles<D>::kHalves * kHalf);
+}
+
+// Whether the last wave's walks are split: few waves, of walks that can be long.
+template <int D>
+bool Splits(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window, int32_t sinks) {
+  const int64_t seen = window > 0 ? Min64(c.context, static_cast<int64_t>(window) + sinks) : c.context;
+  return batch <= 32 && seen >= kSplitFrom &&
+         batch * c.kv_heads * MostTiles<D>(c, max_rows, heads) <= 16 * Tiles<D>::kSlots;
+}
+
+template <int D, bool kSplit>
+int Launch(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
   constexpr int kSmem = Tiles<D>::kBytes + Tiles<D>::kAlign;
   // The roles trade the registers that the launch gives out; were they fewer
   // than the split adds up to, the role that takes more would wait for good.
   static const int regs = [] {
     cudaFuncAttributes f{};
-    return cudaFuncGetAttributes(&f, AttnTilesQ8Kernel<D>) == cudaSuccess ? f.numRegs : 0;
+    return cudaFuncGetAttributes(&f, AttnTilesQ8Kernel<D, kSplit>) == cudaSuccess ? f.numRegs : 0;
   }();
-  if (regs != Tiles<D>::kLaunch) return SetError(ACCEL_B200_ECUDA, "attention_prefill_q8: the kernel's registers do not fit its split");
+  if (regs != Tiles<D>::kLaunch) {
+    return SetError(ACCEL_B200_ECUDA, "attention_prefill_q8: the kernel's registers do not fit its split");
+  }
   const cudaError_t err =
-      cudaFuncSetAttribute(AttnTilesQ8Kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+      cudaFuncSetAttribute(AttnTilesQ8Kernel<D, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (err != cudaSuccess) return CheckLaunchEx(err, "attention_prefill_q8");
   const uint64_t plane_rows = static_cast<uint64_t>(PlaneRows(a.cache));
   CUtensorMap tk{}, tv{};
@@ -800,18 +928,39 @@ int Launch(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stre
       !Encode2D(&tv, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.cache.v, D, plane_rows, D, D, kTile, CU_TENSOR_MAP_SWIZZLE_NONE)) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: cache tensor map rejected");
   }
-  const int64_t vectors = static_cast<int64_t>(max_rows) * (a.heads / a.cache.kv_heads);
-  const int64_t tiles = CeilDiv(vectors, Tiles<D>::kHalves * kHalf);
-  const dim3 grid(static_cast<unsigned>(CeilDiv(tiles, kGridTiles) * a.cache.kv_heads), static_cast<unsigned>(batch),
-                  static_cast<unsigned>(Min64(tiles, kGridTiles)));
-  return CheckLaunchEx(LaunchK(AttnTilesQ8Kernel<D>, grid, dim3(Tiles<D>::kThreads), kSmem, stream, 1u, 1u, tk, tv, a),
-                       "attention_prefill_q8");
+  const int64_t tiles = MostTiles<D>(a.cache, max_rows, a.heads), kv = a.cache.kv_heads;
+  const dim3 grid = kSplit ? dim3(static_cast<unsigned>(a.sequences * kv * tiles + Tiles<D>::kSlots))
+                           : dim3(static_cast<unsigned>(CeilDiv(tiles, kGridTiles) * kv),
+                                  static_cast<unsigned>(a.sequences), static_cast<unsigned>(Min64(tiles, kGridTiles)));
+  return CheckLaunchEx(
+      LaunchK(AttnTilesQ8Kernel<D, kSplit>, grid, dim3(Tiles<D>::kThreads), kSmem, stream, 1u, 1u, tk, tv, a),
+      "attention_prefill_q8");
+}
+
+template <int D>
+int LaunchFor(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
+  return Splits<D>(a.cache, a.sequences, max_rows, a.heads, a.window, a.sinks) ? Launch<D, true>(a, max_rows, stream)
+                                                                               : Launch<D, false>(a, max_rows, stream);
+}
+
+template <int D>
+size_t WorkspaceFor(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
+                    int32_t sinks) {
+  if (!Splits<D>(c, batch, max_rows, heads, window, sinks)) return 0;
+  static_assert(Tiles<D>::kSlots <= kMaxCounters, "a counter per split tile");
+  return kCounterRegion + static_cast<size_t>(Tiles<D>::kSlots) * Tiles<D>::kStateFloats * sizeof(float);
 }
 
 }  // namespace
 
-int LaunchTilesQ8(const AttnArgs& a, int32_t batch, int32_t max_rows, cudaStream_t stream) {
-  return a.cache.head_dim == 64 ? Launch<64>(a, batch, max_rows, stream) : Launch<128>(a, batch, max_rows, stream);
+size_t TilesWorkspaceQ8(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
+                        int32_t sinks) {
+  return c.head_dim == 64 ? WorkspaceFor<64>(c, batch, max_rows, heads, window, sinks)
+                          : WorkspaceFor<128>(c, batch, max_rows, heads, window, sinks);
+}
+
+int LaunchTilesQ8(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
+  return a.cache.head_dim == 64 ? LaunchFor<64>(a, max_rows, stream) : LaunchFor<128>(a, max_rows, stream);
 }
 
 }  // namespace accel_b200

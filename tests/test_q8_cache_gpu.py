@@ -394,6 +394,72 @@ def test_prefill_few_rows_of_a_long_sequence(lib, cuda, count, pos0, heads, kv, 
     check_rows(c, q, got, todo, heads, window, 3)
 
 
+SPLITS = [
+    # Walks of tiles that several CTAs share: fewer tiles than SMs, tiles in front of
+    # whole waves, walks too short to share among others, sequences without rows.
+    (32, 8, 128, 9000, [8500], [300], 0, 0),
+    (9, 3, 64, 8000, [5000, 0, 7001], [700, 1, 333], 0, 0),
+    (16, 8, 128, 14000, [0, 12001], [0, 400], 4500, 5),
+    (6, 1, 64, 30000, [29000, -1, 20000, 100], [1000, 5, 2, 777], 0, 0),
+    (32, 8, 128, 6000, [4700, 300], [1200, 1200], 0, 0),
+    (12, 4, 64, 5000, [0, 900], [4999, 4100], 4100, 200),
+]
+
+
+@pytest.mark.parametrize("heads,kv,d,context,pos0,count,window,sinks", SPLITS)
+def test_prefill_walks_shared_by_ctas(lib, cuda, heads, kv, d, context, pos0, count, window, sinks):
+    rng = np.random.default_rng(heads + d + context)
+    c = filled(rng, len(count), kv, context, d, 64)
+    c.s["v"][0, 0, 3::7] = 2.0 ** -14  # tiles of far-apart scales
+    dev = device_cache(c)
+    first, rows = ragged(count) + 1, int(np.sum(count)) + 2
+    x = T(rng.standard_normal((rows, heads * d), dtype=np.float32))
+    x[first[-1] + count[-1] // 2] *= 30
+    q, most = H(x).copy(), 1500 if sum(count) < 1500 else max(count)
+    run = (dev, I(first.tolist()), I(count), I(pos0), heads, most, window, sinks)
+    ws = K.attention_prefill_q8_workspace(dev, len(count), most, heads, window, sinks)
+    assert ws is not None
+    status = I([0])
+    got = H(K.attention_prefill_q8(x, *run, workspace=ws, status=status))
+    live = [b for b in range(len(count)) if count[b] > 0 and pos0[b] >= 0]
+    check = [(int(first[b]) + i, b, pos0[b] + i) for b in live
+             for i in sorted({0, count[b] // 3, count[b] // 2, count[b] - 1})]
+    check_rows(c, q, got, check, heads, window, sinks)
+    left = np.ones(rows, bool)
+    for b in live:
+        left[first[b]:first[b] + count[b]] = False
+    assert (got[left] == 0).all()
+    # The same bits again, in place too, and the counters as they were.
+    np.testing.assert_array_equal(H(K.attention_prefill_q8(x, *run, workspace=ws)), got)
+    assert (H(ws)[:65536] == 0).all() and H(status)[0] == 0
+    K.attention_prefill_q8(x, *run, workspace=ws, out=x)
+    np.testing.assert_array_equal(H(x)[~left], got[~left])
+    with pytest.raises(B200Error):
+        K.attention_prefill_q8(T(q), *run, workspace=ws[:-16])
+
+
+def test_prefill_walks_shared_by_ctas_skip_and_ignore(lib, cuda):
+    """Sequences that do not fit are skipped with a status; what no row sees may
+    be anything; NaN queries stay in their head."""
+    rng = np.random.default_rng(8)
+    heads, kv, d, context = 16, 4, 128, 9000
+    c = filled(rng, 3, kv, context, d, 64)
+    clean = [(1, 1, 6000), (200, 1, 6199), (420, 1, 6419)]
+    for name in "kv":
+        c.s[name][1, :, 6464 // 64:] = np.nan
+        c.s[name][1, :, :1900 // 64] = np.inf
+    q = rng.standard_normal((900, heads * d), dtype=np.float32)
+    q[300, 5 * d + 7] = np.nan
+    status = I([0])
+    got = H(K.attention_prefill_q8(T(q), device_cache(c), I([0, 1, 500]), I([2, 464, 10]), I([8999, 6000, 0]), heads, 464,
+                                   4096, 0, status=status))
+    assert H(status)[0] == BAD_POSITION and (got[0] == 0).all()
+    check_rows(c, q, got, clean, heads, 4096, 0)
+    check_rows(c, q, got, [(500, 2, 0), (509, 2, 9)], heads, 4096, 0)
+    bad = np.isnan(got[1:465]).reshape(464, heads, d)
+    assert bad[299, 5].all() and bad.sum() == d
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 3e38])
 def test_what_a_row_does_not_see_does_not_matter(lib, cuda, bad):
     """Scales of blocks that hold nothing a row sees (behind it, or before its

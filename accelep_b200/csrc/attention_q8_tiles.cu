@@ -63,7 +63,6 @@ constexpr int kChunk = 32;         // tokens whose scores a thread holds at a ti
 constexpr int kChunks = kTile / kChunk;
 constexpr int kMostShares = 8;      // CTAs that a walk is split over at most
 constexpr int kLeastShare = 4;      // tiles that each of them gets at least (it costs about two to begin and end)
-constexpr int64_t kSplitFrom = 4096;  // tokens from which walks are split
 constexpr float kMostLift = 6.f;    // scales of a tile further apart than 2^6 are applied one by one
 constexpr int kPanel = 128 * 128;  // bytes of 128 rows x 64 fp16, the swizzle's row length
 
@@ -210,12 +209,12 @@ __device__ __forceinline__ bool MeetAny(int id, int threads, bool any) {
 // grid's 65535 go with x.
 constexpr int64_t kGridTiles = 65535;
 //
-// kSplit: a flat grid over the tiles of at most 32 sequences. Those that fill whole
+// kSplit: a flat grid over the tiles of at most 32 sequences, in the same order (the
+// counting costs nothing that was measured). Those that fill whole
 // waves of the SMs go a CTA each; the walks of the rest are dealt to several CTAs,
 // so that the last wave is as short as it has room to be, and the last CTA of a
 // tile to arrive merges their states in order. (480 tiles, 3.2 waves, of walks of
-// 33: 559 -> 489 us. In front of every CTA's first step it is 2000 cycles of counting,
-// so calls of short walks go without.)
+// 33: 559 -> 488 us.)
 template <int D, bool kSplit>
 __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     AttnTilesQ8Kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const AttnArgs a) {
@@ -234,16 +233,11 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   PdlWait();
   Run run;
   if constexpr (kSplit) {
-    // Lane r counts the tiles of sequence r.
+    // Lane r counts the tiles of sequence r. In front of level d (the tiles that
+    // are d-th from the end of their sequences) are min(tiles, d) of each.
     run = lane < a.sequences ? RunOf(a.rows, lane, c.context, blockIdx.x == 0 && warp == 0, a.status) : Run{0, 0, 0};
-    const int own = static_cast<int>((static_cast<int64_t>(run.count) * G + kVectors - 1) / kVectors) * c.kv_heads;
-    int end = own;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int before = __shfl_up_sync(kFull, end, o);
-      if (lane >= o) end += before;
-    }
-    const int items = __shfl_sync(kFull, end, 31), whole = items / L::kSlots * L::kSlots;
+    const int own = static_cast<int>((static_cast<int64_t>(run.count) * G + kVectors - 1) / kVectors);
+    const int items = __reduce_add_sync(kFull, own) * c.kv_heads, whole = items / L::kSlots * L::kSlots;
     int item = blockIdx.x;
     if (item >= whole && items > whole) {
       shares = min(kMostShares, L::kSlots / (items - whole));
@@ -256,10 +250,21 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       PdlTrigger();
       return;
     }
-    b = __ffs(__ballot_sync(kFull, end > item)) - 1;
-    item -= __shfl_sync(kFull, end - own, b);
-    from_end = item / c.kv_heads;
-    g = item % c.kv_heads;
+    const int pair = item / c.kv_heads;
+    g = item - pair * c.kv_heads;
+    int level = 0, next = __reduce_max_sync(kFull, own), before = 0;  // before: tiles in front of `level`
+    while (next - level > 1) {
+      const int mid = (level + next) / 2, count = __reduce_add_sync(kFull, min(own, mid));
+      if (count <= pair) {
+        level = mid;
+        before = count;
+      } else {
+        next = mid;
+      }
+    }
+    from_end = level;
+    const uint32_t at_level = __ballot_sync(kFull, own > level);
+    b = __ffs(__ballot_sync(kFull, own > level && __popc(at_level & ((1u << lane) - 1u)) == pair - before)) - 1;
     run = Run{__shfl_sync(kFull, run.first, b), __shfl_sync(kFull, run.count, b), __shfl_sync(kFull, run.pos0, b)};
   } else {
     if (gridDim.x > c.kv_heads) {
@@ -899,11 +904,11 @@ int64_t MostTiles(const accel_b200_q8_cache& c, int64_t max_rows, int32_t heads)
   return CeilDiv(max_rows * (heads / c.kv_heads), Tiles<D>::kHalves * kHalf);
 }
 
-// Whether the last wave's walks are split: few waves, of walks that can be long.
+// Whether the last wave's walks are split: few waves, of walks long enough.
 template <int D>
 bool Splits(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window, int32_t sinks) {
   const int64_t seen = window > 0 ? Min64(c.context, static_cast<int64_t>(window) + sinks) : c.context;
-  return batch <= 32 && seen >= kSplitFrom &&
+  return batch <= 32 && seen >= 2 * kLeastShare * kTile &&
          batch * c.kv_heads * MostTiles<D>(c, max_rows, heads) <= 16 * Tiles<D>::kSlots;
 }
 

@@ -26,6 +26,7 @@ struct AttnArgs {
   const int32_t* row_pos;
   int32_t single_rows;     // how many of them
   int32_t sequences;       // prefill: sequences of `rows`
+  int32_t by_sequence;     // tiles of one sequence after the other, not the latest of all sequences first
   int32_t heads;
   int32_t group;        // heads per kv head
   int32_t block_shift;  // tokens per scale block, as a power of two

@@ -62,6 +62,7 @@ constexpr int kConverters = 4;     // warps
 constexpr int kChunk = 32;         // tokens whose scores a thread holds at a time: one scale block at most
 constexpr int kChunks = kTile / kChunk;
 constexpr int kMostShares = 8;      // CTAs that a walk is split over at most
+constexpr uint64_t kLevelsUpTo = 64 << 20;  // bytes of keys and values up to which L2 holds what a wave reads
 constexpr int kLeastShare = 4;      // tiles that each of them gets at least (it costs about two to begin and end)
 constexpr float kMostLift = 6.f;    // scales of a tile further apart than 2^6 are applied one by one
 constexpr int kPanel = 128 * 128;  // bytes of 128 rows x 64 fp16, the swizzle's row length
@@ -205,16 +206,18 @@ __device__ __forceinline__ bool MeetAny(int id, int threads, bool any) {
 
 // Grid (kv head, sequence, tile of kHalves * 128 vectors from the latest on): the
 // longest walks of all sequences start first, so that the last to start are short
-// (70 -> 62 us at 32 x 512 rows, against sequence after sequence). Tiles past the
-// grid's 65535 go with x.
+// (70 -> 62 us at 32 x 512 rows, against sequence after sequence). Where the calls'
+// keys and values are more than L2 holds, sequence after sequence, grid (kv head,
+// tile, sequence): CTAs that run together then read the same (5015 against 5452 us
+// for 8 x 1000 rows behind 30000 tokens, 8 kv heads of 128). Tiles past the grid's
+// 65535 go with x.
 constexpr int64_t kGridTiles = 65535;
 //
-// kSplit: a flat grid over the tiles of at most 32 sequences, in the same order (the
-// counting costs nothing that was measured). Those that fill whole
-// waves of the SMs go a CTA each; the walks of the rest are dealt to several CTAs,
-// so that the last wave is as short as it has room to be, and the last CTA of a
-// tile to arrive merges their states in order. (480 tiles, 3.2 waves, of walks of
-// 33: 559 -> 488 us.)
+// kSplit: a flat grid over the tiles of at most 32 sequences, in the same orders (the
+// counting costs nothing that was measured). Those that fill whole waves of the SMs
+// go a CTA each; the walks of the rest are dealt to several CTAs, so that the last
+// wave is as short as it has room to be, and the last CTA of a tile to arrive merges
+// their states in order. (480 tiles, 3.2 waves, of walks of 33: 559 -> 488 us.)
 template <int D, bool kSplit>
 __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     AttnTilesQ8Kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const AttnArgs a) {
@@ -226,8 +229,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
   const accel_b200_q8_cache& c = a.cache;
   const int G = a.group;
   constexpr int kVectors = L::kHalves * kHalf;
-  int g = blockIdx.x, b = blockIdx.y;
-  int64_t from_end = blockIdx.z;
+  int g = blockIdx.x, b = a.by_sequence ? blockIdx.z : blockIdx.y;
+  int64_t from_end = a.by_sequence ? blockIdx.y : blockIdx.z;
   int share = 0, shares = 1;  // this CTA's part of the tile's walk
   int split_tile = 0, state0 = 0;  // the tile's counter and first state
   PdlWait();
@@ -252,26 +255,41 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     }
     const int pair = item / c.kv_heads;
     g = item - pair * c.kv_heads;
-    int level = 0, next = __reduce_max_sync(kFull, own), before = 0;  // before: tiles in front of `level`
-    while (next - level > 1) {
-      const int mid = (level + next) / 2, count = __reduce_add_sync(kFull, min(own, mid));
-      if (count <= pair) {
-        level = mid;
-        before = count;
-      } else {
-        next = mid;
+    // Tiles of keys that the call sees, of a kv head.
+    const int64_t upto = static_cast<int64_t>(run.pos0) + run.count;
+    const int64_t seen = a.window > 0 ? Min64(upto, static_cast<int64_t>(a.window) + a.sinks + run.count) : upto;
+    const uint32_t key_tiles = __reduce_add_sync(kFull, static_cast<uint32_t>(run.count > 0 ? seen / kTile + 1 : 0));
+    if (static_cast<uint64_t>(key_tiles) * c.kv_heads * (2 * kTile * D) > kLevelsUpTo) {
+      int end = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(kFull, end, o);
+        if (lane >= o) end += other;
       }
+      b = __ffs(__ballot_sync(kFull, end > pair)) - 1;
+      from_end = pair - __shfl_sync(kFull, end - own, b);
+    } else {
+      int level = 0, next = __reduce_max_sync(kFull, own), before = 0;  // before: tiles in front of `level`
+      while (next - level > 1) {
+        const int mid = (level + next) / 2, count = __reduce_add_sync(kFull, min(own, mid));
+        if (count <= pair) {
+          level = mid;
+          before = count;
+        } else {
+          next = mid;
+        }
+      }
+      from_end = level;
+      const uint32_t at_level = __ballot_sync(kFull, own > level);
+      b = __ffs(__ballot_sync(kFull, own > level && __popc(at_level & ((1u << lane) - 1u)) == pair - before)) - 1;
     }
-    from_end = level;
-    const uint32_t at_level = __ballot_sync(kFull, own > level);
-    b = __ffs(__ballot_sync(kFull, own > level && __popc(at_level & ((1u << lane) - 1u)) == pair - before)) - 1;
     run = Run{__shfl_sync(kFull, run.first, b), __shfl_sync(kFull, run.count, b), __shfl_sync(kFull, run.pos0, b)};
   } else {
+    run = RunOf(a.rows, b, c.context, g == 0 && from_end == 0 && tid == 0, a.status);
     if (gridDim.x > c.kv_heads) {
       from_end += g / c.kv_heads * kGridTiles;
       g %= c.kv_heads;
     }
-    run = RunOf(a.rows, b, c.context, blockIdx.x == 0 && blockIdx.z == 0 && tid == 0, a.status);
   }
   const int64_t vectors = static_cast<int64_t>(run.count) * G;
   const int64_t tiles = (vectors + kVectors - 1) / kVectors;
@@ -934,18 +952,21 @@ int Launch(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
     return SetError(ACCEL_B200_EINVAL, "attention_prefill_q8: cache tensor map rejected");
   }
   const int64_t tiles = MostTiles<D>(a.cache, max_rows, a.heads), kv = a.cache.kv_heads;
+  const unsigned x = static_cast<unsigned>(CeilDiv(tiles, kGridTiles) * kv), y = static_cast<unsigned>(a.sequences),
+                 z = static_cast<unsigned>(Min64(tiles, kGridTiles));
   const dim3 grid = kSplit ? dim3(static_cast<unsigned>(a.sequences * kv * tiles + Tiles<D>::kSlots))
-                           : dim3(static_cast<unsigned>(CeilDiv(tiles, kGridTiles) * kv),
-                                  static_cast<unsigned>(a.sequences), static_cast<unsigned>(Min64(tiles, kGridTiles)));
+                           : a.by_sequence ? dim3(x, z, y) : dim3(x, y, z);
   return CheckLaunchEx(
       LaunchK(AttnTilesQ8Kernel<D, kSplit>, grid, dim3(Tiles<D>::kThreads), kSmem, stream, 1u, 1u, tk, tv, a),
       "attention_prefill_q8");
 }
 
 template <int D>
-int LaunchFor(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
-  return Splits<D>(a.cache, a.sequences, max_rows, a.heads, a.window, a.sinks) ? Launch<D, true>(a, max_rows, stream)
-                                                                               : Launch<D, false>(a, max_rows, stream);
+int LaunchFor(AttnArgs a, int32_t max_rows, cudaStream_t stream) {
+  if (Splits<D>(a.cache, a.sequences, max_rows, a.heads, a.window, a.sinks)) return Launch<D, true>(a, max_rows, stream);
+  const int64_t most = a.window > 0 ? Min64(a.cache.context, static_cast<int64_t>(a.window) + a.sinks + max_rows) : a.cache.context;
+  a.by_sequence = static_cast<uint64_t>(most) * (2 * D) * a.sequences * a.cache.kv_heads > kLevelsUpTo;
+  return Launch<D, false>(a, max_rows, stream);
 }
 
 template <int D>

@@ -403,6 +403,8 @@ SPLITS = [
     (6, 1, 64, 30000, [29000, -1, 20000, 100], [1000, 5, 2, 777], 0, 0),
     (32, 8, 128, 6000, [4700, 300], [1200, 1200], 0, 0),
     (12, 4, 64, 5000, [0, 900], [4999, 4100], 4100, 200),
+    # More keys and values than L2 holds: tiles of one sequence after the other.
+    (6, 3, 64, 66000, [65000, 60000, 64000], [900, 10, 333], 0, 0),
 ]
 
 
@@ -436,6 +438,22 @@ def test_prefill_walks_shared_by_ctas(lib, cuda, heads, kv, d, context, pos0, co
     np.testing.assert_array_equal(H(x)[~left], got[~left])
     with pytest.raises(B200Error):
         K.attention_prefill_q8(T(q), *run, workspace=ws[:-16])
+
+
+def test_prefill_of_many_sequences_of_a_large_cache(lib, cuda):
+    """More than 32 sequences, more keys and values than L2 holds."""
+    rng = np.random.default_rng(12)
+    heads, kv, d, context, slots = 4, 2, 64, 8300, 33
+    c = filled(rng, slots, kv, context, d, 64)
+    count = rng.integers(0, 300, slots)
+    pos0 = rng.integers(0, context - 300, slots)
+    first = ragged(count)
+    q = rng.standard_normal((int(count.sum()) + 1, heads * d), dtype=np.float32)
+    run = (device_cache(c), I(first.tolist()), I(count.tolist()), I(pos0.tolist()), heads, 1500)
+    got = H(K.attention_prefill_q8(T(q), *run))
+    check = [(int(first[b]) + i, b, int(pos0[b]) + i) for b in range(0, slots, 3) for i in {0, int(count[b]) - 1} if i >= 0]
+    check_rows(c, q, got, [r for r in check if count[r[1]] > 0], heads, 0, 0)
+    assert (got[-1] == 0).all()
 
 
 def test_prefill_walks_shared_by_ctas_skip_and_ignore(lib, cuda):

@@ -680,20 +680,24 @@ int CheckWorkspace(size_t need, const void* workspace, size_t bytes, const std::
   return ACCEL_B200_OK;
 }
 
-// Whether a prefill takes the 256-vector tiles of attention_q8_tiles.cu. Both
-// kernels' times go by the tokens that rows see: a tile CTA walks 128 of them
-// in about 2.4 us (3.0 at 128 dimensions), one wave of 148 CTAs after another;
-// the groups of 8 vectors here share the whole GPU at about 1700 (1100) of
-// their units of 32 tokens per us. Tiles are faster from 900 groups per wave.
-// (Measured behind 16000 tokens, with 3 kv heads of 64, 12 heads: 32 sequences of
-// 16 rows 311 us in tiles and 216 here, of 32 rows 304 and 357; one sequence of
-// 128 rows 209 and 52. With 8 kv heads of 128, 32 heads: 32 sequences of 8 rows
-// 695 and 450, of 16 rows 727 and 734; 4 of 64 rows 425 and 489.)
-constexpr int64_t kTileGroups = 900;
-bool TakesTiles(const accel_b200_q8_cache& c, int64_t batch, int64_t max_rows, int32_t heads) {
-  const int64_t vectors = max_rows * (heads / c.kv_heads), runs = batch * c.kv_heads;
-  const int64_t waves = CeilDiv(runs * CeilDiv(vectors, kTileVectors), kSms);
-  return runs * CeilDiv(vectors, kVec) > kTileGroups * waves;
+// Whether a prefill takes the tiles of attention_q8_tiles.cu. Both kernels' times
+// go by the tokens that rows see. A wave of tile CTAs (256 vectors per SM) walks
+// 128 of them in about 2.4 us (3.0 at 128 dimensions), and where the last wave's
+// walks are split, merging takes 20 us (37). The groups of 8 vectors here share
+// the whole GPU at about 1700 (1100) of their units of 32 tokens per us. So tiles are
+// faster from 900 groups per wave, or where walks are split from 900 per part of a
+// wave and 9000 / steps for the merge.
+// (Measured, tiles and groups. 3 kv heads of 64, 12 heads, behind 16000 tokens: 4
+// sequences of 16 rows 42 and 32 us, of 32 rows 51 and 65, 32 of 16 rows 147 and 214;
+// behind 5000: 4 of 32 rows 26 and 19, of 64 rows 30 and 43. 8 kv heads of 128, 32
+// heads, behind 16000: 1 of 32 rows 42 and 33, of 64 rows 90 and 142, 32 of 8 rows 681
+// and 451, of 16 rows 711 and 735; behind 300, unsplit: 32 of 8 rows 35 and 42.)
+constexpr double kTileGroups = 900, kSplitGroupSteps = 9000;
+bool TakesTiles(const accel_b200_q8_cache& c, int64_t batch, int64_t max_rows, int32_t heads, const TilesPlan& plan) {
+  const int64_t groups = batch * c.kv_heads * CeilDiv(max_rows * (heads / c.kv_heads), kVec);
+  double least = kTileGroups * ceil(plan.waves);
+  if (plan.split) least = fmin(least, kTileGroups * plan.waves + kSplitGroupSteps / static_cast<double>(plan.steps));
+  return static_cast<double>(groups) > least;
 }
 
 AttnArgs ArgsOf(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, const RaggedRows& rows,
@@ -806,7 +810,8 @@ ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200
     return 0;
   }
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));
-  if (TakesTiles(*cache, batch, max_rows, heads)) return TilesWorkspaceQ8(*cache, batch, max_rows, heads, window, sinks);
+  const TilesPlan tiles = PlanTilesQ8(*cache, batch, max_rows, heads, window, sinks);
+  if (TakesTiles(*cache, batch, max_rows, heads, tiles)) return tiles.workspace;
   return SplitFor(*cache, batch, max_rows, heads, window, sinks, false).workspace;
 }
 
@@ -828,12 +833,12 @@ ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld,
   AttnArgs a = ArgsOf(q, q_ld, cache, RaggedRows{first, count, pos0, max_rows, rows}, nullptr, nullptr, heads, window,
                       sinks, out, out_ld, status);
   a.sequences = batch;
-  if (TakesTiles(*cache, batch, max_rows, heads)) {
-    const size_t need = TilesWorkspaceQ8(*cache, batch, max_rows, heads, window, sinks);
-    rc = CheckWorkspace(need, workspace, workspace_bytes, "attention_prefill_q8");
+  const TilesPlan tiles = PlanTilesQ8(*cache, batch, max_rows, heads, window, sinks);
+  if (TakesTiles(*cache, batch, max_rows, heads, tiles)) {
+    rc = CheckWorkspace(tiles.workspace, workspace, workspace_bytes, "attention_prefill_q8");
     if (rc != ACCEL_B200_OK) return rc;
-    if (need > 0) SetWorkspace(&a, workspace);
-    return LaunchTilesQ8(a, max_rows, AsStream(stream));
+    if (tiles.workspace > 0) SetWorkspace(&a, workspace);
+    return LaunchTilesQ8(a, tiles, max_rows, AsStream(stream));
   }
   const Split p = SplitFor(*cache, batch, max_rows, heads, window, sinks, false);
   if (static_cast<int64_t>(cache->kv_heads) * p.vec_groups > 65535) {

@@ -87,10 +87,20 @@ struct Vectors {
 __device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ? max(0, pos - window + 1) : 0; }
 
 // Prefill attention on the tcgen05 tensor cores, kTileVectors query vectors per
-// SM (attention_q8_tiles.cu), and the bytes of workspace that it takes.
+// SM (attention_q8_tiles.cu).
 constexpr int kTileVectors = 256;
-size_t TilesWorkspaceQ8(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
-                        int32_t sinks);
-int LaunchTilesQ8(const AttnArgs& a, int32_t max_rows, cudaStream_t stream);
+
+// How a call would run there: the bytes of workspace that it takes, and for an
+// estimate of its time the waves of CTAs and the 128-token steps of a whole walk
+// (upper bounds: the device alone knows counts and positions).
+struct TilesPlan {
+  bool split;  // the last wave's walks are shared by several CTAs
+  double waves;
+  int64_t steps;
+  size_t workspace;
+};
+TilesPlan PlanTilesQ8(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
+                      int32_t sinks);
+int LaunchTilesQ8(const AttnArgs& a, const TilesPlan& plan, int32_t max_rows, cudaStream_t stream);
 
 }  // namespace accel_b200

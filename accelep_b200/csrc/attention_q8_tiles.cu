@@ -922,12 +922,24 @@ int64_t MostTiles(const accel_b200_q8_cache& c, int64_t max_rows, int32_t heads)
   return CeilDiv(max_rows * (heads / c.kv_heads), Tiles<D>::kHalves * kHalf);
 }
 
-// Whether the last wave's walks are split: few waves, of walks long enough.
+// The last wave's walks are split in calls of few waves and of walks long enough.
 template <int D>
-bool Splits(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window, int32_t sinks) {
+TilesPlan Plan(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
+               int32_t sinks) {
+  constexpr int64_t kSlots = Tiles<D>::kSlots;
+  static_assert(kSlots <= kMaxCounters, "a counter per split tile");
+  TilesPlan p{};
   const int64_t seen = window > 0 ? Min64(c.context, static_cast<int64_t>(window) + sinks) : c.context;
-  return batch <= 32 && seen >= 2 * kLeastShare * kTile &&
-         batch * c.kv_heads * MostTiles<D>(c, max_rows, heads) <= 16 * Tiles<D>::kSlots;
+  const int64_t items = batch * c.kv_heads * MostTiles<D>(c, max_rows, heads), rest = items % kSlots;
+  p.steps = CeilDiv(seen, kTile);
+  p.split = batch <= 32 && p.steps >= 2 * kLeastShare && items <= 16 * kSlots;
+  p.waves = static_cast<double>(items / kSlots);
+  if (rest > 0) {
+    const int64_t shares = p.split ? Min64(Min64(kMostShares, kSlots / rest), p.steps / kLeastShare) : 1;
+    p.waves += 1. / static_cast<double>(shares);
+  }
+  if (p.split) p.workspace = kCounterRegion + static_cast<size_t>(kSlots) * Tiles<D>::kStateFloats * sizeof(float);
+  return p;
 }
 
 template <int D, bool kSplit>
@@ -962,31 +974,24 @@ int Launch(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
 }
 
 template <int D>
-int LaunchFor(AttnArgs a, int32_t max_rows, cudaStream_t stream) {
-  if (Splits<D>(a.cache, a.sequences, max_rows, a.heads, a.window, a.sinks)) return Launch<D, true>(a, max_rows, stream);
-  const int64_t most = a.window > 0 ? Min64(a.cache.context, static_cast<int64_t>(a.window) + a.sinks + max_rows) : a.cache.context;
-  a.by_sequence = static_cast<uint64_t>(most) * (2 * D) * a.sequences * a.cache.kv_heads > kLevelsUpTo;
+int LaunchFor(AttnArgs a, const TilesPlan& plan, int32_t max_rows, cudaStream_t stream) {
+  if (plan.split) return Launch<D, true>(a, max_rows, stream);
+  const int64_t rows = a.window > 0 ? static_cast<int64_t>(a.window) + a.sinks + max_rows : a.cache.context;
+  const int64_t bytes = Min64(a.cache.context, rows) * (2 * D) * a.cache.kv_heads;  // of a sequence
+  a.by_sequence = bytes > static_cast<int64_t>(kLevelsUpTo) / a.sequences;
   return Launch<D, false>(a, max_rows, stream);
-}
-
-template <int D>
-size_t WorkspaceFor(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
-                    int32_t sinks) {
-  if (!Splits<D>(c, batch, max_rows, heads, window, sinks)) return 0;
-  static_assert(Tiles<D>::kSlots <= kMaxCounters, "a counter per split tile");
-  return kCounterRegion + static_cast<size_t>(Tiles<D>::kSlots) * Tiles<D>::kStateFloats * sizeof(float);
 }
 
 }  // namespace
 
-size_t TilesWorkspaceQ8(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
-                        int32_t sinks) {
-  return c.head_dim == 64 ? WorkspaceFor<64>(c, batch, max_rows, heads, window, sinks)
-                          : WorkspaceFor<128>(c, batch, max_rows, heads, window, sinks);
+TilesPlan PlanTilesQ8(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
+                      int32_t sinks) {
+  return c.head_dim == 64 ? Plan<64>(c, batch, max_rows, heads, window, sinks)
+                          : Plan<128>(c, batch, max_rows, heads, window, sinks);
 }
 
-int LaunchTilesQ8(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
-  return a.cache.head_dim == 64 ? LaunchFor<64>(a, max_rows, stream) : LaunchFor<128>(a, max_rows, stream);
+int LaunchTilesQ8(const AttnArgs& a, const TilesPlan& plan, int32_t max_rows, cudaStream_t stream) {
+  return a.cache.head_dim == 64 ? LaunchFor<64>(a, plan, max_rows, stream) : LaunchFor<128>(a, plan, max_rows, stream);
 }
 
 }  // namespace accel_b200

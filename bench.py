@@ -194,6 +194,15 @@ def c4_tasks():
             [("decode", i, i) for i in range(DECODE_BINS)])
 
 
+def reference_missing():
+    """Why the reference's CPU path cannot be timed ("" if it can): a pool whose
+    processes fail as they start would start new ones for good."""
+    from oracle.oracle import REF_C4_LIB, REF_SOURCES
+    if REF_C4_LIB.is_file() or (REF_SOURCES / "src" / "llama_model.cc").is_file():
+        return ""
+    return "the AccelEP sources are not there to build its CPU path from"
+
+
 class ReferencePool:
     """`procs` single-threaded reference processes, each holding the C4 model
     (the reference fp32 Llama with the dequantized int8 weights, which is the
@@ -221,6 +230,10 @@ class ReferencePool:
 def run_reference(args):
     rank = int(os.environ.get("RANK", "0"))
     if rank != 0:
+        return
+    missing = reference_missing()
+    if missing:
+        print(json.dumps({"impl": "reference", "unavailable": missing}), flush=True)
         return
     cores = os.cpu_count() or 1
     procs = max(1, min(SEQS, cores))
@@ -610,7 +623,8 @@ def run_b200(args):
         extras = None if args.no_extras or world > 1 else metric_set(torch, peak)
         cpu = None
         if world == 1 and not args.no_cpu_baseline:
-            cpu = cpu_baseline_one_core()
+            missing = reference_missing()
+            cpu = {"unavailable": missing} if missing else cpu_baseline_one_core()
         cfg_line = config(world, seqs)
         if prompt_len != PROMPT or new != NEW:
             cfg_line["workload"] = f"profiling variant: prompt {prompt_len}, {new} new ids (not the C4 bench number)"

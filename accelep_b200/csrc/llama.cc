@@ -554,18 +554,20 @@ class Engine {
       one.k_scale += slot * one.scale_seq_stride;
       one.v_scale += slot * one.scale_seq_stride;
       one.slots = 1;
-      const int32_t run[3] = {0, nrows, 0};  // first, count, pos0
+      int32_t run[4] = {0, nrows, 0, 0};  // first, count, pos0, and the read's own status word
       DevBuf args, rows_out;
       args.Alloc(sizeof(run));
       rows_out.Alloc(static_cast<size_t>(nrows) * kv_out * 4);
-      Cuda(cudaMemcpy(args.p, run, sizeof(run), cudaMemcpyHostToDevice), "cache");
-      const int32_t* at = args.as<int32_t>();
+      Cuda(cudaMemcpyAsync(args.p, run, sizeof(run), cudaMemcpyHostToDevice, stream), "cache");
+      int32_t* at = args.as<int32_t>();
       float* dst = rows_out.as<float>();
       Abi(accel_b200_cache_rows_q8(&one, at, at + 1, at + 2, 1, nrows, which == 0 ? dst : nullptr,
-                                   which == 1 ? dst : nullptr, kv_out, nrows, nullptr, stream));
+                                   which == 1 ? dst : nullptr, kv_out, nrows, at + 3, stream));
       Cuda(cudaMemcpyAsync(out, dst, static_cast<size_t>(nrows) * kv_out * 4, cudaMemcpyDeviceToHost, stream),
            "cache");
+      Cuda(cudaMemcpyAsync(run, args.p, sizeof(run), cudaMemcpyDeviceToHost, stream), "cache");
       Cuda(cudaStreamSynchronize(stream), "cache");
+      if (run[3] != 0) throw std::runtime_error("the cache read reported status " + std::to_string(run[3]));
       return;
     }
     // Head-major in HBM; the reference layout [rows, kv_heads, head_dim] on the host.

@@ -286,9 +286,9 @@ class Engine {
     std::vector<float> t(static_cast<size_t>(rows * cols));
     for (int64_t o = 0; o < rows; ++o)
       for (int64_t i = 0; i < cols; ++i) t[static_cast<size_t>(i * rows + o)] = data[o * cols + i];
-    Cuda(cudaMemcpy2D(g->w.as<float>() + g->col0[member], g->n * sizeof(float), t.data(), rows * sizeof(float),
-                      rows * sizeof(float), cols, cudaMemcpyHostToDevice),
-         "weight upload");
+    Upload2D(g->w.as<float>() + g->col0[member], g->n * sizeof(float), t.data(), rows * sizeof(float),
+             rows * sizeof(float), cols, "weight upload");
+    Cuda(cudaStreamSynchronize(stream), "weight upload");
     NoteBytesToDevice(t.size() * sizeof(float));
     g->loaded |= 1u << member;
     DropGraphs();
@@ -311,20 +311,14 @@ class Engine {
     if (g->paired) {
       // Block b of this member (gate: 0, up: 1) to columns 128 b + 64 member.
       for (int64_t b = 0; b < rows / 64; ++b) {
-        Cuda(cudaMemcpy2D(g->w.as<int8_t>() + 128 * b + 64 * member, g->n, t.data() + 64 * b, rows, 64, cols,
-                          cudaMemcpyHostToDevice),
-             "weight upload");
-        Cuda(cudaMemcpy(g->scale.as<float>() + 128 * b + 64 * member, scale + 64 * b, 64 * sizeof(float),
-                        cudaMemcpyHostToDevice),
-             "scale upload");
+        Upload2D(g->w.as<int8_t>() + 128 * b + 64 * member, g->n, t.data() + 64 * b, rows, 64, cols, "weight upload");
+        Upload(g->scale.as<float>() + 128 * b + 64 * member, scale + 64 * b, 64 * sizeof(float), "scale upload");
       }
     } else {
-      Cuda(cudaMemcpy2D(g->w.as<int8_t>() + g->col0[member], g->n, t.data(), rows, rows, cols,
-                        cudaMemcpyHostToDevice),
-           "weight upload");
-      Cuda(cudaMemcpy(g->scale.as<float>() + g->col0[member], scale, rows * sizeof(float), cudaMemcpyHostToDevice),
-           "scale upload");
+      Upload2D(g->w.as<int8_t>() + g->col0[member], g->n, t.data(), rows, rows, cols, "weight upload");
+      Upload(g->scale.as<float>() + g->col0[member], scale, rows * sizeof(float), "scale upload");
     }
+    Cuda(cudaStreamSynchronize(stream), "weight upload");
     NoteBytesToDevice(t.size() + rows * sizeof(float));
     g->loaded |= 1u << member;
     DropGraphs();
@@ -619,10 +613,22 @@ class Engine {
     }
   }
 
+  // Host memory (of any kind) to device memory, in front of the engine's next
+  // kernels: a copy from pageable memory on the legacy stream may return before
+  // its bytes arrive, and the engine's stream does not wait for it. The caller
+  // waits for the stream before the host memory goes.
+  void Upload(void* dst, const void* src, size_t bytes, const char* what) {
+    Cuda(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyHostToDevice, stream), what);
+  }
+  void Upload2D(void* dst, size_t dst_ld, const void* src, size_t src_ld, size_t width, size_t rows, const char* what) {
+    Cuda(cudaMemcpy2DAsync(dst, dst_ld, src, src_ld, width, rows, cudaMemcpyHostToDevice, stream), what);
+  }
+
   void UploadRaw(DevBuf* slot, const void* data, size_t bytes) {
     slot->Alloc(bytes);
     if (bytes > 0) {
-      Cuda(cudaMemcpy(slot->p, data, bytes, cudaMemcpyHostToDevice), "upload");
+      Upload(slot->p, data, bytes, "upload");
+      Cuda(cudaStreamSynchronize(stream), "upload");
       NoteBytesToDevice(bytes);
     }
     DropGraphs();

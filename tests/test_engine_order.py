@@ -21,7 +21,7 @@ def engine_on_host(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("case", ["cache_rows"])
+@pytest.mark.parametrize("case", ["cache_rows", "weights", "int8_weights"])
 def test_copies_arrive_before_the_kernels_that_read_them(engine_on_host, case):
     out = subprocess.run([str(engine_on_host), case], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0, out.stdout

@@ -142,7 +142,10 @@ ACCEL_B200_API AccelBuf* accel_sim_upload(AccelSim* sim, const float* data, int6
     const size_t bytes = FloatBytes(count);
     float* dev = nullptr;
     OrThrow(cudaMalloc(&dev, bytes == 0 ? 1 : bytes), "upload");
-    const cudaError_t err = bytes == 0 ? cudaSuccess : cudaMemcpy(dev, data, bytes, cudaMemcpyHostToDevice);
+    // On the Sim's own stream: it does not wait for the legacy stream, where a
+    // copy from pageable memory may return before its bytes arrive.
+    cudaError_t err = bytes == 0 ? cudaSuccess : cudaMemcpyAsync(dev, data, bytes, cudaMemcpyHostToDevice, sim->stream);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(sim->stream);
     if (err != cudaSuccess) cudaFree(dev);
     OrThrow(err, "upload");
     accel_b200::NoteBytesToDevice(bytes);

@@ -1,5 +1,5 @@
-// Test support: the Llama engine (csrc/llama.cc) over a CUDA runtime of host
-// memory, for what a GPU shows only by luck: the order of copies and kernels.
+// Test support: the Llama engine (csrc/llama.cc) and the Sim's C API
+// (csrc/sim_api.cc) over a CUDA runtime of host memory, for what a GPU shows only by luck: the order of copies and kernels.
 // A copy from pageable memory on the legacy stream may return before its bytes
 // arrive, and a non-blocking stream does not wait for it; here such bytes
 // arrive at the next device synchronisation or legacy operation, no earlier.
@@ -114,6 +114,7 @@ int accel_b200_matmul_q8_rmsnorm(const float*, int64_t, const float*, float, con
                                  int64_t, int64_t, int64_t, const accel_b200_epilogue*, void*, size_t, void*) {
   return Kernel();
 }
+int accel_b200_matmul(const float*, const float*, float*, int64_t, int64_t, int64_t, void*) { return Kernel(); }
 int accel_b200_rope_append(float*, int64_t, const int32_t*, const int32_t*, int64_t, int32_t, int32_t, int32_t,
                            const float*, const float*, float*, float*, int64_t, int64_t, int64_t, void*) {
   return Kernel();
@@ -153,6 +154,8 @@ void NoteLaunches(int64_t) {}
 void NoteKernelMatmuls(int64_t) {}
 void NoteBytesToDevice(size_t) {}
 void NoteBytesToHost(size_t) {}
+void ResetCounters() {}
+Counters GetCounters() { return {}; }
 }  // namespace accel_b200
 
 namespace {
@@ -206,6 +209,19 @@ int Weights(AccelLlama* model, bool int8) {
   return Check(g_overtaken == 0, "kernels ran in front of copies that they read");
 }
 
+// An uploaded matrix is there when the first product reads it.
+int SimUpload() {
+  AccelSim* sim = accel_sim_create();
+  const float x[4] = {1, 2, 3, 4};
+  float c[4];
+  AccelBuf* b = accel_sim_upload(sim, x, 4);
+  int bad = Check(b != nullptr && accel_sim_matmul(sim, x, 2, 2, b, 2, c) == 0, accel_sim_last_error());
+  bad |= Check(g_overtaken == 0, "the product ran in front of its operand's copy");
+  accel_sim_release(sim, b);
+  accel_sim_destroy(sim);
+  return bad;
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -216,6 +232,7 @@ int main(int argc, char** argv) {
   if (name == "cache_rows") bad = CacheRows(model);
   if (name == "weights") bad = Weights(model, false);
   if (name == "int8_weights") bad = Weights(model, true);
+  if (name == "sim_upload") bad = SimUpload();
   accel_llama_destroy(model);
   return bad;
 }

@@ -390,8 +390,8 @@ def _rows(name, t, index, width):
     if t.dtype is not _FLOAT32 or t.get_device() != index or len(shape) != 2 or shape[1] != width or stride[1] != 1:
         raise ValueError(f"{name} must be fp32 [rows, {width}] with contiguous rows on cuda:{index}")
     rows = shape[0]
-    # One row has no stride that matters (torch may report any).
-    return rows, stride[0] if rows > 1 else max(stride[0], width)
+    # One row has no stride that matters (torch reports that of the tensor it was cut from).
+    return rows, stride[0] if rows > 1 else width
 
 
 def _i32(name, t, index, n):

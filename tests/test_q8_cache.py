@@ -160,3 +160,13 @@ def test_python_cache_refuses_other_blocks(block):
         K.Q8Cache(k, k.clone(), s, s.clone(), block)
     with pytest.raises(ValueError, match="block"):
         K.Q8Cache.zeros(1, 1, 8, 64, block, device="cpu")
+
+
+def test_python_rows_of_one_have_no_stride():
+    """One row of a wider tensor, whatever its stride there."""
+    wide = torch.zeros(3, 131)
+    assert K._rows("x", wide[1:2, :128], -1, 128) == (1, 128)
+    assert K._rows("x", wide[:1, :128], -1, 128) == K._rows("x", torch.zeros(1, 128), -1, 128)
+    assert K._rows("x", torch.zeros(1, 128).expand(1, 128), -1, 128) == (1, 128)
+    assert K._rows("x", wide[:0, :128], -1, 128) == (0, 128)
+    assert K._rows("x", torch.zeros(3, 136)[:, :128], -1, 128) == (3, 136)

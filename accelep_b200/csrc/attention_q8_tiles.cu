@@ -43,6 +43,7 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 #include <type_traits>
 
@@ -947,15 +948,19 @@ int Launch(const AttnArgs& a, int32_t max_rows, cudaStream_t stream) {
   constexpr int kSmem = Tiles<D>::kBytes + Tiles<D>::kAlign;
   // The roles trade the registers that the launch gives out; were they fewer
   // than the split adds up to, the role that takes more would wait for good.
-  static const int regs = [] {
+  // Asked for until there is an answer: a device that cannot give one now may later.
+  static std::atomic<int> regs{0};
+  cudaError_t err = cudaSuccess;
+  if (regs.load(std::memory_order_relaxed) == 0) {
     cudaFuncAttributes f{};
-    return cudaFuncGetAttributes(&f, AttnTilesQ8Kernel<D, kSplit>) == cudaSuccess ? f.numRegs : 0;
-  }();
-  if (regs != Tiles<D>::kLaunch) {
+    err = cudaFuncGetAttributes(&f, AttnTilesQ8Kernel<D, kSplit>);
+    if (err != cudaSuccess) return CheckLaunchEx(err, "attention_prefill_q8");
+    regs.store(f.numRegs, std::memory_order_relaxed);
+  }
+  if (regs.load(std::memory_order_relaxed) != Tiles<D>::kLaunch) {
     return SetError(ACCEL_B200_ECUDA, "attention_prefill_q8: the kernel's registers do not fit its split");
   }
-  const cudaError_t err =
-      cudaFuncSetAttribute(AttnTilesQ8Kernel<D, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  err = cudaFuncSetAttribute(AttnTilesQ8Kernel<D, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (err != cudaSuccess) return CheckLaunchEx(err, "attention_prefill_q8");
   const uint64_t plane_rows = static_cast<uint64_t>(PlaneRows(a.cache));
   CUtensorMap tk{}, tv{};

@@ -170,3 +170,15 @@ def test_python_rows_of_one_have_no_stride():
     assert K._rows("x", torch.zeros(1, 128).expand(1, 128), -1, 128) == (1, 128)
     assert K._rows("x", wide[:0, :128], -1, 128) == (0, 128)
     assert K._rows("x", torch.zeros(3, 136)[:, :128], -1, 128) == (3, 136)
+
+
+def test_prefill_without_a_device_says_so(lib):
+    """The tile kernel's registers cannot be asked for without a device: the
+    call gives CUDA's error, not one about the registers."""
+    if torch.cuda.is_available():
+        pytest.skip("there is a device")
+    big = cache(k=1 << 30, v=1 << 31, k_scale=1 << 32, v_scale=1 << 33, context=512, seq_stride=2 * 512 * 64,
+                head_stride=512 * 64, scale_seq_stride=16, scale_head_stride=8)
+    for _ in range(2):
+        assert prefill(lib, big, heads=16, ld=1024, out=1 << 34, out_ld=1024, max_rows=512) == 3
+        assert b"CUDA" in lib.accel_b200_last_error() and b"registers" not in lib.accel_b200_last_error()

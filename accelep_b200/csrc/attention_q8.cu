@@ -100,6 +100,13 @@ __device__ __forceinline__ Units UnitsOf(int near, int pos, int sinks) {
   return u;
 }
 
+// The sizes (in units) that a CTA of a balanced launch may have: 32, evenly
+// spread from the even share to twice that.
+constexpr int BalancedSize(int even, int i) { return even + (even * i + 30) / 31; }
+static_assert(BalancedSize(8, 0) == 8 && BalancedSize(8, 31) == 16 && BalancedSize(33, 31) == 66 &&
+                  BalancedSize(1 << 25, 0) == 1 << 25 && BalancedSize(1 << 25, 31) == 1 << 26,
+              "from the even share to exactly twice that, without overflow");
+
 // What a launch's rows are: single rows or runs of a sequence's rows, in grid
 // (split, kv head x vector group, row or sequence); or single rows, at most 32,
 // over a flat grid whose CTAs go to the rows by how much each row sees.
@@ -149,13 +156,12 @@ __global__ void __launch_bounds__(kThreads, kResident<D>) AttnVectorsQ8Kernel(
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(kFull, total, o);
     const int even = static_cast<int>(Max64(kWarps * kWarpUnits, (total * pairs + T - 1) / T));
-    const int size = even + (even * lane + 31) / 32;
+    const int size = BalancedSize(even, lane);
     int64_t ctas = 0;
     for (int r = 0; r < a.single_rows; ++r) ctas += (__shfl_sync(kFull, mine_units, r) + size - 1) / size;
-    // (Twice the even share always fits: it needs T / 2 CTAs and one more for
-    // each row and pair, of which there are T / 2 at most.)
-    const int fits = __ffs(__ballot_sync(kFull, ctas * pairs <= T)) - 1;
-    const int q = __shfl_sync(kFull, size, fits < 0 ? 31 : fits);
+    // (Lane 31's size, twice the even share, always fits: it needs T / 2 CTAs
+    // and less than one more for each row and pair, of which there are T / 2 at most.)
+    const int q = __shfl_sync(kFull, size, __ffs(__ballot_sync(kFull, ctas * pairs <= T)) - 1);
     const int share = (mine_units + q - 1) / q;  // CTAs per pair of row `lane`
     int end = share * pairs;
 #pragma unroll
@@ -624,8 +630,9 @@ Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run,
   const int64_t resident = kSms * (c.head_dim == 64 ? kResident<64> : kResident<128>);
   const int64_t seen = window > 0 ? Min64(c.context, static_cast<int64_t>(window) + sinks + rows_per_run) : c.context;
   const int64_t most = CeilDiv(CeilDiv(seen, kUnit), kWarps * kWarpUnits);
-  int64_t s = Max64(1, Min64(resident / Max64(1, p.groups), most));
-  if (p.groups > kMaxCounters) s = Min64(s, kMaxCluster);
+  const int64_t s = Max64(1, Min64(resident / Max64(1, p.groups), most));
+  static_assert(kSms * kResident<64> <= kMaxCounters && kSms * kResident<128> <= kMaxCounters,
+                "a counter per group: where they are split there are no more than resident CTAs");
   p.s = static_cast<int>(s);
   // Single rows of few, long sequences take CTAs by their own lengths, where the
   // grid has room for a CTA more per row and pair. (Measured with 8 kv heads

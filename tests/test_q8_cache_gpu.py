@@ -822,3 +822,24 @@ def test_python_calls_of_nothing(lib, cuda):
         assert K.cache_rows_q8(k_out=kv, **run)[0] is kv
     assert K.attention_decode_q8(torch.ones(0, 256, device="cuda"), dev, none, 4).shape == (0, 256)
     assert lib.accel_b200_launch_count() == before
+
+
+@pytest.mark.parametrize("rows,heads,d", [(18, 64, 128), (27, 64, 64), (32, 32, 128), (32, 48, 64)])
+@pytest.mark.parametrize("lengths", ["equal", "a unit more", "one long", "spread"])
+def test_decode_balanced_over_as_many_rows_as_fit(lib, cuda, rows, heads, d, lengths):
+    """Grids of which rows and vector groups need half, the most that CTAs go to by
+    length: every row is written, whatever the lengths leave to round up."""
+    rng = np.random.default_rng(rows + heads + d)
+    context = 16400
+    c = filled(rng, rows, 1, context, d, 64)
+    pos = {"equal": np.full(rows, context - 1), "a unit more": np.arange(1, rows + 1) * 32 * 16,
+           "one long": np.where(np.arange(rows) == rows // 2, context - 1, 32),
+           "spread": np.linspace(0, context - 1, rows).astype(int)}[lengths].astype(np.int32)
+    q = rng.standard_normal((rows, heads * d), dtype=np.float32)
+    dev = device_cache(c)
+    ws = K.attention_decode_q8_workspace(dev, rows, heads)
+    assert ws is not None
+    got = H(K.attention_decode_q8(T(q), dev, T(pos), heads, out=torch.full((rows, heads * d), np.nan, device="cuda"),
+                                  workspace=ws))
+    assert np.isfinite(got).all() and not H(ws)[:65536].any()
+    check_rows(c, q, got, [(r, r, int(pos[r])) for r in (0, 1, rows // 2, rows - 1)], heads, 0, 0)

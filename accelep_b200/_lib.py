@@ -119,6 +119,7 @@ SIGNATURES = {
                                                         c_vp, c_i64, c_vp, c_sz, c_vp, ctypes.POINTER(L2Prefetch),
                                                         c_vp]),
     "accel_b200_attention_prefill_q8_workspace": (c_sz, [P_q8c, c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "accel_b200_attention_prefill_q8_tiles": (c_int, [P_q8c, c_i32, c_i32, c_i32, c_i32, c_i32]),
     "accel_b200_attention_prefill_q8": (c_int, [c_vp, c_i64, P_q8c, c_vp, c_vp, c_vp, c_i32, c_i32, c_i64, c_i32,
                                                 c_i32, c_i32, c_vp, c_i64, c_vp, c_sz, c_vp, c_vp]),
     "accel_b200_silu_mul_rows": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp]),

@@ -729,6 +729,13 @@ AttnArgs ArgsOf(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, 
   return a;
 }
 
+// Whether sizes are those of a prefill call that has something to do.
+bool PrefillSizes(const accel_b200_q8_cache* cache, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
+                  int32_t sinks, const char* what) {
+  return CheckQ8Cache(cache, what) == ACCEL_B200_OK && batch > 0 && max_rows > 0 && heads > 0 &&
+         heads % cache->kv_heads == 0 && window >= 0 && sinks >= 0;
+}
+
 int CheckAttention(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache, int32_t heads, int32_t window,
                    int32_t sinks, const float* out, int64_t out_ld, int64_t rows, const std::string& what) {
   const int rc = CheckQ8Cache(cache, what.c_str());
@@ -812,14 +819,19 @@ ACCEL_B200_API int accel_b200_attention_decode_q8(const float* q, int64_t q_ld, 
 ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200_q8_cache* cache, int32_t batch,
                                                                 int32_t max_rows, int32_t heads, int32_t window,
                                                                 int32_t sinks) {
-  if (CheckQ8Cache(cache, "attention_prefill_q8_workspace") != ACCEL_B200_OK || batch <= 0 || max_rows <= 0 ||
-      heads <= 0 || heads % cache->kv_heads != 0 || window < 0 || sinks < 0) {
-    return 0;
-  }
+  if (!PrefillSizes(cache, batch, max_rows, heads, window, sinks, "attention_prefill_q8_workspace")) return 0;
   max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));
   const TilesPlan tiles = PlanTilesQ8(*cache, batch, max_rows, heads, window, sinks);
   if (TakesTiles(*cache, batch, max_rows, heads, tiles)) return tiles.workspace;
   return SplitFor(*cache, batch, max_rows, heads, window, sinks, false).workspace;
+}
+
+ACCEL_B200_API int accel_b200_attention_prefill_q8_tiles(const accel_b200_q8_cache* cache, int32_t batch,
+                                                         int32_t max_rows, int32_t heads, int32_t window,
+                                                         int32_t sinks) {
+  if (!PrefillSizes(cache, batch, max_rows, heads, window, sinks, "attention_prefill_q8_tiles")) return 0;
+  max_rows = static_cast<int32_t>(Min64(max_rows, cache->context));
+  return TakesTiles(*cache, batch, max_rows, heads, PlanTilesQ8(*cache, batch, max_rows, heads, window, sinks)) ? 1 : 0;
 }
 
 ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,

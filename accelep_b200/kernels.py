@@ -541,6 +541,13 @@ def attention_prefill_q8_workspace(cache, batch, max_rows, heads, window=0, sink
     return torch.zeros(need, dtype=torch.uint8, device=cache.device) if need else None
 
 
+def attention_prefill_q8_tiles(cache, batch, max_rows, heads, window=0, sinks=0):
+    """Whether attention_prefill_q8 calls of these sizes take the tcgen05 tiles
+    (else the groups of 8 query vectors)."""
+    _counts(batch | max_rows | window | sinks)
+    return bool(load().accel_b200_attention_prefill_q8_tiles(cache._ref, batch, max_rows, heads, window, sinks))
+
+
 def attention_prefill_q8(q, cache, first, count, pos0, heads, max_rows, window=0, sinks=0, out=None, workspace=None,
                          status=None):
     """Causal attention of sequence b's rows first[b] .. + count[b] - 1 of q

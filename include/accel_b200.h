@@ -553,10 +553,15 @@ ACCEL_B200_API int accel_b200_attention_decode_q8_prefetch(
    every count) at positions pos0[b] + i of slot b, no row of two sequences; the
    cache already holds their keys and values. Sequences are skipped as by
    accel_b200_rope_append_q8 (a skipped sequence's output is not written).
-   Workspace as above. */
+   Workspace as above. accel_b200_attention_prefill_q8_tiles says which of its
+   two kernels a call of these sizes takes, for tests and profiles: 1 the
+   tcgen05 tiles, 0 the groups of 8 query vectors (or bad arguments). */
 ACCEL_B200_API size_t accel_b200_attention_prefill_q8_workspace(const accel_b200_q8_cache* cache, int32_t batch,
                                                                 int32_t max_rows, int32_t heads, int32_t window,
                                                                 int32_t sinks);
+ACCEL_B200_API int accel_b200_attention_prefill_q8_tiles(const accel_b200_q8_cache* cache, int32_t batch,
+                                                         int32_t max_rows, int32_t heads, int32_t window,
+                                                         int32_t sinks);
 ACCEL_B200_API int accel_b200_attention_prefill_q8(const float* q, int64_t q_ld, const accel_b200_q8_cache* cache,
                                                    const int32_t* first, const int32_t* count, const int32_t* pos0,
                                                    int32_t batch, int32_t max_rows, int64_t rows, int32_t heads,

@@ -182,3 +182,20 @@ def test_prefill_without_a_device_says_so(lib):
     for _ in range(2):
         assert prefill(lib, big, heads=16, ld=1024, out=1 << 34, out_ld=1024, max_rows=512) == 3
         assert b"CUDA" in lib.accel_b200_last_error() and b"registers" not in lib.accel_b200_last_error()
+
+
+def test_which_kernel_a_prefill_takes(lib):
+    """By sizes alone; bad sizes: 0."""
+    def tiles(c, batch, rows, heads, window=0, sinks=0):
+        return lib.accel_b200_attention_prefill_q8_tiles(c, batch, rows, heads, window, sinks)
+
+    c = cache()
+    assert tiles(c, 3, 100, 4) == 0  # 3 x 2 x 25 groups
+    assert tiles(c, 3, 100, 64) == 1  # 3 x 2 x 400
+    assert tiles(c, 3, 1 << 30, 64) == tiles(c, 3, 100, 64)  # a run is no longer than the context
+    long = cache(context=1 << 16, seq_stride=2 << 22, head_stride=1 << 22, scale_seq_stride=2048, scale_head_stride=1024,
+                 k=1 << 30, v=1 << 31, k_scale=1 << 32, v_scale=1 << 33)
+    assert tiles(long, 1, 4000, 8) == 1 and tiles(long, 1, 1, 8) == 0
+    for bad in ((0, 5, 4), (1, 0, 4), (1, 5, 3), (1, 5, 0), (1, 5, 4, -1), (1, 5, 4, 0, -1)):
+        assert tiles(c, *bad) == 0
+    assert tiles(None, 1, 5, 4) == 0 and tiles(cache(block=16), 3, 100, 64) == 0

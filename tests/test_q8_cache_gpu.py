@@ -843,3 +843,46 @@ def test_decode_balanced_over_as_many_rows_as_fit(lib, cuda, rows, heads, d, len
                                   workspace=ws))
     assert np.isfinite(got).all() and not H(ws)[:65536].any()
     check_rows(c, q, got, [(r, r, int(pos[r])) for r in (0, 1, rows // 2, rows - 1)], heads, 0, 0)
+
+
+LAYOUTS = [  # heads, kv heads, head_dim, block, positions, rows
+    (9, 3, 64, 64, [0, 37, 250], [200, 100, 50]),
+    (4, 4, 128, 32, [0, 1, 299, 100], [33, 65, 1, 0]),
+    (8, 1, 64, 128, [0, 60], [70, 129]),
+    (10, 2, 128, 64, [130], [17]),
+    (20, 1, 64, 32, [5, -1], [80, 4]),
+    (7, 7, 128, 128, [0, 5], [256, 40]),
+    (16, 2, 128, 64, [0, 3], [90, 77]),
+    (12, 4, 64, 32, [0, 1, 0], [1, 2, 150]),
+]
+
+
+@pytest.mark.parametrize("heads,kv,d,block,pos0,count", LAYOUTS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 2), (50, 4), (130, 1), (1000, 7)])
+@pytest.mark.parametrize("kernel", ["vectors", "tiles", "shared tiles"])
+def test_prefill_by_each_kernel(lib, cuda, heads, kv, d, block, pos0, count, window, sinks, kernel):
+    """Every layout by groups of 8 vectors, by tiles, and by tiles that may share
+    walks (max_rows and the context choose), and that it was that kernel."""
+    rng = np.random.default_rng(heads * 1000 + d + window + 1)
+    most, context = {"vectors": (max(count), 330), "tiles": (880, 880), "shared tiles": (1200, 1200)}[kernel]
+    c = filled(rng, len(pos0), kv, context, d, block)
+    dev = device_cache(c)
+    sizes = (len(pos0), most, heads, window, sinks)
+    assert K.attention_prefill_q8_tiles(dev, *sizes) == (kernel != "vectors")
+    if window == 0 and kernel != "vectors":
+        assert (K.attention_prefill_q8_workspace(dev, *sizes) is not None) == (kernel == "shared tiles")
+    first, rows = ragged(count), int(np.sum(count)) + 3
+    q = rng.standard_normal((rows, heads * d), dtype=np.float32)
+    out = torch.full((rows, heads * d), 7.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    K.attention_prefill_q8(T(q), dev, I(first), I(count), I(pos0), heads, most, window=window, sinks=sinks, out=out,
+                           status=status)
+    got = H(out)
+    assert H(status)[0] == 0 and (got[-3:] == 7.0).all()
+    todo = []
+    for b, (f, n, p) in enumerate(zip(first, count, pos0)):
+        if p >= 0:
+            todo += [(f + i, b, p + i) for i in sorted({*range(0, n, 13), n - 1, n - 2, 1, 31, 32, 63, 64}) if 0 <= i < n]
+        else:
+            assert (got[f:f + n] == 7.0).all()
+    check_rows(c, q, got, todo, heads, window, sinks)

@@ -37,8 +37,10 @@
 // instruction cache (-> 632); on the second: one half per CTA (80 -> 76), no 64-bit
 // divisions in any role and the first loads ahead of the set-up (-> 69).
 //
-// Every wait is bounded; one that runs out sets a flag that ends every role,
-// gives NaN and ORs ACCEL_B200_STATUS_COPY_TIMEOUT.
+// Every wait is bounded. A role whose wait runs out notes it and stops, and with
+// it stop, each at the end of a wait of its own, the roles that wait for its
+// work: a CTA ends after a few wait limits, gives NaN and ORs
+// ACCEL_B200_STATUS_COPY_TIMEOUT.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     return (w == 0 || second) && SeesSome(range, token_of(j), kTile, a.sinks);
   };
   volatile int32_t* failed = &bars.failed;
-  // A bounded wait; false, and every role's cue to stop, once any ran out.
+  // A bounded wait; false where it ran out, which the CTA reports as it ends.
   const auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (MbarWaitSleep(bar, parity)) return true;
     *failed = 1;

@@ -1,8 +1,8 @@
 // Bulk-copy (TMA) and mbarrier helpers in inline PTX for sm_100a.
 //
 // This header holds the untiled global -> shared bulk copy and the L2
-// prefetch; the tiled tensor-map copies (cp.async.bulk.tensor) of the
-// tensor-core product live in gemm_tc.cu. Every copy in this library has a
+// prefetch; the tiled tensor-map copies (cp.async.bulk.tensor) are those of
+// tensor_map.cuh (two-dimensional) and gemm_tc.cu (three-dimensional). Every copy in this library has a
 // CTA-local destination and no cluster multicast: it reads this GPU's own
 // memory into the issuing CTA's shared memory. Waits on an mbarrier are
 // bounded; a wait that runs out reports failure to its caller instead of

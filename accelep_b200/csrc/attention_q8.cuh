@@ -90,9 +90,12 @@ __device__ __forceinline__ int NearOf(int pos, int window) { return window > 0 ?
 // SM (attention_q8_tiles.cu).
 constexpr int kTileVectors = 256;
 
-// How a call would run there: the bytes of workspace that it takes, and for an
-// estimate of its time the waves of CTAs and the 128-token steps of a whole walk
-// (upper bounds: the device alone knows counts and positions).
+// How a call would run there: the bytes of workspace that it takes, and estimates
+// by which the kernel is chosen and shared walks are prepared, of the waves of
+// CTAs and the 128-token steps of a whole walk. The device alone knows counts and
+// positions: sequences shorter than the cache's context take fewer steps, and a
+// tile's walk through a window a few more (its own rows, and partly seen tiles at
+// the ends of window and sinks). Results do not depend on them.
 struct TilesPlan {
   bool split;  // the last wave's walks are shared by several CTAs
   double waves;

@@ -91,11 +91,10 @@ struct Tiles {
   static_assert(kMore % 8 == 0 && kSoftWarps * 32 * kMore + 256 * kLess <= kThreads * kLaunch, "");
   static constexpr int kPanels = D / 64;
   static constexpr int kOperand = kPanels * kPanel;     // a 128 x D fp16 operand
-  static constexpr int kStages = 1;                     // fp16 key and value tiles
   static constexpr int kQ = 0;                          // [half][hi, lo]
   static constexpr int kK = kQ + 2 * kHalves * kOperand;
-  static constexpr int kV = kK + kStages * kOperand;
-  static constexpr int kRaw = kV + kStages * kOperand;  // int8 tiles as they come: keys, values
+  static constexpr int kV = kK + kOperand;
+  static constexpr int kRaw = kV + kOperand;            // int8 tiles as they come: keys, values
   static constexpr int kRawBytes = kTile * D;
   static constexpr int kBars = kRaw + 2 * kRawBytes;
   static constexpr int kShared = kBars + 256;           // float [half][vector] and [2][half][part][vector]
@@ -111,8 +110,8 @@ struct Tiles {
 
 struct Bars {
   uint64_t raw_full[2];       // TMA -> converters (keys, values)
-  uint64_t full[2][2];        // converters -> MMA: fp16 keys, values by stage
-  uint64_t empty[2][2];       // MMA -> converters
+  uint64_t full[2];           // converters -> MMA: fp16 keys, values
+  uint64_t empty[2];          // MMA -> converters
   uint64_t queries[2];        // softmax -> MMA, by half
   uint64_t scores[2];         // MMA -> softmax
   uint64_t weights[2];        // softmax -> MMA
@@ -758,10 +757,8 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     if (ct == 0) {
       for (int i = 0; i < 2; ++i) {
         MbarInit(&bars.raw_full[i], 1);
-        for (int s = 0; s < 2; ++s) {
-          MbarInit(&bars.full[i][s], kConverters);
-          MbarInit(&bars.empty[i][s], 1);
-        }
+        MbarInit(&bars.full[i], kConverters);
+        MbarInit(&bars.empty[i], 1);
         MbarInit(&bars.queries[i], 4 * L::kParts);
         MbarInit(&bars.scores[i], 1);
         MbarInit(&bars.weights[i], 4 * L::kParts);
@@ -777,14 +774,12 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     bool ok = true;
     int fetched[2] = {0, 0};  // tiles read of each plane; the next is in flight
     for (int j = 0; j < n && ok; ++j) {
-      const int stage = j % L::kStages;
-      const uint32_t lap = static_cast<uint32_t>(j / L::kStages) & 1;
 #pragma unroll 1
       for (int plane = 0; plane < 2; ++plane) {
         if (!ok) break;  // all converters together
-        ok = wait(&bars.raw_full[plane], j & 1) && wait(&bars.empty[plane][stage], lap ^ 1);
+        ok = wait(&bars.raw_full[plane], j & 1) && wait(&bars.empty[plane], (j & 1) ^ 1);
         const char* src = smem + L::kRaw + plane * L::kRawBytes;
-        char* dst = smem + (plane == 0 ? L::kK : L::kV) + stage * L::kOperand;
+        char* dst = smem + (plane == 0 ? L::kK : L::kV);
         // 8 elements at a time. The threads are whole multiples of 8 rows, so a
         // thread's swizzle and piece stay the same from row to row.
         constexpr int kPieces = D / 8, kStep = kConverters * 32 / kPieces;  // pieces of a row, rows per pass
@@ -807,7 +802,7 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
         }
         FenceProxyAsyncSmem();
         __syncwarp();
-        if (lane == 0) MbarArrive(&bars.full[plane][stage]);
+        if (lane == 0) MbarArrive(&bars.full[plane]);
         // Every converter has read the int8 tile: its bytes take the next one.
         // One whose wait ran out takes all of them out of the loop together.
         ok = !MeetAny(1, kConverters * 32, !ok);
@@ -830,28 +825,28 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
     if (warp == L::kMmaWarp && ElectOne()) {
       constexpr uint32_t kQkDesc = InstrDescF16(kTile, false), kPvDesc = InstrDescF16(D, true);
       const uint32_t q_at = SmemAddr(smem + L::kQ), k_at = SmemAddr(smem + L::kK), v_at = SmemAddr(smem + L::kV);
-      const auto scores = [&](int w, int stage) {
+      const auto scores = [&](int w) {
         // The small parts' products first: fewer roundings at full size.
 #pragma unroll 1
         for (int part = 1; part >= 0; --part) {
-          const uint32_t qa = q_at + (w * 2 + part) * L::kOperand, kb = k_at + stage * L::kOperand;
+          const uint32_t qa = q_at + (w * 2 + part) * L::kOperand;
 #pragma unroll
           for (int s = 0; s < D / 16; ++s) {
             const uint32_t at = (s / 4) * kPanel + (s % 4) * 32;  // 16 elements along the swizzled row
-            MmaF16(tmem + L::kScores + w * kTile, SmemDescSw128(qa + at, 16, 1024), SmemDescSw128(kb + at, 16, 1024),
+            MmaF16(tmem + L::kScores + w * kTile, SmemDescSw128(qa + at, 16, 1024), SmemDescSw128(k_at + at, 16, 1024),
                    kQkDesc, part == 0 || s > 0);
           }
         }
         MmaCommit(&bars.scores[w]);
       };
       // Weighted values of tokens 16 s0 .. 16 (s0 + kSteps) - 1 of the tile.
-      const auto values = [&](int w, int stage, int s0, auto steps) {
+      const auto values = [&](int w, int s0, auto steps) {
         constexpr int kSteps = decltype(steps)::value;
 #pragma unroll 1
         for (int part = 1; part >= 0; --part) {
           // A step: 16 tokens, 8 columns of weights, 16 rows of values.
           const uint32_t pa = tmem + L::kScores + w * kTile + part * 8 + s0 * 16;
-          const uint32_t vb = v_at + stage * L::kOperand + s0 * 2048;
+          const uint32_t vb = v_at + s0 * 2048;
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             MmaF16FromTmem(tmem + L::kOut + w * D, pa + s * 16, SmemDescSw128(vb + s * 2048, kPanel, 1024), kPvDesc,
@@ -866,24 +861,24 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
       // Scores of tile j for half w, once the half's queries and the keys are there.
       const auto next_scores = [&](int w, int j) {
         if (!ok || !needed(w == 0 ? range0 : range1, w, j)) return;
-        ok = wait(&bars.queries[w], 0) && wait(&bars.full[0][j % L::kStages], (j / L::kStages) & 1);
+        ok = wait(&bars.queries[w], 0) && wait(&bars.full[0], j & 1);
         if (!ok) return;
         TcFenceAfterSync();
-        scores(w, j % L::kStages);
+        scores(w);
       };
       next_scores(0, 0);
       if (L::kHalves > 1) next_scores(1, 0);
-      if (ok) MmaCommit(&bars.empty[0][0]);
+      if (ok) MmaCommit(&bars.empty[0]);
       for (int j = 0; j < n && ok; ++j) {
 #pragma unroll
         for (int w = 0; w < L::kHalves; ++w) {
           if (ok && needed(w == 0 ? range0 : range1, w, j)) {
-            ok = wait(&bars.weights[w], done[w] & 1) && wait(&bars.full[1][j % L::kStages], (j / L::kStages) & 1);
+            ok = wait(&bars.weights[w], done[w] & 1) && wait(&bars.full[1], j & 1);
             if (!ok) continue;
             ++done[w];
             TcFenceAfterSync();
             if (*reinterpret_cast<volatile int32_t*>(&bars.apart[w]) == 0) {
-              values(w, j % L::kStages, 0, std::integral_constant<int, kTile / 16>{});
+              values(w, 0, std::integral_constant<int, kTile / 16>{});
             } else {
               for (int k = 0; k < kChunks && ok; ++k) {
                 if (k > 0) {
@@ -892,16 +887,16 @@ __global__ void __launch_bounds__(Tiles<D>::kThreads, Tiles<D>::kCtas)
                   ++done[w];
                   TcFenceAfterSync();
                 }
-                values(w, j % L::kStages, k * (kChunk / 16), std::integral_constant<int, kChunk / 16>{});
+                values(w, k * (kChunk / 16), std::integral_constant<int, kChunk / 16>{});
               }
             }
           }
           // The values are free before the next scores are.
-          if (ok && w == L::kHalves - 1) MmaCommit(&bars.empty[1][j % L::kStages]);
+          if (ok && w == L::kHalves - 1) MmaCommit(&bars.empty[1]);
           if (j + 1 < n) next_scores(w, j + 1);
         }
         if (!ok) break;
-        if (j + 1 < n) MmaCommit(&bars.empty[0][(j + 1) % L::kStages]);
+        if (j + 1 < n) MmaCommit(&bars.empty[0]);
       }
       if (!ok) {
         // After a failure: what was issued ends before the TMEM is freed (bounded).

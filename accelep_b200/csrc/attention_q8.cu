@@ -23,7 +23,7 @@
 // value scale, to fp32 registers (the tensor core's running sum rounds towards
 // zero, which would drift over a long context). Bound by HBM on long sequences:
 // 4 of 40001 to 65536 tokens, 8 kv heads of 128, take 77 us, 5.6 TB/s with inputs
-// that no cache holds. Before the split by lengths it took 88 us, with loads to
+// that no cache holds, in a captured graph (87 called one by one). Before the split by lengths it took 88 us, with loads to
 // registers 128 and with per-lane cp.async 132: an SM keeps too few of those in
 // flight. Short calls are a chain of latencies, so what needs no division has none.
 //
@@ -638,7 +638,9 @@ Split SplitFor(const accel_b200_q8_cache& c, int64_t runs, int64_t rows_per_run,
   // grid has room for a CTA more per row and pair. (Measured with 8 kv heads
   // of 128: 16 sequences of 2048..16384 tokens 91 -> 61 us, of 4096..32768 178
   // -> 127; where all have the same length the states' way through the
-  // workspace instead of the cluster costs 3 us of 51 to 97.)
+  // workspace instead of the cluster costs 3 us of 51 to 97. A lane counts a row,
+  // and a CTA serves one row and pair: beyond either limit the longest row's CTA
+  // sets the time, 18 sequences of 2048..16384 tokens 78 us, 19 of them 142.)
   const bool few = single && runs <= 32 && p.groups <= resident / 2;
   if (few && (s > kMaxCluster || seen >= kBalanceFrom)) p.balanced = static_cast<int>(resident);
   if (s > kMaxCluster || p.balanced > 0) {
@@ -698,7 +700,10 @@ int CheckWorkspace(size_t need, const void* workspace, size_t bytes, const std::
 // sequences of 16 rows 42 and 32 us, of 32 rows 51 and 65, 32 of 16 rows 147 and 214;
 // behind 5000: 4 of 32 rows 26 and 19, of 64 rows 30 and 43. 8 kv heads of 128, 32
 // heads, behind 16000: 1 of 32 rows 42 and 33, of 64 rows 90 and 142, 32 of 8 rows 681
-// and 451, of 16 rows 711 and 735; behind 300, unsplit: 32 of 8 rows 35 and 42.)
+// and 451, of 16 rows 711 and 735; behind 300, unsplit: 32 of 8 rows 35 and 42. All of
+// them in caches that they fill: the plan goes by the context, so that 64 rows behind
+// 300 tokens of 16384 take tiles, 23 us, whose walks are then too short to be shared,
+// where in a cache of 2048 the groups take 7.)
 constexpr double kTileGroups = 900, kSplitGroupSteps = 9000;
 bool TakesTiles(const accel_b200_q8_cache& c, int64_t batch, int64_t max_rows, int32_t heads, const TilesPlan& plan) {
   const int64_t groups = batch * c.kv_heads * CeilDiv(max_rows * (heads / c.kv_heads), kVec);

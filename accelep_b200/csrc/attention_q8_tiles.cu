@@ -23,19 +23,20 @@
 // TMA brings into fp16 operands with the 128-byte swizzle; one thread of the
 // next issues every MMA.
 //
-// Measured: 2 sequences of 2047 and fewer rows behind 14000 tokens, 32 heads over
-// 8 kv heads of 128, window 4096: 489 us, 489 TFLOP/s of scores and values (twice
-// that in fp16 products). A half's chain (weights 2600 cycles, its four products
+// Measured (in a captured graph; called one by one 528 and 63): 2 sequences of 2047
+// and fewer rows behind 14000 tokens, 32 heads over 8 kv heads of 128, window 4096:
+// 487 us, 490 TFLOP/s of scores and values (twice that in fp16 products). A half's chain (weights 2600 cycles, its four products
 // 2800, maximum 900, read-out 500) and the other's overlap to 7000 cycles a tile,
 // of which the tensor core works 5600: an M = 128, N = 128, K = 16 product takes
 // 102 cycles with A in shared memory, 72 from TMEM. 32 sequences of 512 rows, 9
-// heads over 3 of 64: 69 us, by issue slots (55% of them used) and the first and
+// heads over 3 of 64: 63 us, by issue slots (55% of them used) and the first and
 // last steps of short walks (13000 of a four-tile CTA's 39000 cycles). What brought
 // it there, on the first of these: one elected thread instead of lane 0 issuing
 // (1617 -> 1250 us), values freed in front of the next scores and four converter
 // warps (-> 806), chunk loops kept rolled so that their code stays in the
 // instruction cache (-> 632); on the second: one half per CTA (80 -> 76), no 64-bit
-// divisions in any role and the first loads ahead of the set-up (-> 69).
+// divisions in any role and the first loads ahead of the set-up (-> 69), the longest
+// walks first (-> 63). ptxas reports spills (72 to 172 bytes of stores).
 //
 // Every wait is bounded. A role whose wait runs out notes it and stops, and with
 // it stop, each at the end of a wait of its own, the roles that wait for its
@@ -920,7 +921,8 @@ int64_t MostTiles(const accel_b200_q8_cache& c, int64_t max_rows, int32_t heads)
   return CeilDiv(max_rows * (heads / c.kv_heads), Tiles<D>::kHalves * kHalf);
 }
 
-// The last wave's walks are split in calls of few waves and of walks long enough.
+// The last wave's walks are split in calls of few waves and of walks long enough,
+// and of 32 sequences at most (a lane counts each; more of them go a CTA per tile).
 template <int D>
 TilesPlan Plan(const accel_b200_q8_cache& c, int32_t batch, int32_t max_rows, int32_t heads, int32_t window,
                int32_t sinks) {

@@ -2,11 +2,11 @@
 //
 // This header holds the untiled global -> shared bulk copy and the L2
 // prefetch; the tiled tensor-map copies (cp.async.bulk.tensor) are those of
-// tensor_map.cuh (two-dimensional) and gemm_tc.cu (three-dimensional). Every copy in this library has a
-// CTA-local destination and no cluster multicast: it reads this GPU's own
-// memory into the issuing CTA's shared memory. Waits on an mbarrier are
-// bounded; a wait that runs out reports failure to its caller instead of
-// spinning on.
+// tensor_map.cuh (two-dimensional) and gemm_tc.cu (three-dimensional). Every
+// copy in this library has a CTA-local destination and no cluster multicast: it
+// reads this GPU's own memory into the issuing CTA's shared memory. Waits on an
+// mbarrier are bounded; a wait that runs out reports failure to its caller
+// instead of spinning on.
 #pragma once
 
 #include <cuda_runtime.h>
